@@ -214,6 +214,110 @@ int lc_attn_bwd_shard_ws(const lc_attn_shape_t* shape, const lc_attn_mask_t* mas
                          const float* delta, float* dq_acc, float* dk_acc, float* dv_acc,
                          void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- operators on a KV cache ------------------------------------------------- */
+
+/* A batch of KV caches and the new tokens that look at them.  No counterpart in
+ * the reference, which keeps no cache (distributed_infer.py:185-219).  Row j of
+ * sequence b and KV head h starts at element
+ *   b * seq_stride + j * row_stride + h * head_stride
+ * of both K and V (head_dim elements, contiguous), so [B, C, Hkv, D] and
+ * [B, Hkv, C, D] caches and slices of larger ones are all described.  Strides
+ * are multiples of 16 bytes, K and V 16-byte aligned, row_stride <= 2^24.
+ * past[b] (int32, device) rows of sequence b hold earlier tokens, in any order;
+ * the new tokens' K and V are in rows past[b] .. past[b] + tokens - 1, where
+ * the caller has put them.  A new token whose row lies at or past capacity is
+ * not there, and with past[b] < 0 no token of sequence b is (a batch slot
+ * without a sequence); past[b] > capacity counts as capacity.
+ * parents [B, tokens] (int32, device) makes the new tokens a tree (drafted
+ * continuations): parents[i] = -1 hangs token i off the past, p < i off token
+ * p.  Any other value, or a chain of parents that meets one, means that the
+ * token is not there (padding of a smaller tree).  A token sees the past, its
+ * chain of parents and itself; NULL is the chain (each token sees those before
+ * it).  Neither the kernels nor the host reads other rows of the cache. */
+typedef struct lc_cache {
+  int32_t batch;    /* B */
+  int32_t tokens;   /* new tokens of each sequence */
+  int32_t capacity; /* C, rows of each sequence */
+  int32_t heads_q;  /* a multiple of heads_kv */
+  int32_t heads_kv;
+  int32_t head_dim; /* a multiple of 16, <= 256 */
+  int32_t dtype;    /* enum lc_dtype of q, k, v and the output */
+  uint32_t flags;   /* LC_FLAG_PRECISE */
+  int64_t seq_stride;
+  int64_t row_stride;
+  int64_t head_stride;
+} lc_cache_t;
+
+/* Attention of the new tokens over the cache (at most LC_CACHE_MAX_TOKENS of
+ * them): out [B, tokens, heads_q, head_dim] in dtype, and, where the pointers
+ * are set, the statistics m and l [B, heads_q, tokens] fp32 of
+ * lc_attn_fwd_shard; q is contiguous like out.  A token that is not there has
+ * out = 0, m = -inf, l = 0.  The past is attended to by split-KV kernels whose
+ * partials lie in the workspace (lc_cache_attn_workspace_bytes, 16-byte
+ * aligned); a second kernel merges them with the token's own chain, which it
+ * computes in fp32.  What a token does not see never enters its result, not
+ * even as a product with zero: infinities and NaN stay where they are.
+ * Calls that overlap need a workspace each. */
+#define LC_CACHE_MAX_TOKENS 256
+size_t lc_cache_attn_workspace_bytes(const lc_cache_t* cache);
+int lc_cache_attn(const lc_cache_t* cache, const int32_t* past, const int32_t* parents,
+                  const void* q, const void* k, const void* v, void* out, float* m, float* l,
+                  void* workspace, size_t workspace_bytes, void* stream);
+
+/* The attention weight that each row of the cache receives from the new
+ * tokens: with the statistics m and l of lc_cache_attn (or of a forward over the
+ * same rows),
+ *   w[h][j] = sum over the query rows of KV head h that see row j of
+ *             exp(s - m) / l
+ * (a query row with l = 0 or m = -inf gives nothing), added to what was
+ * accumulated before:
+ *   weights_out[b][h][j] = weights[b][h][j] + w[h][j]   (j < past[b])
+ *   weights_out[b][h][j] = w[h][j]                      (a new token's own row)
+ * weights (NULL: zeros) and weights_out are [B, heads_kv, capacity] fp32 and
+ * may be the same; rows behind the new tokens, and a sequence with past < 0,
+ * stay as they are.  Sums are fp32 in a fixed order.  tokens is limited to
+ * LC_CACHE_MAX_TOKENS with parents only (a whole prompt is one chain). */
+int lc_cache_weights(const lc_cache_t* cache, const int32_t* past, const int32_t* parents,
+                     const void* q, const void* k, const float* m, const float* l,
+                     const float* weights, float* weights_out, void* stream);
+
+/* Cuts each sequence's cache to budget rows per KV head, by accumulated weight.
+ * Of the lens[b] rows a head holds (clipped to [0, capacity]) it keeps those
+ * with a position < sinks, those with a position >= ends[b] - recent, then the
+ * rows of the largest weight; equal ones by the lowest row, NaN weights last.
+ * (More protected rows than budget: the lowest rows of them.)  With lens[b] <=
+ * budget every row stays.
+ * Rows move in place: kept rows below budget stay, and the j-th row below
+ * budget that goes is overwritten by the j-th kept row from budget on, in K, V,
+ * weights and positions.  The head then holds rows 0 .. lens_out[b] - 1, in no
+ * order; K and V rows from there on stay as they are.
+ * Positions: row j < kept[b] (rows of an earlier eviction) is at
+ * positions[b][h][j]; the rows from there on were appended one by one, the last
+ * at ends[b] - 1.  kept NULL: 0; ends NULL: lens; positions may be NULL where
+ * kept is.
+ * weights, positions and their outputs are [B, heads_kv, capacity] fp32 and
+ * int32; an output may be its input, and rows from lens_out[b] on are not
+ * written.  lens_out [B] must not overlap another array.
+ * Reads batch, capacity, heads_kv, head_dim, dtype and the strides of cache;
+ * no two rows of it may overlap. */
+size_t lc_cache_evict_workspace_bytes(const lc_cache_t* cache);
+int lc_cache_evict(const lc_cache_t* cache, int32_t budget, int32_t sinks, int32_t recent,
+                   const int32_t* lens, const int32_t* kept, const int32_t* ends, void* k, void* v,
+                   const float* weights, const int32_t* positions, float* weights_out,
+                   int32_t* positions_out, int32_t* lens_out, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/* Makes an accepted path of the tree the continuation of every layer's cache:
+ * path [B, tokens] (int32, device) holds node numbers in ascending order, and
+ * K and V row past[b] + path[b][j] moves to past[b] + j, for each of `layers`
+ * caches of the same shape (host arrays of device pointers).  The path ends at
+ * the first entry that is not above the one before it (>= 0 the first) or whose
+ * row lies past the capacity, e.g. at a -1.  lens_out[b] = past[b] + the path's
+ * length; a sequence with past < 0 keeps it.  lens_out must not overlap past or
+ * path.  Here tokens is the path's length, and heads_q is not read. */
+int lc_cache_commit(const lc_cache_t* cache, int32_t layers, void* const* ks, void* const* vs,
+                    const int32_t* past, const int32_t* path, int32_t* lens_out, void* stream);
+
 /* ---- emulated ring (one GPU, ordered loop over KV shards in HBM) ------------ */
 
 /* Ring geometry: world equal shards of local_tokens tokens. */

@@ -25,6 +25,7 @@ LC_ERR_UNSUPPORTED = 3
 LC_ERR_WORKSPACE = 4
 
 LC_DECODE_STATIC_SCRATCH_BYTES = 16 << 20
+LC_CACHE_MAX_TOKENS = 256
 
 
 class Shape(ctypes.Structure):
@@ -47,6 +48,22 @@ class Mask(ctypes.Structure):
         ("valid_length", c_int64),
         ("causal", c_int32),
         ("reserved", c_int32),
+    ]
+
+
+class Cache(ctypes.Structure):
+    _fields_ = [
+        ("batch", c_int32),
+        ("tokens", c_int32),
+        ("capacity", c_int32),
+        ("heads_q", c_int32),
+        ("heads_kv", c_int32),
+        ("head_dim", c_int32),
+        ("dtype", c_int32),
+        ("flags", c_uint32),
+        ("seq_stride", c_int64),
+        ("row_stride", c_int64),
+        ("head_stride", c_int64),
     ]
 
 
@@ -104,7 +121,7 @@ class GemvFused(ctypes.Structure):
 
 
 _vpp = POINTER(c_void_p)
-_S, _M, _R = POINTER(Shape), POINTER(Mask), POINTER(RingDesc)
+_S, _M, _R, _C = POINTER(Shape), POINTER(Mask), POINTER(RingDesc), POINTER(Cache)
 
 # name -> (restype, argtypes); exactly the entry points the header declares.
 SIGNATURES = {
@@ -130,6 +147,14 @@ SIGNATURES = {
     "lc_attn_bwd_shard_ws": (c_int, [_S, _M, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                      c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
                                      c_void_p]),
+    "lc_cache_attn_workspace_bytes": (c_size_t, [_C]),
+    "lc_cache_attn": (c_int, [_C, *[c_void_p] * 9, c_size_t, c_void_p]),
+    "lc_cache_weights": (c_int, [_C, *[c_void_p] * 9]),
+    "lc_cache_evict_workspace_bytes": (c_size_t, [_C]),
+    "lc_cache_evict": (c_int, [_C, c_int32, c_int32, c_int32, *[c_void_p] * 11, c_size_t,
+                               c_void_p]),
+    "lc_cache_commit": (c_int, [_C, c_int32, _vpp, _vpp, c_void_p, c_void_p, c_void_p,
+                                c_void_p]),
     "lc_ring_fwd_workspace_bytes": (c_size_t, [_R]),
     "lc_ring_bwd_workspace_bytes": (c_size_t, [_R]),
     "lc_ring_bwd_ds_workspace_bytes": (c_size_t, [_R]),
