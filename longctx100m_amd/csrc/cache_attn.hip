@@ -20,9 +20,12 @@
 #include "common.h"
 #include "cache.h"
 #include "kernels.h"
+#include "stream_tile.h"
+#include "tile128.h"
 #include "tile32.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace lc {
 namespace {
@@ -231,6 +234,414 @@ __global__ __launch_bounds__(256) void cache_prefix32_kernel(AttnArgs a) {
   }
 }
 
+// -------------------------------------------- the past, bf16, up to 32 rows --
+
+// Few query rows: bound by the stream of the cache.  Every wave holds all of
+// the workgroup's 16 * NB rows (Q^T in registers, the B operand) and takes its
+// own 8 KB tiles of K, straight into registers as the A operand of S^T = K Q^T,
+// and of V, through LDS for the transposed reads of O^T += V^T P^T; both one
+// tile ahead and non-temporal.  The W waves of a workgroup take the tiles of
+// their split in turn and meet in LDS.
+template <int D, int NB, int W>
+__global__ __launch_bounds__(64 * W, NB * W == 1 ? 1 : 2) void cache_stream_kernel(AttnArgs a) {
+  using C = DecodeTile<D>;
+  constexpr int TK = C::TK, MB = C::MB, KS = C::KS, DB = C::DB;
+  constexpr int kRows = 16 * NB;
+  constexpr int kStages = 2;
+  constexpr int kPitch = D + 4;  // floats per row of a wave's partial
+  constexpr int kVBytes = W * kStages * kTileBytes;
+  constexpr int kPartBytes = W > 1 ? W * kRows * kPitch * 4 : 0;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[kVBytes > kPartBytes ? kVBytes : kPartBytes];
+  __shared__ float msm[W][kRows], lsm[W][kRows];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int slot = blockIdx.x / a.units;
+  const int unit = blockIdx.x - slot * a.units;
+  const int hk = unit % a.Hkv;
+  const int rb = unit / a.Hkv;
+  Share s;
+  if (!share_of(a, slot, s)) return;  // the whole workgroup
+
+  const uint16_t* kbase = static_cast<const uint16_t*>(a.k) + s.b * a.seq + hk * a.head;
+  const uint16_t* vbase = static_cast<const uint16_t*>(a.v) + s.b * a.seq + hk * a.head;
+  const int kb0 = s.k0 + wave * TK;
+  const int ntiles = s.k1 > kb0 ? (s.k1 - kb0 + W * TK - 1) / (W * TK) : 0;
+
+  VTile<D> ld;
+  ld.init(a.row, lane);
+  const uint32_t vlds = t128::lds_addr(smem) + wave * kStages * kTileBytes;
+  const uint8_t* vmem = smem + wave * kStages * kTileBytes;
+  auto issue = [&](int j) {  // V tile j into stage j % kStages
+    ld.load(vbase, a.row, kb0 + j * (W * TK), s.k1, vlds + (j % kStages) * kTileBytes, lane);
+  };
+  auto kload = [&](int j, bf16x8 (&kr)[MB][KS]) {  // lane (c, g): key 16 mb + c, dims 32 kk + 8 g
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+      const int row = min(kb0 + j * (W * TK) + 16 * mb + c, s.k1 - 1);
+#pragma unroll
+      for (int kk = 0; kk < KS; ++kk)
+        kr[mb][kk] = __builtin_nontemporal_load(
+            reinterpret_cast<const bf16x8*>(kbase + row * a.row + 32 * kk + 8 * g));
+    }
+  };
+
+  bf16x8 kra[MB][KS], krb[MB][KS];
+  if (ntiles > 0) {
+    issue(0);
+    kload(0, kra);
+  }
+  bf16x8 qreg[NB][KS];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const int r = rb * kRows + 16 * nb + c, rr = r < a.R ? r : 0;
+    const int64_t qi = ((int64_t)s.b * a.N + rr / a.group) * a.Hq + hk * a.group + rr % a.group;
+    const uint16_t* qrow = static_cast<const uint16_t*>(a.q) + qi * D;
+#pragma unroll
+    for (int kk = 0; kk < KS; ++kk) {
+      qreg[nb][kk] = *reinterpret_cast<const bf16x8*>(qrow + 32 * kk + 8 * g);
+      if (r >= a.R) qreg[nb][kk] = bf16x8{};
+    }
+  }
+  t128::wait_vmem();  // Q is there (the compiler cannot count the tile loads below)
+
+  int voff[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) voff[db] = VTile<D>::tr_off(16 * db, lane);
+  f32x4 o[NB][DB];
+  float mrow[NB], lsum[NB];  // running maximum (log2 units), lane-partial sum of p
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db) o[nb][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+    mrow[nb] = -INFINITY;
+    lsum[nb] = 0.f;
+  }
+
+  // Tile j: wait for V(j) and K(j) (issued at tile j - 1), issue V(j + 1) into
+  // the stage that tile j - 1 is done with and K(j + 1) into the other
+  // registers, then compute.
+  auto tile = [&](int j, bf16x8 (&kc)[MB][KS], bf16x8 (&kn)[MB][KS]) {
+    t128::wait_vmem();
+    if (j + 1 < ntiles) {
+      issue(j + 1);
+      kload(j + 1, kn);
+    }
+    const uint8_t* vt = vmem + (j % kStages) * kTileBytes;
+    const int left = s.k1 - (kb0 + j * (W * TK));  // keys of the split from this tile on
+    f32x4 sc[NB][MB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) sc[nb][mb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int kk = 0; kk < KS; ++kk)
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) sc[nb][mb] = mfma16x16x32(kc[mb][kk], qreg[nb][kk], sc[nb][mb]);
+    if (left < TK) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (16 * mb + 4 * g + i >= left) sc[nb][mb][i] = -INFINITY;
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[nb][mb][i]);
+      mx = group4_max(mx) * a.sl2;
+      if (mx > mrow[nb]) {
+        const float up = fast_exp2(mrow[nb] - mx);  // mrow = -inf: 0
+        lsum[nb] *= up;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) o[nb][db] *= up;
+        mrow[nb] = mx;
+      }
+      const float muse = mrow[nb] == -INFINITY ? 0.f : mrow[nb];
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p = fast_exp2(fmaf(sc[nb][mb][i], a.sl2, -muse));
+          lsum[nb] += p;
+          sc[nb][mb][i] = p;
+        }
+    }
+#pragma unroll
+    for (int k2 = 0; k2 < TK / 32; ++k2) {
+      bf16x8 pb[NB];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) pb[nb] = pack_bf16x8(sc[nb][2 * k2], sc[nb][2 * k2 + 1]);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        const uint8_t* p = vt + voff[db] + 32 * k2 * 2 * D;
+        const bf16x8 va = concat_bf16x4(t128::ds_read_tr(p), t128::ds_read_tr(p + 16 * 2 * D));
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) o[nb][db] = mfma16x16x32(va, pb[nb], o[nb][db]);
+      }
+    }
+  };
+  for (int j = 0; j < ntiles; j += 2) {
+    tile(j, kra, krb);
+    if (j + 1 < ntiles) tile(j + 1, krb, kra);
+  }
+
+  const int64_t prow0 = (int64_t)slot * a.N * a.Hq + hk * a.group;
+  auto emit = [&](int r, int d, const f32x4& acc, float L, float M) {
+    const int64_t pr = prow0 + (int64_t)(r / a.group) * a.Hq + r % a.group;
+    *reinterpret_cast<f32x4*>(a.po + pr * D + d) = acc;
+    if (d == 0) {
+      a.pm[pr] = M;
+      a.pl[pr] = L;
+    }
+  };
+  if constexpr (W == 1) {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const float L = group4_sum(lsum[nb]);
+      const int r = rb * kRows + 16 * nb + c;
+      if (r < a.R)
+#pragma unroll
+        for (int db = 0; db < DB; ++db) emit(r, 16 * db + 4 * g, o[nb][db], L, mrow[nb]);
+    }
+    return;
+  }
+  // The waves' partials, brought to each row's maximum, meet in LDS.
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+    if (g == 0) msm[wave][16 * nb + c] = mrow[nb];
+  __syncthreads();  // also: every wave is done with its V tiles
+  float* part = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < W; ++w) M = fmaxf(M, msm[w][16 * nb + c]);
+    const float f = mrow[nb] == -INFINITY ? 0.f : fast_exp2(mrow[nb] - M);
+    const float lt = group4_sum(lsum[nb]) * f;
+    if (g == 0) lsm[wave][16 * nb + c] = lt;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+      *reinterpret_cast<f32x4*>(part + (wave * kRows + 16 * nb + c) * kPitch + 16 * db + 4 * g) = o[nb][db] * f;
+  }
+  __syncthreads();
+  constexpr int kPer = D / 4;  // threads per row
+  for (int it = threadIdx.x; it < kRows * kPer; it += 64 * W) {
+    const int rr = it / kPer, d = 4 * (it % kPer);
+    const int r = rb * kRows + rr;
+    if (r >= a.R) break;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    float L = 0.f, M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      acc += *reinterpret_cast<const f32x4*>(part + (w * kRows + rr) * kPitch + d);
+      L += lsm[w][rr];
+      M = fmaxf(M, msm[w][rr]);
+    }
+    emit(r, d, acc, L, M);
+  }
+}
+
+// ------------------------------------- the past, bf16, head_dim 128, 33+ rows --
+
+// Many query rows: the matrix cores and the softmax beside them bound it.
+// Workgroup = NW waves x 32 rows that share 64-key tiles of K and V in LDS
+// (tile128.h), filled by LDS DMA; S^T = K Q^T and O^T += V^T P^T on 32 x 32 x 16
+// products.  Iteration j issues the products of S^T for tile j + 1 and beside
+// them, on the VALU, the softmax of tile j, then O^T += V_j^T P_j^T; K runs one
+// tile ahead of V, two buffers each, one barrier per tile.  A row's reference
+// maximum is only raised by more than 2^kSlack, so rescaling is rare; the true
+// one is tracked beside it.
+template <int NW, bool NT>
+__global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void cache_tile128_kernel(AttnArgs a) {
+  constexpr int D = 128, BN = 64;
+  constexpr int kTileB = BN * t128::kRowBytes;
+  constexpr float kSlack = 8.f;  // log2 units
+  __shared__ __attribute__((aligned(1024))) uint8_t kbuf[2][kTileB];
+  __shared__ __attribute__((aligned(1024))) uint8_t vbuf[2][kTileB];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kc = lane & 31;  // this lane's row within the wave
+  const int hh = lane >> 5;  // which half of each 8-key group the lane holds
+  const int slot = blockIdx.x / a.units;
+  const int unit = blockIdx.x - slot * a.units;
+  const int hk = unit % a.Hkv;
+  const int rb = unit / a.Hkv;
+  Share s;
+  if (!share_of(a, slot, s)) return;  // the whole workgroup
+
+  const uint16_t* kbase = static_cast<const uint16_t*>(a.k) + s.b * a.seq + hk * a.head;
+  const uint16_t* vbase = static_cast<const uint16_t*>(a.v) + s.b * a.seq + hk * a.head;
+  const int ntiles = (s.k1 - s.k0 + BN - 1) / BN;
+  const int r = 32 * (rb * NW + wave) + kc;
+
+  t128::RowLoader<BN, NW> ld;
+  ld.init(a.row, wave, lane);
+  auto load = [&](const uint16_t* base, int j, uint32_t lds) {
+    ld.template load<false, NT>(base, a.row, s.k0 + j * BN, s.k1, lds, wave, lane);
+  };
+  if (ntiles > 0) {
+    load(kbase, 0, t128::lds_addr(kbuf));
+    load(vbase, 0, t128::lds_addr(vbuf));
+  }
+  if (ntiles > 1) load(kbase, 1, t128::lds_addr(kbuf) + kTileB);
+
+  bf16x8 qreg[D / 16];  // lane: row r, dims 16 t + 8 hh .. + 7
+  {
+    const int rr = r < a.R ? r : 0;
+    const int64_t qi = ((int64_t)s.b * a.N + rr / a.group) * a.Hq + hk * a.group + rr % a.group;
+    const uint16_t* qrow = static_cast<const uint16_t*>(a.q) + qi * D;
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) qreg[t] = *reinterpret_cast<const bf16x8*>(qrow + 16 * t + 8 * hh);
+  }
+  const int roff0 = t128::row_chunk_off(kc, hh);
+  const int toff0 = t128::tr32_off(0, lane), toff1 = t128::tr32_off(1, lane);
+  int koff[8], voff0[4], voff1[4];
+#pragma unroll
+  for (int t = 0; t < 8; ++t) koff[t] = opaque(roff0 ^ (32 * t));
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    voff0[u] = opaque(toff0 ^ (64 * u));
+    voff1[u] = opaque(toff1 ^ (64 * u));
+  }
+  f32x16 o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = f32x16{};
+  float mrun = -INFINITY, mtrue = -INFINITY;  // log2 units, shared by the lanes l, l ^ 32
+  float lsum = 0.f;                           // lane-partial, relative to mrun
+
+  auto kread = [&](const uint8_t* kt, int i) {  // S step i: t = i / 2, mb = i % 2
+    return *reinterpret_cast<const bf16x8*>(kt + koff[i >> 1] + (i & 1) * 32 * t128::kRowBytes);
+  };
+  auto vread = [&](const uint8_t* vt, int i) {  // PV step i: u = i / 4, dims 32 (i % 4) ..
+    const int o0 = voff0[i & 3] + (i >> 2) * 16 * t128::kRowBytes;
+    const int o1 = voff1[i & 3] + (i >> 2) * 16 * t128::kRowBytes;
+    return concat_bf16x4(t128::ds_read_tr(vt + o0), t128::ds_read_tr(vt + o1));
+  };
+  auto scores_only = [&](const uint8_t* kt, f32x16 (&x)[2]) {
+    bf16x8 A[2] = {kread(kt, 0), kread(kt, 1)};
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      x[i & 1] = mfma32x32x16(A[i & 1], qreg[i >> 1], i < 2 ? f32x16{} : x[i & 1]);
+      if (i + 2 < 16) A[i & 1] = kread(kt, i + 2);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // left: keys of the split from this tile on (read on its last tile alone).
+  auto iteration = [&](auto last_tag, const uint8_t* kt, const uint8_t* vt, f32x16 (&sc)[2],
+                       f32x16 (&sn)[2], int left) {
+    constexpr bool LAST = decltype(last_tag)::value;
+    bf16x8 A[2], B[2], pb[4];
+    if constexpr (!LAST) {
+      A[0] = kread(kt, 0);
+      A[1] = kread(kt, 1);
+    }
+    const int klim = left - 4 * hh;
+    float pmax = -INFINITY, muse = 0.f;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if constexpr (!LAST) {
+        sn[i & 1] = mfma32x32x16(A[i & 1], qreg[i >> 1], i < 2 ? f32x16{} : sn[i & 1]);
+        if (i + 2 < 16) A[i & 1] = kread(kt, i + 2);
+      }
+      if (i < 4) {  // the maximum, 8 scores per step
+#pragma unroll
+        for (int e = 8 * i; e < 8 * i + 8; ++e) {
+          const int mb = e >> 4, v = e & 15;
+          if constexpr (LAST)
+            if (32 * mb + 8 * (v >> 2) + (v & 3) >= klim) sc[mb][v] = -INFINITY;
+          pmax = fmaxf(pmax, sc[mb][v]);
+        }
+      }
+      if (i == 7) {
+        const float mx = xor32_max(pmax) * a.sl2;
+        mtrue = fmaxf(mtrue, mx);
+        const bool raise = mx > mrun + kSlack;
+        if (__any(raise)) {
+          const float mnew = raise ? mx : mrun;
+          const float alpha = raise ? fast_exp2(mrun - mnew) : 1.f;  // mrun = -inf: 0
+          mrun = mnew;
+          lsum *= alpha;
+#pragma unroll
+          for (int d = 0; d < 4; ++d) o[d] *= alpha;
+        }
+        muse = mrun == -INFINITY ? 0.f : mrun;
+      }
+      if (i >= 8) {  // probabilities, 4 per step
+#pragma unroll
+        for (int e = 4 * (i - 8); e < 4 * (i - 8) + 4; ++e) {
+          const int mb = e >> 4, v = e & 15;
+          const float p = fast_exp2(fmaf(sc[mb][v], a.sl2, -muse));
+          lsum += p;
+          sc[mb][v] = p;
+        }
+      }
+      if (i == 11 || i == 15) {  // B operands of keys 32 mb .. 32 mb + 31
+        const int mb = (i - 11) >> 2;
+#pragma unroll
+        for (int u2 = 0; u2 < 2; ++u2) {
+          const int e0 = 8 * u2;
+          pb[2 * mb + u2] = pack_bf16x8(
+              f32x4{sc[mb][e0], sc[mb][e0 + 2], sc[mb][e0 + 4], sc[mb][e0 + 6]},
+              f32x4{sc[mb][e0 + 1], sc[mb][e0 + 3], sc[mb][e0 + 5], sc[mb][e0 + 7]});
+        }
+      }
+      if (i == 14) B[0] = vread(vt, 0);
+      if (i == 15) B[1] = vread(vt, 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      o[i & 3] = mfma32x32x16(B[i & 1], pb[i >> 2], o[i & 3]);
+      if (i + 2 < 16) B[i & 1] = vread(vt, i + 2);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto stage = [&](int j, f32x16 (&sc)[2], f32x16 (&sn)[2]) {
+    t128::wait_vmem();
+    __syncthreads();
+    if (j + 2 < ntiles) load(kbase, j + 2, t128::lds_addr(kbuf) + (j & 1) * kTileB);
+    if (j + 1 < ntiles) load(vbase, j + 1, t128::lds_addr(vbuf) + ((j + 1) & 1) * kTileB);
+    if (j + 1 < ntiles) iteration(std::false_type{}, kbuf[(j + 1) & 1], vbuf[j & 1], sc, sn, BN);
+    else iteration(std::true_type{}, kbuf[0], vbuf[j & 1], sc, sn, s.k1 - s.k0 - j * BN);
+  };
+  f32x16 sa[2], sb[2];
+  t128::wait_vmem();
+  __syncthreads();
+  if (ntiles > 0) scores_only(kbuf[0], sa);
+  for (int j = 0; j < ntiles; j += 2) {
+    stage(j, sa, sb);
+    if (j + 1 < ntiles) stage(j + 1, sb, sa);
+  }
+
+  // The partial, relative to the true maximum.
+  const float f = mtrue == -INFINITY ? 0.f : fast_exp2(mrun - mtrue);
+  const float lt = xor32_sum(lsum) * f;
+  if (r < a.R) {
+    const int64_t pr = (int64_t)slot * a.N * a.Hq + (int64_t)(r / a.group) * a.Hq + hk * a.group + r % a.group;
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        *reinterpret_cast<f32x4*>(a.po + pr * D + 32 * d + 8 * w + 4 * hh) =
+            f32x4{o[d][4 * w], o[d][4 * w + 1], o[d][4 * w + 2], o[d][4 * w + 3]} * f;
+    if (hh == 0) {
+      a.pm[pr] = mtrue;
+      a.pl[pr] = lt;
+    }
+  }
+}
+
 // ------------------------------------------------ own chain and the merge --
 
 __device__ __forceinline__ void wave_lds_sync() {
@@ -245,18 +656,25 @@ __device__ __forceinline__ void store_vec4(T* p, const f32x4& r) {
   else store4(nullptr, p, r);
 }
 
-// A wave per query row.  Lane 16 u + j holds 4-element chunks j, j + 16, .. of
-// the head dim for the u-th of every four keys (splits).  NI: such chunks.
-template <typename T, int NI>
-__global__ __launch_bounds__(256) void cache_merge_kernel(AttnArgs a) {
-  __shared__ uint16_t chain_s[4][kCacheMaxTokens];
-  __shared__ float score_s[4][kCacheMaxTokens];
+// WPR waves per query row, which share its splits and the keys of its chain and
+// meet in LDS.  Lane 16 u + j holds 4-element chunks j, j + 16, .. of the head
+// dim (NI of them) for the u-th of every four keys (splits) of the wave.
+template <typename T, int NI, int WPR>
+__global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void cache_merge_kernel(AttnArgs a) {
+  constexpr int kWaves = WPR > 4 ? WPR : 4;
+  constexpr int kRows = kWaves / WPR;
+  __shared__ uint16_t chain_s[kWaves][kCacheMaxTokens];
+  __shared__ float score_s[kWaves][kCacheMaxTokens];
+  __shared__ float top_s[kWaves], l_s[kWaves];
+  __shared__ f32x4 acc_s[WPR > 1 ? kWaves : 1][16 * NI];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int part = wave % WPR;
   const int j = lane & 15, u = lane >> 4;
   const int nrows = a.B * a.N * a.Hq;
-  const int row = blockIdx.x * 4 + wave;
-  if (row >= nrows) return;  // waves work by themselves: no barrier follows
+  const int row = blockIdx.x * kRows + wave / WPR;
+  if (row >= nrows) return;  // with WPR > 1 waves of one row stay together: kRows > 1 has no barrier
+  static_assert(WPR == 1 || kRows == 1, "a barrier is for the waves of one row");
   const int h = row % a.Hq;
   const int bi = row / a.Hq;
   const int i = bi % a.N, b = bi / a.N;
@@ -295,14 +713,16 @@ __global__ __launch_bounds__(256) void cache_merge_kernel(AttnArgs a) {
   T* out = static_cast<T*>(a.out) + (int64_t)row * a.D;
   const int nch = a.D / 4;
   if (!there) {
+    if (part == 0) {
 #pragma unroll
-    for (int x = 0; x < NI; ++x)
-      if (u == 0 && j + 16 * x < nch) store_vec4<T>(out + 4 * (j + 16 * x), f32x4{0.f, 0.f, 0.f, 0.f});
-    if (lane == 0) {
-      if (a.m) a.m[si] = -INFINITY;
-      if (a.l) a.l[si] = 0.f;
+      for (int x = 0; x < NI; ++x)
+        if (u == 0 && j + 16 * x < nch) store_vec4<T>(out + 4 * (j + 16 * x), f32x4{0.f, 0.f, 0.f, 0.f});
+      if (lane == 0) {
+        if (a.m) a.m[si] = -INFINITY;
+        if (a.l) a.l[si] = 0.f;
+      }
     }
-    return;
+    return;  // all waves of the row
   }
   wave_lds_sync();
 
@@ -313,7 +733,7 @@ __global__ __launch_bounds__(256) void cache_merge_kernel(AttnArgs a) {
   const T* kb = static_cast<const T*>(a.k) + b * a.seq + hk * a.head + past * a.row;
   const T* vb = static_cast<const T*>(a.v) + b * a.seq + hk * a.head + past * a.row;
   float top = -INFINITY;
-  for (int x0 = 0; x0 < n; x0 += 4) {
+  for (int x0 = 4 * part; x0 < n; x0 += 4 * WPR) {
     const int x = min(x0 + u, n - 1);
     const T* kp = kb + chain[x] * a.row;
     f32x4 s4 = {0.f, 0.f, 0.f, 0.f};
@@ -331,16 +751,23 @@ __global__ __launch_bounds__(256) void cache_merge_kernel(AttnArgs a) {
   const Deal d = deal_slots(a.past, a.B, a.C, a.slots, -1, b);
   const int64_t rows = (int64_t)a.N * a.Hq;
   const int64_t pr0 = d.first * rows + (int64_t)i * a.Hq + h;
-  for (int s = lane; s < d.count; s += 64) top = fmaxf(top, a.pm[pr0 + s * rows]);
+  for (int s = 64 * part + lane; s < d.count; s += 64 * WPR) top = fmaxf(top, a.pm[pr0 + s * rows]);
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+  if constexpr (WPR > 1) {
+    if (lane == 0) top_s[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WPR; ++w) top = fmaxf(top, top_s[w]);
+  }
   const float muse = top == -INFINITY ? 0.f : top;
 
   f32x4 acc[NI];
 #pragma unroll
   for (int x = 0; x < NI; ++x) acc[x] = f32x4{0.f, 0.f, 0.f, 0.f};
   float l = 0.f;
-  for (int s = u; s < d.count; s += 4) {
+#pragma unroll 4
+  for (int s = 4 * part + u; s < d.count; s += 4 * WPR) {
     const int64_t pr = pr0 + s * rows;
     const float w = exp2f(a.pm[pr] - muse);  // a split without keys: 0
     l += w * a.pl[pr];
@@ -348,7 +775,7 @@ __global__ __launch_bounds__(256) void cache_merge_kernel(AttnArgs a) {
     for (int x = 0; x < NI; ++x)
       acc[x] += load_w<float, 4>(a.po + pr * a.D, 4 * (j + 16 * x), a.D, true) * w;
   }
-  for (int x = u; x < n; x += 4) {
+  for (int x = 4 * part + u; x < n; x += 4 * WPR) {
     const float p = exp2f(score[x] - muse);
     const T* vp = vb + chain[x] * a.row;
     l += p;
@@ -356,13 +783,31 @@ __global__ __launch_bounds__(256) void cache_merge_kernel(AttnArgs a) {
     for (int y = 0; y < NI; ++y) acc[y] += load_w<T, 4>(vp, 4 * (j + 16 * y), a.D, true) * p;
   }
   l = group4_sum(l);
+#pragma unroll
+  for (int x = 0; x < NI; ++x)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[x][e] = group4_sum(acc[x][e]);
+  if constexpr (WPR > 1) {
+    if (u == 0)
+#pragma unroll
+      for (int x = 0; x < NI; ++x) acc_s[wave][j + 16 * x] = acc[x];
+    if (lane == 0) l_s[wave] = l;
+    __syncthreads();
+    if (part != 0) return;
+    l = 0.f;
+#pragma unroll
+    for (int x = 0; x < NI; ++x) acc[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < WPR; ++w) {
+      l += l_s[w];
+#pragma unroll
+      for (int x = 0; x < NI; ++x) acc[x] += acc_s[w][j + 16 * x];
+    }
+  }
   const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
-  for (int x = 0; x < NI; ++x) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[x][e] = group4_sum(acc[x][e]) * inv;
-    if (u == 0 && j + 16 * x < nch) store_vec4<T>(out + 4 * (j + 16 * x), acc[x]);
-  }
+  for (int x = 0; x < NI; ++x)
+    if (u == 0 && j + 16 * x < nch) store_vec4<T>(out + 4 * (j + 16 * x), acc[x] * inv);
   if (lane == 0) {
     if (a.m) a.m[si] = top == -INFINITY ? top : top * kLn2;
     if (a.l) a.l[si] = l;
@@ -371,18 +816,41 @@ __global__ __launch_bounds__(256) void cache_merge_kernel(AttnArgs a) {
 
 // ------------------------------------------------------------------- host --
 
+enum class Form { kFp32, kStream, kTiled };
+
 struct Plan {
-  int wave_rows, units, slots;
+  Form form;
+  int waves;  // of a workgroup
+  int rows;   // of a workgroup (fp32: 16 for each of its row blocks)
+  int units, slots;
 };
 
 Plan make_plan(const CacheProblem& p) {
   const int64_t R = (int64_t)p.N * (p.Hq / p.Hkv);
-  Plan x;
-  x.wave_rows = R <= 16 ? 1 : R <= 32 ? 2 : 4;
-  const int64_t rb = (R + 16 * x.wave_rows - 1) / (16 * x.wave_rows);
-  x.units = (int)(rb * p.Hkv);
   const int64_t tiles = (int64_t)p.B * ((p.C + kTile - 1) / kTile);
-  const int64_t deal = std::max<int64_t>(1, std::min<int64_t>(512 / x.units, tiles));
+  const bool bf16 = p.dtype == 1 && !p.precise && (p.D == 64 || p.D == 128);
+  Plan x;
+  x.waves = 4;
+  int64_t want = 512;  // workgroups
+  if (!bf16) {
+    x.form = Form::kFp32;
+    x.rows = R <= 16 ? 16 : R <= 32 ? 32 : 64;
+  } else if (R <= 32 || p.D == 64) {
+    x.form = Form::kStream;
+    x.rows = R <= 16 ? 16 : 32;
+    const int64_t units = (R + x.rows - 1) / x.rows * p.Hkv;
+    if (units * p.B <= 16 && tiles * units * p.D >= 64 * 6 * 2048) {
+      x.waves = 1;
+      want = 2048;
+    }
+  } else {
+    x.form = Form::kTiled;
+    x.waves = R <= 64 ? 2 : R <= 128 ? 4 : 8;
+    x.rows = 32 * x.waves;
+    if (x.waves == 8) want = 256;
+  }
+  x.units = (int)((R + x.rows - 1) / x.rows * p.Hkv);
+  const int64_t deal = std::max<int64_t>(1, std::min<int64_t>(want / x.units, tiles));
   x.slots = (int)(deal + p.B);
   return x;
 }
@@ -420,15 +888,15 @@ hipError_t launch_cache_attn(const CacheProblem& p, const void* q, const void* k
   a.R = p.N * a.group;
   a.slots = x.slots;
   a.units = x.units;
-  a.wave_rows = x.wave_rows;
+  a.wave_rows = x.rows / 16;
   a.seq = p.seq;
   a.row = p.row;
   a.head = p.head;
   a.sl2 = p.sl2;
   auto prefix = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(x.slots * x.units)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(x.slots * x.units)), dim3(64 * x.waves), 0, st, a);
   };
-  auto by_dim = [&](auto t) {
+  auto fp32 = [&](auto t) {
     using T = decltype(t);
     if (p.D <= 16) prefix(cache_prefix32_kernel<T, 1>);
     else if (p.D <= 32) prefix(cache_prefix32_kernel<T, 2>);
@@ -437,20 +905,44 @@ hipError_t launch_cache_attn(const CacheProblem& p, const void* q, const void* k
     else if (p.D <= 128) prefix(cache_prefix32_kernel<T, 8>);
     else prefix(cache_prefix32_kernel<T, 16>);
   };
-  if (p.dtype == 1) by_dim(uint16_t{});
-  else by_dim(float{});
+  auto stream = [&](auto d) {
+    constexpr int kD = decltype(d)::value;
+    if (x.waves == 1) x.rows == 16 ? prefix(cache_stream_kernel<kD, 1, 1>) : prefix(cache_stream_kernel<kD, 2, 1>);
+    else x.rows == 16 ? prefix(cache_stream_kernel<kD, 1, 4>) : prefix(cache_stream_kernel<kD, 2, 4>);
+  };
+  if (x.form == Form::kFp32) {
+    if (p.dtype == 1) fp32(uint16_t{});
+    else fp32(float{});
+  } else if (x.form == Form::kStream) {
+    if (p.D == 64) stream(std::integral_constant<int, 64>{});
+    else stream(std::integral_constant<int, 128>{});
+  } else {
+    const bool once = x.units == p.Hkv;  // the cache is read once: L2 need not keep it
+    if (x.waves == 2) prefix(cache_tile128_kernel<2, true>);
+    else if (x.waves == 4) prefix(cache_tile128_kernel<4, true>);
+    else if (once) prefix(cache_tile128_kernel<8, true>);
+    else prefix(cache_tile128_kernel<8, false>);
+  }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const unsigned blocks = (unsigned)(((int64_t)p.B * p.N * p.Hq + 3) / 4);
-  auto merge = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, st, a); };
-  auto merge_dim = [&](auto t) {
-    using T = decltype(t);
-    if (p.D <= 64) merge(cache_merge_kernel<T, 1>);
-    else if (p.D <= 128) merge(cache_merge_kernel<T, 2>);
-    else merge(cache_merge_kernel<T, 4>);
+  const int64_t rows = (int64_t)p.B * p.N * p.Hq;
+  const bool wide = x.slots - p.B >= 64 && rows < 1024;
+  auto merge = [&](auto kernel, int threads, int per) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + per - 1) / per)), dim3(threads), 0, st, a);
   };
-  if (p.dtype == 1) merge_dim(uint16_t{});
-  else merge_dim(float{});
+  auto merge_dim = [&](auto t, auto ni) {
+    using T = decltype(t);
+    constexpr int kNI = decltype(ni)::value;
+    if (wide) merge(cache_merge_kernel<T, kNI, 16>, 1024, 1);
+    else merge(cache_merge_kernel<T, kNI, 1>, 256, 4);
+  };
+  auto merge_type = [&](auto t) {
+    if (p.D <= 64) merge_dim(t, std::integral_constant<int, 1>{});
+    else if (p.D <= 128) merge_dim(t, std::integral_constant<int, 2>{});
+    else merge_dim(t, std::integral_constant<int, 4>{});
+  };
+  if (p.dtype == 1) merge_type(uint16_t{});
+  else merge_type(float{});
   return hipGetLastError();
 }
 
