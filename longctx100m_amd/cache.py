@@ -35,34 +35,33 @@ from .ring_attention import _dtype_code
 MAX_TOKENS = _lib.LC_CACHE_MAX_TOKENS
 
 
-def _stream_of(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-def _call(device: torch.device, fn, *args) -> None:
+def _call(device: int, fn, *args) -> None:
     """fn(*args, stream) with the tensors' device current, as HIP launches want it."""
-    if torch.cuda.current_device() == device.index:
-        _lib.check(fn(*args, _stream_of(device)))
+    if torch._C._cuda_getDevice() == device:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            _lib.check(fn(*args, _stream_of(device)))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if rc:
+        _lib.check(rc)
 
 
-def _buf(t, shape, dtype, device, name: str) -> int:
+def _buf(t, shape, dtype, device: int, name: str) -> int:
     """The address of a contiguous tensor of exactly this shape, type and device."""
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != shape or \
-            t.device != device or not t.is_contiguous():
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.shape != shape or \
+            t.get_device() != device or not t.is_contiguous():
         what = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t)
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} "
-                         f"on {device}, got {what}")
+                         f"on cuda:{device}, got {what}")
     return t.data_ptr()
 
 
-def _opt(t, shape, dtype, device, name: str) -> Optional[int]:
+def _opt(t, shape, dtype, device: int, name: str) -> Optional[int]:
     return None if t is None else _buf(t, shape, dtype, device, name)
 
 
-def _kv(k: torch.Tensor, v: Optional[torch.Tensor]) -> None:
+def _kv(k: torch.Tensor, v: Optional[torch.Tensor]) -> int:
+    """Checks a cache; returns its device."""
     for t, name in ((k, "k"), (v, "v")):
         if t is None:
             continue
@@ -73,9 +72,10 @@ def _kv(k: torch.Tensor, v: Optional[torch.Tensor]) -> None:
         if t.dim() != 4 or t.stride(3) != 1:
             raise ValueError(f"{name} must be a cache [batch, rows, kv_heads, head_dim] with "
                              "contiguous head_dim")
-    if v is not None and (v.shape != k.shape or v.stride() != k.stride() or v.dtype != k.dtype
-                          or v.device != k.device):
+    if v is not None and (v.shape != k.shape or v.stride() != k.stride() or v.dtype is not k.dtype
+                          or v.get_device() != k.get_device()):
         raise ValueError("k and v must have the same shape, strides, type and device")
+    return k.get_device()
 
 
 def _describe(k: torch.Tensor, tokens: int, heads_q: int, precise: bool = False) -> _lib.Cache:
@@ -89,7 +89,7 @@ def _describe(k: torch.Tensor, tokens: int, heads_q: int, precise: bool = False)
 
 def _queries(q: torch.Tensor, k: torch.Tensor) -> Tuple[int, int, int, int]:
     if not isinstance(q, torch.Tensor) or q.dim() != 4 or not q.is_contiguous() or \
-            q.dtype != k.dtype or q.device != k.device:
+            q.dtype is not k.dtype or q.get_device() != k.get_device():
         raise ValueError("q must be a contiguous [batch, tokens, heads, head_dim] tensor of the "
                          "cache's type and device")
     if q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
@@ -114,9 +114,8 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, past: torc
     fp32), the statistics as those of ``ring_attention.fwd_shard``.  Padded
     tokens have out = 0, m = -inf, l = 0.  ``precise`` takes bf16 inputs
     through the fp32-math kernels."""
-    _kv(k, v)
+    dev = _kv(k, v)
     b, n, hq, d = _queries(q, k)
-    dev = q.device
     stats = (b, hq, n)
     out = torch.empty_like(q) if out is None else out
     m = torch.empty(stats, dtype=torch.float32, device=dev) if m is None else m
@@ -133,11 +132,11 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, past: torc
     return out, m, l
 
 
-def _workspace(workspace, size, c: _lib.Cache, dev) -> torch.Tensor:
+def _workspace(workspace, size, c: _lib.Cache, dev: int) -> torch.Tensor:
     if workspace is None:
         return torch.empty(max(size(c), 1), dtype=torch.uint8, device=dev)
-    if not workspace.is_contiguous() or workspace.device != dev:
-        raise ValueError(f"workspace must be a contiguous tensor on {dev}")
+    if not workspace.is_contiguous() or workspace.get_device() != dev:
+        raise ValueError(f"workspace must be a contiguous tensor on cuda:{dev}")
     return workspace
 
 
@@ -154,9 +153,8 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, past: torch.Tensor, m: torch.T
     weights + w (weights None: w), the tokens' own rows w, and rows behind them
     keep what ``out`` holds; without ``out`` a tensor of zeros is made.  ``out``
     may be ``weights``.  N is limited to 256 with parents only."""
-    _kv(k, None)
+    dev = _kv(k, None)
     b, n, hq, d = _queries(q, k)
-    dev = q.device
     shape, stats = (b, k.shape[2], k.shape[1]), (b, hq, n)
     out = torch.zeros(shape, dtype=torch.float32, device=dev) if out is None else out
     ptrs = (_buf(past, (b,), torch.int32, dev, "past"),
@@ -195,9 +193,9 @@ def evict(k: torch.Tensor, v: torch.Tensor, weights: torch.Tensor, lens: torch.T
 
     ``weights_out`` and ``positions_out`` may be their inputs; they are written up to
     lens_out.  Without them tensors of zeros are made."""
-    _kv(k, v)
+    dev = _kv(k, v)
     b, c, hkv, d = k.shape
-    dev, shape = k.device, (b, hkv, c)
+    shape = (b, hkv, c)
     weights_out = torch.zeros(shape, dtype=torch.float32, device=dev) \
         if weights_out is None else weights_out
     positions_out = torch.zeros(shape, dtype=torch.int32, device=dev) \
@@ -246,7 +244,7 @@ def commit(layers: Layers, past: torch.Tensor, path: torch.Tensor, *,
     past + j.  path [B, P] int32 holds token numbers in ascending order and
     ends at the first -1.  Returns the new lengths, past + the path's length."""
     k = layers.ks[0]
-    dev, b = k.device, k.shape[0]
+    dev, b = k.get_device(), k.shape[0]
     if not isinstance(path, torch.Tensor) or path.dim() != 2:
         raise ValueError("path must be a [batch, tokens] tensor")
     lens_out = torch.empty(b, dtype=torch.int32, device=dev) if lens_out is None else lens_out

@@ -36,7 +36,10 @@ struct AttnArgs {
   const void *q, *k, *v;
   void* out;
   float *m, *l;
-  float *po, *pm, *pl;  // partials: [slots][N * Hq] rows of D, and their statistics (log2 units)
+  // Partials, slot s of query row (token, head) at row * slots + s: D values, and
+  // (m, l), m in log2 units.
+  float* po;
+  float2* ps;
   const int32_t *past, *parents;
   int B, N, C, Hq, Hkv, D, group, R;  // R: query rows of a KV head
   int slots, units;                   // units: workgroups of a slot
@@ -121,6 +124,11 @@ __device__ __forceinline__ bool share_of(const AttnArgs& a, int slot, Share& s) 
   s.k1 = min(s.k0 + d.per * kTile, s.rows);
   if (s.k0 > s.k1) s.k0 = s.k1;
   return true;
+}
+
+// Where the partial of query row r of KV head hk goes.
+__device__ __forceinline__ int64_t partial_row(const AttnArgs& a, int r, int hk, int slot) {
+  return ((int64_t)(r / a.group) * a.Hq + hk * a.group + r % a.group) * a.slots + slot;
 }
 
 // ------------------------------------------------- the past, fp32 products --
@@ -212,7 +220,6 @@ __global__ __launch_bounds__(256) void cache_prefix32_kernel(AttnArgs a) {
   store_part<NJ>(smem + wave * kPart, o, c, g);
   __syncthreads();
   const int per_row = a.D / 4;
-  const int64_t prow0 = (int64_t)slot * a.N * a.Hq;
   for (int i = threadIdx.x; i < 16 * a.wave_rows * per_row; i += 256) {
     const int lr = i / per_row, d = 4 * (i - lr * per_row);
     const int row = 16 * rb * a.wave_rows + lr;
@@ -225,12 +232,9 @@ __global__ __launch_bounds__(256) void cache_prefix32_kernel(AttnArgs a) {
       ls += lsm[w][cc];
       mt = fmaxf(mt, msm[w][cc]);
     }
-    const int64_t pr = prow0 + (int64_t)(row / a.group) * a.Hq + hk * a.group + row % a.group;
+    const int64_t pr = partial_row(a, row, hk, slot);
     *reinterpret_cast<f32x4*>(a.po + pr * a.D + d) = acc;
-    if (d == 0) {
-      a.pm[pr] = mt;
-      a.pl[pr] = ls;
-    }
+    if (d == 0) a.ps[pr] = make_float2(mt, ls);
   }
 }
 
@@ -394,14 +398,10 @@ __global__ __launch_bounds__(64 * W, NB * W == 1 ? 1 : 2) void cache_stream_kern
     if (j + 1 < ntiles) tile(j + 1, krb, kra);
   }
 
-  const int64_t prow0 = (int64_t)slot * a.N * a.Hq + hk * a.group;
   auto emit = [&](int r, int d, const f32x4& acc, float L, float M) {
-    const int64_t pr = prow0 + (int64_t)(r / a.group) * a.Hq + r % a.group;
+    const int64_t pr = partial_row(a, r, hk, slot);
     *reinterpret_cast<f32x4*>(a.po + pr * D + d) = acc;
-    if (d == 0) {
-      a.pm[pr] = M;
-      a.pl[pr] = L;
-    }
+    if (d == 0) a.ps[pr] = make_float2(M, L);
   };
   if constexpr (W == 1) {
 #pragma unroll
@@ -457,7 +457,8 @@ __global__ __launch_bounds__(64 * W, NB * W == 1 ? 1 : 2) void cache_stream_kern
 // (tile128.h), filled by LDS DMA; S^T = K Q^T and O^T += V^T P^T on 32 x 32 x 16
 // products.  Iteration j issues the products of S^T for tile j + 1 and beside
 // them, on the VALU, the softmax of tile j, then O^T += V_j^T P_j^T; K runs one
-// tile ahead of V, two buffers each, one barrier per tile.  A row's reference
+// tile ahead of V, two buffers each, one barrier per tile.
+// A row's reference
 // maximum is only raised by more than 2^kSlack, so rescaling is rare; the true
 // one is tracked beside it.
 template <int NW, bool NT>
@@ -628,17 +629,14 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void cache_tile128_kernel
   const float f = mtrue == -INFINITY ? 0.f : fast_exp2(mrun - mtrue);
   const float lt = xor32_sum(lsum) * f;
   if (r < a.R) {
-    const int64_t pr = (int64_t)slot * a.N * a.Hq + (int64_t)(r / a.group) * a.Hq + hk * a.group + r % a.group;
+    const int64_t pr = partial_row(a, r, hk, slot);
 #pragma unroll
     for (int d = 0; d < 4; ++d)
 #pragma unroll
       for (int w = 0; w < 4; ++w)
         *reinterpret_cast<f32x4*>(a.po + pr * D + 32 * d + 8 * w + 4 * hh) =
             f32x4{o[d][4 * w], o[d][4 * w + 1], o[d][4 * w + 2], o[d][4 * w + 3]} * f;
-    if (hh == 0) {
-      a.pm[pr] = mtrue;
-      a.pl[pr] = lt;
-    }
+    if (hh == 0) a.ps[pr] = make_float2(mtrue, lt);
   }
 }
 
@@ -656,64 +654,78 @@ __device__ __forceinline__ void store_vec4(T* p, const f32x4& r) {
   else store4(nullptr, p, r);
 }
 
-// WPR waves per query row, which share its splits and the keys of its chain and
-// meet in LDS.  Lane 16 u + j holds 4-element chunks j, j + 16, .. of the head
-// dim (NI of them) for the u-th of every four keys (splits) of the wave.
+// WPR waves (a workgroup) per query row share its splits and the keys of its
+// chain and meet in LDS.  Lane 16 u + j holds 4-element chunks j, j + 16, .. of
+// the head dim (NI of them) for the u-th of every four keys (splits) of the
+// wave.  A row costs few bytes and would cost many memory latencies, so what
+// does not depend on the chain (the first partials) is read before the chain
+// is followed, and the keys and values of kKeys steps together (64 tokens of 32
+// heads over 32 splits, chains of some ten keys: 17.5 us with one step at a
+// time).
 template <typename T, int NI, int WPR>
-__global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void cache_merge_kernel(AttnArgs a) {
-  constexpr int kWaves = WPR > 4 ? WPR : 4;
-  constexpr int kRows = kWaves / WPR;
-  __shared__ uint16_t chain_s[kWaves][kCacheMaxTokens];
-  __shared__ float score_s[kWaves][kCacheMaxTokens];
-  __shared__ float top_s[kWaves], l_s[kWaves];
-  __shared__ f32x4 acc_s[WPR > 1 ? kWaves : 1][16 * NI];
+__global__ __launch_bounds__(64 * WPR) void cache_merge_kernel(AttnArgs a) {
+  constexpr int kStep = 4 * WPR;                              // splits and keys of a step
+  constexpr int kFirst = (WPR == 1 ? 8 : 4) / (NI > 1 ? NI : 2);  // steps of partials read up front
+  constexpr int kKeys = WPR == 1 && NI < 4 ? 4 : 1;
+  __shared__ uint16_t chain_s[WPR][kCacheMaxTokens];
+  __shared__ float top_s[WPR], l_s[WPR];
+  __shared__ f32x4 acc_s[WPR][16 * NI];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int part = wave % WPR;
   const int j = lane & 15, u = lane >> 4;
-  const int nrows = a.B * a.N * a.Hq;
-  const int row = blockIdx.x * kRows + wave / WPR;
-  if (row >= nrows) return;  // with WPR > 1 waves of one row stay together: kRows > 1 has no barrier
-  static_assert(WPR == 1 || kRows == 1, "a barrier is for the waves of one row");
+  const int row = blockIdx.x;
   const int h = row % a.Hq;
   const int bi = row / a.Hq;
   const int i = bi % a.N, b = bi / a.N;
   const int hk = h / a.group;
-  const int past = __builtin_amdgcn_readfirstlane(a.past[b]);
+  const int past = a.past[b];
+  const int nch = a.D / 4;
+
+  // The parents of the tokens up to this one, over the lanes.
+  int par[kCacheMaxTokens / 64];
+#pragma unroll
+  for (int x = 0; x < kCacheMaxTokens / 64; ++x) {
+    const int at = 64 * x + lane;
+    par[x] = at - 1;
+    if (a.parents != nullptr && 64 * x <= i) par[x] = a.parents[(int64_t)b * a.N + min(at, a.N - 1)];
+  }
+  f32x4 qv[NI];
+  const T* qp = static_cast<const T*>(a.q) + (int64_t)row * a.D;
+#pragma unroll
+  for (int x = 0; x < NI; ++x) qv[x] = load_w<T, 4>(qp, 4 * (j + 16 * x), a.D, true);
+
+  const Deal d = deal_slots(a.past, a.B, a.C, a.slots, -1, b);
+  const int64_t pr0 = ((int64_t)i * a.Hq + h) * a.slots + d.first;
+  f32x4 po[kFirst][NI];
+  float2 ps[kFirst];
+#pragma unroll
+  for (int f = 0; f < kFirst; ++f) {
+    const int s = kStep * f + 4 * wave + u;
+    const int64_t pr = pr0 + min(s, d.count - 1);
+    ps[f] = a.ps[pr];
+#pragma unroll
+    for (int x = 0; x < NI; ++x) po[f][x] = load_w<float, 4>(a.po + pr * a.D, 4 * (j + 16 * x), a.D, true);
+  }
 
   // The chain of parents, the token itself first.
   uint16_t* chain = chain_s[wave];
-  float* score = score_s[wave];
   bool there = past >= 0 && past < a.C && i < a.C - past;
   int n = 0;
-  if (there) {
-    int par[kCacheMaxTokens / 64];
+  for (int at = i; there;) {  // at falls with every step
+    if (lane == 0) chain[n] = (uint16_t)at;
+    ++n;
+    int p = -2;
 #pragma unroll
-    for (int x = 0; x < kCacheMaxTokens / 64; ++x) {
-      const int at = 64 * x + lane;
-      par[x] = at < a.N ? (a.parents ? a.parents[(int64_t)b * a.N + at] : at - 1) : -2;
-    }
-    int at = i;
-    while (true) {  // at falls with every step
-      if (lane == 0) chain[n] = (uint16_t)at;
-      ++n;
-      int p = -2;
-#pragma unroll
-      for (int x = 0; x < kCacheMaxTokens / 64; ++x)
-        if (at >> 6 == x) p = __builtin_amdgcn_readlane(par[x], at & 63);
-      if (p == -1) break;
-      if (p < -1 || p >= at) {
-        there = false;
-        break;
-      }
-      at = p;
-    }
+    for (int x = 0; x < kCacheMaxTokens / 64; ++x)
+      if (at >> 6 == x) p = __builtin_amdgcn_readlane(par[x], at & 63);
+    if (p == -1) break;
+    there = p >= 0 && p < at;
+    at = p;
   }
   const int64_t si = ((int64_t)b * a.Hq + h) * a.N + i;
   T* out = static_cast<T*>(a.out) + (int64_t)row * a.D;
-  const int nch = a.D / 4;
-  if (!there) {
-    if (part == 0) {
+  if (!there) {  // the whole workgroup
+    if (wave == 0) {
 #pragma unroll
       for (int x = 0; x < NI; ++x)
         if (u == 0 && j + 16 * x < nch) store_vec4<T>(out + 4 * (j + 16 * x), f32x4{0.f, 0.f, 0.f, 0.f});
@@ -722,36 +734,67 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void cache_merge_kernel(A
         if (a.l) a.l[si] = 0.f;
       }
     }
-    return;  // all waves of the row
+    return;
   }
   wave_lds_sync();
 
-  f32x4 qv[NI];
-  const T* qp = static_cast<const T*>(a.q) + (int64_t)row * a.D;
-#pragma unroll
-  for (int x = 0; x < NI; ++x) qv[x] = load_w<T, 4>(qp, 4 * (j + 16 * x), a.D, true);
+  // The chain's keys: every group of 16 lanes has a running maximum of its own.
   const T* kb = static_cast<const T*>(a.k) + b * a.seq + hk * a.head + past * a.row;
   const T* vb = static_cast<const T*>(a.v) + b * a.seq + hk * a.head + past * a.row;
-  float top = -INFINITY;
-  for (int x0 = 4 * part; x0 < n; x0 += 4 * WPR) {
-    const int x = min(x0 + u, n - 1);
-    const T* kp = kb + chain[x] * a.row;
-    f32x4 s4 = {0.f, 0.f, 0.f, 0.f};
+  f32x4 acc[NI];
 #pragma unroll
-    for (int y = 0; y < NI; ++y) s4 += qv[y] * load_w<T, 4>(kp, 4 * (j + 16 * y), a.D, true);
-    float s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+  for (int x = 0; x < NI; ++x) acc[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  for (int x0 = 4 * wave + u; x0 < n; x0 += kKeys * kStep) {
+    f32x4 kx[kKeys][NI], vx[kKeys][NI];
 #pragma unroll
-    for (int off = 1; off < 16; off <<= 1) s += __shfl_xor(s, off, 64);
-    s *= a.sl2;
-    top = fmaxf(top, s);
-    if (j == 0 && x0 + u < n) score[x0 + u] = s;
+    for (int f = 0; f < kKeys; ++f) {
+      const int64_t off = chain[min(x0 + kStep * f, n - 1)] * a.row;
+#pragma unroll
+      for (int y = 0; y < NI; ++y) {
+        kx[f][y] = load_w<T, 4>(kb + off, 4 * (j + 16 * y), a.D, true);
+        vx[f][y] = load_w<T, 4>(vb + off, 4 * (j + 16 * y), a.D, true);
+      }
+    }
+    float s[kKeys], mnew = m;
+#pragma unroll
+    for (int f = 0; f < kKeys; ++f) {
+      f32x4 s4 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int y = 0; y < NI; ++y) s4 += qv[y] * kx[f][y];
+      s[f] = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+    }
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1)
+#pragma unroll
+      for (int f = 0; f < kKeys; ++f) s[f] += __shfl_xor(s[f], o, 64);
+#pragma unroll
+    for (int f = 0; f < kKeys; ++f) {
+      s[f] *= a.sl2;
+      if (x0 + kStep * f < n) mnew = fmaxf(mnew, s[f]);
+    }
+    const float muse = mnew == -INFINITY ? 0.f : mnew;
+    const float alpha = exp2f(m - muse);  // m = -inf: 0
+    l *= alpha;
+#pragma unroll
+    for (int y = 0; y < NI; ++y) acc[y] *= alpha;
+    m = mnew;
+#pragma unroll
+    for (int f = 0; f < kKeys; ++f) {
+      if (x0 + kStep * f >= n) continue;
+      const float p = exp2f(s[f] - muse);
+      l += p;
+#pragma unroll
+      for (int y = 0; y < NI; ++y) acc[y] += vx[f][y] * p;
+    }
   }
-  wave_lds_sync();
 
-  const Deal d = deal_slots(a.past, a.B, a.C, a.slots, -1, b);
-  const int64_t rows = (int64_t)a.N * a.Hq;
-  const int64_t pr0 = d.first * rows + (int64_t)i * a.Hq + h;
-  for (int s = 64 * part + lane; s < d.count; s += 64 * WPR) top = fmaxf(top, a.pm[pr0 + s * rows]);
+  // The row's maximum, and everything relative to it.
+  float top = m;
+#pragma unroll
+  for (int f = 0; f < kFirst; ++f) top = fmaxf(top, ps[f].x);  // (a re-read split changes nothing)
+  for (int s = kStep * kFirst + 64 * wave + lane; s < d.count; s += 64 * WPR)
+    top = fmaxf(top, a.ps[pr0 + s].x);
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
   if constexpr (WPR > 1) {
@@ -761,26 +804,29 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void cache_merge_kernel(A
     for (int w = 0; w < WPR; ++w) top = fmaxf(top, top_s[w]);
   }
   const float muse = top == -INFINITY ? 0.f : top;
-
-  f32x4 acc[NI];
+  {
+    const float alpha = exp2f(m - muse);
+    l *= alpha;
 #pragma unroll
-  for (int x = 0; x < NI; ++x) acc[x] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float l = 0.f;
-#pragma unroll 4
-  for (int s = 4 * part + u; s < d.count; s += 4 * WPR) {
-    const int64_t pr = pr0 + s * rows;
-    const float w = exp2f(a.pm[pr] - muse);  // a split without keys: 0
-    l += w * a.pl[pr];
+    for (int x = 0; x < NI; ++x) acc[x] *= alpha;
+  }
+#pragma unroll
+  for (int f = 0; f < kFirst; ++f) {
+    if (kStep * f + 4 * wave + u >= d.count) continue;
+    const float w = exp2f(ps[f].x - muse);  // a split without keys: 0
+    l += w * ps[f].y;
+#pragma unroll
+    for (int x = 0; x < NI; ++x) acc[x] += po[f][x] * w;
+  }
+#pragma unroll(NI == 4 ? 1 : 4)
+  for (int s = kStep * kFirst + 4 * wave + u; s < d.count; s += kStep) {
+    const int64_t pr = pr0 + s;
+    const float2 st = a.ps[pr];
+    const float w = exp2f(st.x - muse);
+    l += w * st.y;
 #pragma unroll
     for (int x = 0; x < NI; ++x)
       acc[x] += load_w<float, 4>(a.po + pr * a.D, 4 * (j + 16 * x), a.D, true) * w;
-  }
-  for (int x = 4 * part + u; x < n; x += 4 * WPR) {
-    const float p = exp2f(score[x] - muse);
-    const T* vp = vb + chain[x] * a.row;
-    l += p;
-#pragma unroll
-    for (int y = 0; y < NI; ++y) acc[y] += load_w<T, 4>(vp, 4 * (j + 16 * y), a.D, true) * p;
   }
   l = group4_sum(l);
 #pragma unroll
@@ -793,12 +839,12 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void cache_merge_kernel(A
       for (int x = 0; x < NI; ++x) acc_s[wave][j + 16 * x] = acc[x];
     if (lane == 0) l_s[wave] = l;
     __syncthreads();
-    if (part != 0) return;
-    l = 0.f;
+    if (wave != 0) return;
+    l = l_s[0];
 #pragma unroll
-    for (int x = 0; x < NI; ++x) acc[x] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < WPR; ++w) {
+    for (int x = 0; x < NI; ++x) acc[x] = acc_s[0][j + 16 * x];
+#pragma unroll 4
+    for (int w = 1; w < WPR; ++w) {
       l += l_s[w];
 #pragma unroll
       for (int x = 0; x < NI; ++x) acc[x] += acc_s[w][j + 16 * x];
@@ -831,7 +877,7 @@ Plan make_plan(const CacheProblem& p) {
   const bool bf16 = p.dtype == 1 && !p.precise && (p.D == 64 || p.D == 128);
   Plan x;
   x.waves = 4;
-  int64_t want = 512;  // workgroups
+  int64_t want = 256;  // workgroups
   if (!bf16) {
     x.form = Form::kFp32;
     x.rows = R <= 16 ? 16 : R <= 32 ? 32 : 64;
@@ -847,7 +893,6 @@ Plan make_plan(const CacheProblem& p) {
     x.form = Form::kTiled;
     x.waves = R <= 64 ? 2 : R <= 128 ? 4 : 8;
     x.rows = 32 * x.waves;
-    if (x.waves == 8) want = 256;
   }
   x.units = (int)((R + x.rows - 1) / x.rows * p.Hkv);
   const int64_t deal = std::max<int64_t>(1, std::min<int64_t>(want / x.units, tiles));
@@ -874,8 +919,7 @@ hipError_t launch_cache_attn(const CacheProblem& p, const void* q, const void* k
   a.m = m;
   a.l = l;
   a.po = static_cast<float*>(ws);
-  a.pm = a.po + prows * p.D;
-  a.pl = a.pm + prows;
+  a.ps = reinterpret_cast<float2*>(a.po + prows * p.D);
   a.past = p.past;
   a.parents = p.parents;
   a.B = p.B;
@@ -926,15 +970,16 @@ hipError_t launch_cache_attn(const CacheProblem& p, const void* q, const void* k
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int64_t rows = (int64_t)p.B * p.N * p.Hq;
-  const bool wide = x.slots - p.B >= 64 && rows < 1024;
-  auto merge = [&](auto kernel, int threads, int per) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + per - 1) / per)), dim3(threads), 0, st, a);
+  const bool wide = x.slots - p.B >= 128 && rows <= 256;
+  auto merge = [&](auto kernel, int waves) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(64 * waves), 0, st, a);
   };
   auto merge_dim = [&](auto t, auto ni) {
     using T = decltype(t);
     constexpr int kNI = decltype(ni)::value;
-    if (wide) merge(cache_merge_kernel<T, kNI, 16>, 1024, 1);
-    else merge(cache_merge_kernel<T, kNI, 1>, 256, 4);
+    if (wide) merge(cache_merge_kernel<T, kNI, 16>, 16);
+    else if (rows < 1024) merge(cache_merge_kernel<T, kNI, 4>, 4);
+    else merge(cache_merge_kernel<T, kNI, 1>, 1);
   };
   auto merge_type = [&](auto t) {
     if (p.D <= 64) merge_dim(t, std::integral_constant<int, 1>{});

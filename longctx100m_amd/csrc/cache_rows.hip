@@ -3,13 +3,22 @@
 //
 // Eviction of a head's L rows to a budget of n: rows are ranked by (protected,
 // weight), ties by the lower row.  Each row's rank is a 32-bit key that orders
-// as the weights do, so the smallest kept key T and the number of rows with
-// that very key that stay come from three histogram passes over the key's
-// digits (11, 11 and 10 bits).  The kept rows below n stay where they are; the
+// as the weights do, so the smallest kept key and the number of rows with that
+// very key that stay (the cut) come from three histograms over the key's digits
+// (11, 11 and 10 bits).  The kept rows below n stay where they are; the
 // others, ascending, go to the holes below n, ascending.  Sources lie at n and
 // above and targets below, so all moves run at once and in place, and no row
 // moves that could stay: a cache that is cut back by a few rows costs a few
 // rows' copies.
+//
+// Up to kShortRows rows one workgroup holds a head's keys in registers and plans
+// it in one launch.  Longer heads are split over the chip, one launch for each
+// histogram (a digit needs all of the digits before it) and one that plans.
+// Every chunk leaves its histogram by itself and the next launch adds them up:
+// adding them in memory costs more (64 chunks' atomics to the same bins from
+// all XCDs: 10 us a launch), and needs a cleared array.  What is left is a few
+// microseconds of latency and instructions a launch, so a thread loads its
+// consecutive rows in vectors, all before the first is used.
 #include "common.h"
 #include "cache.h"
 
@@ -18,31 +27,53 @@
 namespace lc {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kPer = 16;                    // consecutive rows of a thread
-constexpr int kChunk = kThreads * kPer;     // rows of a workgroup
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+
+constexpr int kPer = 16;                // rows of a thread of the long form
+constexpr int kThreads = 512;           // of a workgroup of it
+constexpr int kPart = kThreads * kPer;  // rows that it holds at a time
+constexpr int kParts = 7;               // at most: a chunk's histogram has 16-bit bins
+constexpr int kShortThreads = 1024;
+constexpr int kShortRows = kShortThreads * 16;
 constexpr int kDigits = 3;
 constexpr int kBins = 2048;
 __host__ __device__ constexpr int shift_of(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
+__host__ __device__ constexpr uint32_t digit_mask(int pass) { return pass == 2 ? 1023u : 2047u; }
+// The bits of the digits before a pass.
+__host__ __device__ constexpr uint32_t prefix_mask(int pass) {
+  return pass == 0 ? 0u : ~0u << shift_of(pass - 1);
+}
+
+// The digits of the smallest kept key found so far, and how many of the rows
+// that share them stay.
+struct Cut {
+  uint32_t prefix;
+  int need;
+};
 
 struct EvictArgs {
   int B, C, Hkv, budget, sinks, recent;
+  int chunk;             // rows of a workgroup of the long form, a multiple of kPart
   int chunks_a, chunks;  // chunks of rows below the budget, and of all rows
   const int32_t *lens, *kept, *ends;
   const float* w;
   const int32_t* pos;
   float* w_out;
   int32_t *pos_out, *lens_out;
-  // Workspace, per (sequence, head): histograms, the chunks' (above, equal)
-  // counts, holes and movers, the number of moves.
-  uint32_t* hist;
-  int2* counts;
-  int32_t *holes, *movers, *moves;
+  // Workspace, per (sequence, head): the chunks' histograms of each pass, the
+  // cuts, the chunks' rows above the last pass's prefix, holes and movers, the
+  // number of moves.
+  uint16_t* hist;  // [pass][head][chunk][bin]
+  Cut* cuts;
+  int32_t *above, *holes, *movers, *moves;
   int half;  // room of holes and movers
 };
 
 struct RowInfo {
   int b, L, kept, end;
+  int recent_from;  // positions from here on are protected
 };
 __device__ __forceinline__ RowInfo row_info(const EvictArgs& a, int bh) {
   RowInfo r;
@@ -50,20 +81,68 @@ __device__ __forceinline__ RowInfo row_info(const EvictArgs& a, int bh) {
   r.L = max(0, min(a.lens[r.b], a.C));
   r.kept = a.kept ? min(a.kept[r.b], r.L) : 0;
   r.end = a.ends ? a.ends[r.b] : r.L;
+  r.recent_from = (int)max((int64_t)r.end - a.recent, (int64_t)INT32_MIN);
   return r;
 }
 __device__ __forceinline__ int position(const EvictArgs& a, const RowInfo& r, int64_t base, int j) {
   return j < r.kept ? a.pos[base + j] : (int)((int64_t)r.end - r.L + j);
 }
-// The rank of row j: larger stays longer.
-__device__ __forceinline__ uint32_t rank_key(const EvictArgs& a, const RowInfo& r, int64_t base,
-                                             int j) {
-  const int p = position(a, r, base, j);
-  if (p < a.sinks || (int64_t)p >= (int64_t)r.end - a.recent) return 0xffffffffu;
-  const float w = a.w[base + j];
-  if (w != w) return 0u;
-  const uint32_t u = __float_as_uint(w + 0.f);  // -0 counts as 0
-  return u >> 31 ? ~u : u | 0x80000000u;
+// A key that orders as the weights do (-0 as 0), NaN below all.
+__device__ __forceinline__ uint32_t weight_key(float w) {
+  const uint32_t u = __float_as_uint(w + 0.f);
+  const uint32_t k = u ^ (uint32_t)((int32_t)u >> 31 | (int32_t)0x80000000);
+  return w != w ? 0u : k;
+}
+constexpr uint32_t kProtected = 0xffffffffu;
+
+// The weights, positions and keys of a thread's P rows from `first` on, n of
+// them below row hi (keys past them: 0).
+template <int P>
+struct Rows {
+  float w[P];
+  int pos[P];
+  uint32_t key[P];
+  int n;
+};
+template <int P>
+__device__ __forceinline__ void load_rows(const EvictArgs& a, const RowInfo& r, int64_t base, int first,
+                                          int hi, Rows<P>& x) {
+  x.n = max(0, min(hi - first, P));
+  if (x.n == P) {
+    const float* p = a.w + base + first;
+#pragma unroll
+    for (int i = 0; i < P; i += 4) {
+      const f32x4u v = *reinterpret_cast<const f32x4u*>(p + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x.w[i + e] = v[e];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < P; ++i) x.w[i] = i < x.n ? a.w[base + first + i] : 0.f;
+  }
+  const int p0 = (int)((int64_t)r.end - r.L + first);
+#pragma unroll
+  for (int i = 0; i < P; ++i) x.pos[i] = p0 + i;
+  if (x.n > 0 && first < r.kept) {
+    int old[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) old[i] = a.pos[base + min(first + i, r.kept - 1)];
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+      if (first + i < r.kept) x.pos[i] = old[i];
+  }
+#pragma unroll
+  for (int i = 0; i < P; ++i) x.key[i] = weight_key(x.w[i]);
+  if (first < r.kept || p0 < a.sinks || (int64_t)p0 + P > r.recent_from) {  // elsewhere none is protected
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+      if (x.pos[i] < a.sinks || x.pos[i] >= r.recent_from) x.key[i] = kProtected;
+  }
+  if (x.n < P) {
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+      if (i >= x.n) x.key[i] = 0u;
+  }
 }
 
 // Rows of a chunk: those below the budget and those from it on lie in
@@ -75,130 +154,272 @@ __device__ __forceinline__ Chunk chunk_of(const EvictArgs& a, int x, int L) {
   Chunk c;
   const int n = min(a.budget, L);
   if (x < a.chunks_a) {
-    c.lo = min(x * kChunk, n);
-    c.hi = min(c.lo + kChunk, n);
+    c.lo = (int)min((int64_t)x * a.chunk, (int64_t)n);
+    c.hi = (int)min((int64_t)c.lo + a.chunk, (int64_t)n);
   } else {
-    c.lo = (int)min((int64_t)a.budget + (int64_t)(x - a.chunks_a) * kChunk, (int64_t)L);
-    c.hi = (int)min((int64_t)c.lo + kChunk, (int64_t)L);
+    c.lo = (int)min((int64_t)a.budget + (int64_t)(x - a.chunks_a) * a.chunk, (int64_t)L);
+    c.hi = (int)min((int64_t)c.lo + a.chunk, (int64_t)L);
   }
   return c;
 }
 
-// Exclusive prefix sum of x over the workgroup, and the sum of all.
-__device__ __forceinline__ int2 block_scan(int x, int* part) {
+// Inclusive prefix sum over a wave's lanes with DPP: within the rows of 16 lanes
+// by shifts of 1, 2, 4 and 8, then the last lane of row 0 (2) into row 1 (3),
+// and lane 31 into the upper half.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int dpp_add(int x) {
+  return x + __builtin_amdgcn_update_dpp(0, x, kCtrl, kRows, 0xf, true);
+}
+__device__ __forceinline__ int wave_scan(int x) {
+  x = dpp_add<0x111, 0xf>(x);
+  x = dpp_add<0x112, 0xf>(x);
+  x = dpp_add<0x114, 0xf>(x);
+  x = dpp_add<0x118, 0xf>(x);
+  x = dpp_add<0x142, 0xa>(x);
+  return dpp_add<0x143, 0xc>(x);
+}
+
+// Exclusive prefix sums of x over a workgroup of NT threads, and the sum.
+struct Scan {
+  int before, all;
+};
+template <int NT>
+__device__ __forceinline__ Scan block_scan(int x, int* part) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int inc = x;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int y = __shfl_up(inc, off, 64);
-    if (lane >= off) inc += y;
-  }
+  const int inc = wave_scan(x);
   __syncthreads();  // part may still be in use
   if (lane == 63) part[wave] = inc;
   __syncthreads();
-  int before = 0, all = 0;
+  Scan s{inc - x, 0};
 #pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) {
-    if (w < wave) before += part[w];
-    all += part[w];
+  for (int w = 0; w < NT / 64; ++w) {
+    const int y = part[w];
+    if (w < wave) s.before += y;
+    s.all += y;
   }
-  return make_int2(before + inc - x, all);
+  return s;
 }
 
-// The digits of the smallest kept key found so far, and how many of the rows
-// that share them stay.
-struct Cut {
-  uint32_t prefix;
-  int need;
-};
-// From the histograms of the passes before `passes`; by the whole workgroup.
-__device__ __forceinline__ Cut find_cut(const EvictArgs& a, int bh, int passes, int* part, int* pick) {
-  Cut cut{0u, a.budget};
-  for (int p = 0; p < passes; ++p) {
-    const uint32_t* h = a.hist + ((int64_t)bh * kDigits + p) * kBins;
-    // Bins from the top: thread t holds 8 of them, the largest first.
-    int cnt[kBins / kThreads], sum = 0;
+// Adds the digits of a thread's keys that share the prefix to the histogram h
+// (in LDS); keys that agree (many equal weights) are added at once.
+template <int P>
+__device__ __forceinline__ void count_digits(const Rows<P>& x, uint32_t prefix, int pass, uint32_t* h) {
+  if (x.n == 0) return;
+  const uint32_t mask = prefix_mask(pass);
+  uint32_t diff = 0;
 #pragma unroll
-    for (int i = 0; i < kBins / kThreads; ++i) {
-      cnt[i] = (int)h[kBins - 1 - (threadIdx.x * (kBins / kThreads) + i)];
-      sum += cnt[i];
-    }
-    int above = block_scan(sum, part).x;
-#pragma unroll
-    for (int i = 0; i < kBins / kThreads; ++i) {
-      if (above < cut.need && above + cnt[i] >= cut.need) {
-        pick[0] = kBins - 1 - (threadIdx.x * (kBins / kThreads) + i);
-        pick[1] = cut.need - above;
-      }
-      above += cnt[i];
-    }
-    __syncthreads();
-    cut.prefix |= (uint32_t)pick[0] << shift_of(p);
-    cut.need = pick[1];
-    __syncthreads();
+  for (int i = 1; i < P; ++i)
+    if (i < x.n) diff |= x.key[i] ^ x.key[0];
+  if (diff >> shift_of(pass) == 0) {
+    if ((x.key[0] & mask) == prefix)
+      atomicAdd(&h[x.key[0] >> shift_of(pass) & digit_mask(pass)], (uint32_t)x.n);
+    return;
   }
+#pragma unroll
+  for (int i = 0; i < P; ++i)
+    if (i < x.n && (x.key[i] & mask) == prefix)
+      atomicAdd(&h[x.key[i] >> shift_of(pass) & digit_mask(pass)], 1u);
+}
+
+// The bin that the cut falls into; by the whole workgroup, thread t with the
+// counts of bins kBins - 1 - t * kOwn - i.  need: rows that stay of those
+// counted (1 .. their number).
+template <int NT>
+__device__ __forceinline__ Cut narrow(Cut cut, const int (&cnt)[kBins / NT], int pass, int* part,
+                                      int* pick) {
+  constexpr int kOwn = kBins / NT;
+  int sum = 0;
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) sum += cnt[i];
+  int over = block_scan<NT>(sum, part).before;
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) {
+    if (over < cut.need && over + cnt[i] >= cut.need) {
+      pick[0] = kBins - 1 - (threadIdx.x * kOwn + i);
+      pick[1] = cut.need - over;
+    }
+    over += cnt[i];
+  }
+  __syncthreads();
+  cut.prefix |= (uint32_t)pick[0] << shift_of(pass);
+  cut.need = pick[1];
   return cut;
 }
 
-__global__ __launch_bounds__(kThreads) void evict_clear_kernel(uint32_t* hist, int64_t n) {
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (i < n) hist[i] = 0;
-}
-
-// Histogram of digit `pass` of the keys that share the digits before it.
-__global__ __launch_bounds__(kThreads) void evict_hist_kernel(EvictArgs a, int pass) {
-  __shared__ uint32_t h[kBins];
-  __shared__ int part[kThreads / 64], pick[2];
-  const int bh = blockIdx.x / a.chunks, x = blockIdx.x - bh * a.chunks;
-  const RowInfo r = row_info(a, bh);
-  const Chunk c = chunk_of(a, x, r.L);
-  if (r.L <= a.budget || c.lo >= c.hi) return;
-  for (int i = threadIdx.x; i < kBins; i += kThreads) h[i] = 0;
-  const Cut cut = find_cut(a, bh, pass, part, pick);
-  __syncthreads();
-  const int64_t base = (int64_t)bh * a.C;
-  const int sh = shift_of(pass);
-  const uint32_t mask = pass == 0 ? 0u : ~0u << shift_of(pass - 1);
-  const uint32_t digit = pass == 2 ? 1023u : 2047u;
-  for (int j = c.lo + threadIdx.x; j < c.hi; j += kThreads) {
-    const uint32_t k = rank_key(a, r, base, j);
-    if ((k & mask) == cut.prefix) atomicAdd(&h[k >> sh & digit], 1u);
+// Which of a thread's rows stay.  left: of the rows with the cut's own key, how
+// many still stay from its first row on.
+template <int P>
+__device__ __forceinline__ uint32_t staying(const Rows<P>& x, uint32_t cut, int left) {
+  uint32_t keep = 0;
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    if (i >= x.n) continue;
+    const bool same = x.key[i] == cut;
+    keep |= (uint32_t)(x.key[i] > cut || (same && left > 0)) << i;
+    left -= same;
   }
-  __syncthreads();
-  uint32_t* out = a.hist + ((int64_t)bh * kDigits + pass) * kBins;
-  for (int i = threadIdx.x; i < kBins; i += kThreads)
-    if (h[i]) atomicAdd(&out[i], h[i]);  // whole numbers: the order does not matter
+  return keep;
+}
+template <int P>
+__device__ __forceinline__ int equal_rows(const Rows<P>& x, uint32_t cut) {
+  int eq = 0;
+#pragma unroll
+  for (int i = 0; i < P; ++i) eq += i < x.n && x.key[i] == cut;
+  return eq;
 }
 
-// How many of a chunk's rows rank above the smallest kept key, and how many have it.
-__global__ __launch_bounds__(kThreads) void evict_count_kernel(EvictArgs a) {
+// Writes the weights and positions of the rows from lo on, below hi, whose bit
+// is set in keep (in LDS, P rows a word): consecutive lanes, consecutive rows
+// (thread by thread the 2 x 16 stores of a wave touch 64 lines each: 8 us).
+// Inputs may be the outputs: a thread reads all its rows first.
+template <int P, int NT>
+__device__ __forceinline__ void write_kept(const EvictArgs& a, const RowInfo& r, int64_t base, int lo,
+                                           int hi, const uint32_t* keep) {
+  float w[P];
+  int p[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const int j = min(lo + (int)threadIdx.x + i * NT, hi - 1);
+    w[i] = a.w[base + j];
+    p[i] = position(a, r, base, j);
+  }
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const int x = threadIdx.x + i * NT;
+    if (lo + x >= hi || !(keep[x / P] >> (x % P) & 1)) continue;
+    a.w_out[base + lo + x] = w[i];
+    a.pos_out[base + lo + x] = p[i];
+  }
+}
+
+// A whole head, P rows a thread.
+template <int P>
+__global__ __launch_bounds__(kShortThreads) void evict_short_kernel(EvictArgs a) {
+  constexpr int NT = kShortThreads;
+  __shared__ uint32_t h[kDigits][kBins], keep_s[NT];
+  __shared__ int part[NT / 64], pick[2];
+  const int bh = blockIdx.x;
+  const RowInfo r = row_info(a, bh);
+  const int64_t base = (int64_t)bh * a.C;
+  if (bh % a.Hkv == 0 && threadIdx.x == 0) a.lens_out[r.b] = min(r.L, a.budget);
+  Rows<P> x;
+  const int first = threadIdx.x * P;
+  load_rows<P>(a, r, base, first, r.L, x);
+  uint32_t keep = ~0u;
+  if (r.L > a.budget) {
+    for (int i = threadIdx.x; i < kDigits * kBins; i += NT) (&h[0][0])[i] = 0;
+    __syncthreads();
+    Cut cut{0u, a.budget};
+#pragma unroll
+    for (int pass = 0; pass < kDigits; ++pass) {
+      count_digits<P>(x, cut.prefix, pass, h[pass]);
+      __syncthreads();
+      int cnt[kBins / NT];
+#pragma unroll
+      for (int i = 0; i < kBins / NT; ++i) cnt[i] = (int)h[pass][kBins - 1 - (threadIdx.x * (kBins / NT) + i)];
+      cut = narrow<NT>(cut, cnt, pass, part, pick);
+    }
+    const int left = cut.need - block_scan<NT>(equal_rows<P>(x, cut.prefix), part).before;
+    keep = staying<P>(x, cut.prefix, left);
+  }
+  // Holes below the budget in the low half, movers from it on in the high half:
+  // at most kShortRows / 2 of each.
+  int both = 0;
+#pragma unroll
+  for (int i = 0; i < P; ++i)
+    if (i < x.n && (first + i < a.budget) != (keep >> i & 1)) both += first + i < a.budget ? 1 : 1 << 16;
+  const Scan s = block_scan<NT>(both, part);
+  if (threadIdx.x == 0) a.moves[bh] = s.all & 0xffff;
+  int at = s.before & 0xffff, am = s.before >> 16;
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    if (i >= x.n) continue;
+    const int j = first + i;
+    const bool stay = keep >> i & 1;
+    if (j < a.budget && !stay) a.holes[(int64_t)bh * a.half + at++] = j;
+    if (j >= a.budget && stay) a.movers[(int64_t)bh * a.half + am++] = j;
+  }
+  keep_s[threadIdx.x] = keep;
+  __syncthreads();
+  const int hi = min(r.L, a.budget);
+  if (hi > 0) write_kept<P, NT>(a, r, base, 0, hi, keep_s);
+}
+
+// The bins of a thread in histogram `pass` of a chunk, from the top.
+__device__ __forceinline__ u16x4 chunk_bins(const EvictArgs& a, int bh, int pass, int chunk) {
+  static_assert(kBins / kThreads == 4 && digit_mask(kDigits - 1) == 16 * 64 - 1, "bins of a thread, of a lane");
+  const int64_t at = (((int64_t)pass * a.B * a.Hkv + bh) * a.chunks + chunk) * kBins;
+  const u16x4 v = *reinterpret_cast<const u16x4*>(a.hist + at + kBins - 4 - 4 * threadIdx.x);
+  return u16x4{v[3], v[2], v[1], v[0]};
+}
+
+// The cut after `passes` passes: the last histogram, added up over the chunks,
+// narrows the cut stored by the launch before; the first workgroup of a head
+// stores the new one.
+__device__ __forceinline__ Cut cut_after(const EvictArgs& a, int bh, int passes, int* part, int* pick) {
+  Cut cut{0u, a.budget};
+  if (passes == 0) return cut;
+  int cnt[4] = {0, 0, 0, 0};
+#pragma unroll 16
+  for (int x = 0; x < a.chunks; ++x) {
+    const u16x4 v = chunk_bins(a, bh, passes - 1, x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) cnt[i] += v[i];
+  }
+  if (passes > 1) cut = a.cuts[bh * kDigits + passes - 2];
+  cut = narrow<kThreads>(cut, cnt, passes - 1, part, pick);
+  if (blockIdx.x % a.chunks == 0 && threadIdx.x == 0) a.cuts[bh * kDigits + passes - 1] = cut;
+  return cut;
+}
+
+// Histogram of digit PASS of a chunk's keys that share the digits before it.
+template <int PASS>
+__global__ __launch_bounds__(kThreads) void evict_hist_kernel(EvictArgs a) {
+  __shared__ __attribute__((aligned(16))) uint32_t h[kBins];
   __shared__ int part[kThreads / 64], pick[2];
   const int bh = blockIdx.x / a.chunks, x = blockIdx.x - bh * a.chunks;
   const RowInfo r = row_info(a, bh);
   if (r.L <= a.budget) return;
   const Chunk c = chunk_of(a, x, r.L);
-  const Cut cut = find_cut(a, bh, kDigits, part, pick);
   const int64_t base = (int64_t)bh * a.C;
-  int gt = 0, eq = 0;
-  for (int j = c.lo + threadIdx.x; j < c.hi; j += kThreads) {
-    const uint32_t k = rank_key(a, r, base, j);
-    gt += k > cut.prefix;
-    eq += k == cut.prefix;
+  Rows<kPer> rows;
+  load_rows<kPer>(a, r, base, c.lo + threadIdx.x * kPer, c.hi, rows);
+  for (int i = threadIdx.x; i < kBins; i += kThreads) h[i] = 0;
+  const Cut cut = cut_after(a, bh, PASS, part, pick);
+  __syncthreads();
+  int over = 0;  // rows above the prefix
+  for (int lo = c.lo;;) {
+    count_digits<kPer>(rows, cut.prefix, PASS, h);
+    if constexpr (PASS == kDigits - 1)
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) over += i < rows.n && (rows.key[i] & prefix_mask(PASS)) > cut.prefix;
+    lo += kPart;
+    if (lo >= c.hi) break;
+    load_rows<kPer>(a, r, base, lo + threadIdx.x * kPer, c.hi, rows);
   }
-  const int gts = block_scan(gt, part).y, eqs = block_scan(eq, part).y;
-  if (threadIdx.x == 0) a.counts[(int64_t)bh * a.chunks + x] = make_int2(gts, eqs);
+  if constexpr (PASS == kDigits - 1) {
+    const int all = block_scan<kThreads>(over, part).all;
+    if (threadIdx.x == 0) a.above[(int64_t)bh * a.chunks + x] = all;
+  }
+  __syncthreads();
+  const int64_t at = (((int64_t)PASS * a.B * a.Hkv + bh) * a.chunks + x) * kBins;
+  const u32x4 v = *reinterpret_cast<const u32x4*>(h + 4 * threadIdx.x);
+  *reinterpret_cast<u16x4*>(a.hist + at + 4 * threadIdx.x) =
+      u16x4{(uint16_t)v[0], (uint16_t)v[1], (uint16_t)v[2], (uint16_t)v[3]};
 }
 
-// Which rows of a chunk stay, and the holes or movers among them.
-__global__ __launch_bounds__(kThreads) void evict_plan_kernel(EvictArgs a) {
+// Which rows of a chunk stay, and the holes or movers among them.  (Two
+// workgroups a CU: 33 chunks of eight heads are 264.)
+__global__ __launch_bounds__(kThreads, 4) void evict_plan_kernel(EvictArgs a) {
   __shared__ int part[kThreads / 64], pick[2];
+  __shared__ int over_s[kThreads], eq_s[kThreads], mine[2];
+  __shared__ uint32_t keep_s[kThreads];
   const int bh = blockIdx.x / a.chunks, x = blockIdx.x - bh * a.chunks;
   const RowInfo r = row_info(a, bh);
   const Chunk c = chunk_of(a, x, r.L);
   const int64_t base = (int64_t)bh * a.C;
   const bool lower = x < a.chunks_a;
   if (x == 0 && bh % a.Hkv == 0 && threadIdx.x == 0) a.lens_out[r.b] = min(r.L, a.budget);
-  const int first = c.lo + threadIdx.x * kPer;  // the thread's rows, in order
   if (r.L <= a.budget) {
     for (int j = c.lo + threadIdx.x; j < c.hi; j += kThreads) {
       a.w_out[base + j] = a.w[base + j];
@@ -207,61 +428,96 @@ __global__ __launch_bounds__(kThreads) void evict_plan_kernel(EvictArgs a) {
     if (x == 0 && threadIdx.x == 0) a.moves[bh] = 0;
     return;
   }
-  const Cut cut = find_cut(a, bh, kDigits, part, pick);
-  // Over the chunks before this one: rows with the smallest kept key, then
-  // (with how many of those stay) the holes or movers.
-  int eq_before = 0;
+  Rows<kPer> rows;
+  load_rows<kPer>(a, r, base, c.lo + threadIdx.x * kPer, c.hi, rows);
+  const Cut cut = cut_after(a, bh, kDigits, part, pick);
+  const int bin = (int)(cut.prefix & digit_mask(kDigits - 1));
+  // Over the chunks before this one: rows with the cut's key and, with how many
+  // of those stay in each, the holes or movers.
+  int eq_before = 0, before = 0, all = 0, eq_run = 0;
   for (int i0 = 0; i0 < a.chunks; i0 += kThreads) {
-    const int i = i0 + threadIdx.x;
-    eq_before += block_scan(i < x ? a.counts[(int64_t)bh * a.chunks + i].y : 0, part).y;
-  }
-  int before = 0, all = 0, eq_run = 0;
-  for (int i0 = 0; i0 < a.chunks; i0 += kThreads) {
-    const int i = i0 + threadIdx.x;
-    const int2 n = i < a.chunks ? a.counts[(int64_t)bh * a.chunks + i] : make_int2(0, 0);
-    const int2 e = block_scan(n.y, part);
-    const int stay = n.x + min(max(cut.need - eq_run - e.x, 0), n.y);
-    eq_run += e.y;
+    const int cn = min(kThreads, a.chunks - i0), i = i0 + threadIdx.x;
+    __syncthreads();
+    over_s[threadIdx.x] = i < a.chunks ? a.above[(int64_t)bh * a.chunks + i] : 0;
+    eq_s[threadIdx.x] = 0;
+    __syncthreads();
+    // A wave takes a chunk's histogram (the last digit has 1,024 bins), 16 bins a
+    // lane; the chunks of a wave are read together, kEach at a time.  Few rows
+    // share all the digits before, so most lanes find nothing.
+    constexpr int kEach = 5;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int y0 = wave; y0 < cn; y0 += kEach * (kThreads / 64)) {
+      u32x4 v[kEach][2];
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int y = min(y0 + e * (kThreads / 64), cn - 1);
+        const int64_t at = (((int64_t)(kDigits - 1) * a.B * a.Hkv + bh) * a.chunks + i0 + y) * kBins;
+        v[e][0] = *reinterpret_cast<const u32x4*>(a.hist + at + 16 * lane);
+        v[e][1] = *reinterpret_cast<const u32x4*>(a.hist + at + 16 * lane + 8);
+      }
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int y = y0 + e * (kThreads / 64);
+        const u32x4 any = v[e][0] | v[e][1];
+        if (y >= cn || (any[0] | any[1] | any[2] | any[3]) == 0 || 16 * lane + 15 < bin) continue;
+        int over = 0, eq = 0;
+#pragma unroll
+        for (int i2 = 0; i2 < 16; ++i2) {
+          const int n = (int)(v[e][i2 >> 3][(i2 >> 1) & 3] >> 16 * (i2 & 1) & 0xffffu);
+          over += 16 * lane + i2 > bin ? n : 0;
+          eq += 16 * lane + i2 == bin ? n : 0;
+        }
+        if (over != 0) atomicAdd(&over_s[y], over);
+        if (eq != 0) eq_s[y] = eq;  // one lane has the bin
+      }
+    }
+    __syncthreads();
+    const int over = over_s[threadIdx.x], eq = eq_s[threadIdx.x];
+    const Scan e = block_scan<kThreads>(eq, part);
+    const int stay = over + min(max(cut.need - eq_run - e.before, 0), eq);
     int cnt = 0;
     if (i < a.chunks && (i < a.chunks_a) == lower) {
       const Chunk ci = chunk_of(a, i, r.L);
       cnt = lower ? ci.hi - ci.lo - stay : stay;
     }
-    before += block_scan(i < x ? cnt : 0, part).y;
-    all += block_scan(cnt, part).y;
-  }
-  if (x == 0 && threadIdx.x == 0) a.moves[bh] = all;  // holes
-  uint32_t key[kPer];
-  int eq = 0;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    key[i] = first + i < c.hi ? rank_key(a, r, base, first + i) : 0u;
-    eq += first + i < c.hi && key[i] == cut.prefix;
-  }
-  int left = cut.need - eq_before - block_scan(eq, part).x;  // equal rows that still stay
-  uint32_t keep = 0;
-  int listed = 0;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    if (first + i >= c.hi) continue;
-    const bool same = key[i] == cut.prefix;
-    const bool k = key[i] > cut.prefix || (same && left > 0);
-    left -= same;
-    keep |= (uint32_t)k << i;
-    listed += k != lower;
-  }
-  int at = before + block_scan(listed, part).x;
-  int32_t* list = (lower ? a.holes : a.movers) + (int64_t)bh * a.half;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int j = first + i;
-    if (j >= c.hi) continue;
-    const bool k = keep >> i & 1;
-    if (k != lower) list[at++] = j;
-    if (k && lower) {
-      a.w_out[base + j] = a.w[base + j];
-      a.pos_out[base + j] = position(a, r, base, j);
+    const Scan s = block_scan<kThreads>(cnt, part);
+    if (i == x) {
+      mine[0] = eq_run + e.before;
+      mine[1] = all + s.before;
     }
+    eq_run += e.all;
+    all += s.all;
+  }
+  __syncthreads();
+  eq_before = mine[0];
+  before = mine[1];
+  if (x == 0 && threadIdx.x == 0) a.moves[bh] = all;  // holes
+  int32_t* list = (lower ? a.holes : a.movers) + (int64_t)bh * a.half;
+  for (int lo = c.lo;;) {
+    const Scan e = block_scan<kThreads>(equal_rows<kPer>(rows, cut.prefix), part);
+    const uint32_t keep = staying<kPer>(rows, cut.prefix, cut.need - eq_before - e.before);
+    int listed = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) listed += i < rows.n && lower != (keep >> i & 1);
+    const Scan s = block_scan<kThreads>(listed, part);
+    int at = before + s.before;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (i >= rows.n) continue;
+      const int j = lo + threadIdx.x * kPer + i;
+      if ((bool)(keep >> i & 1) != lower) list[at++] = j;
+    }
+    if (lower && lo < c.hi) {  // the whole workgroup
+      __syncthreads();  // keep_s may still be in use
+      keep_s[threadIdx.x] = keep;
+      __syncthreads();
+      write_kept<kPer, kThreads>(a, r, base, lo, c.hi, keep_s);
+    }
+    eq_before += e.all;
+    before += s.all;
+    lo += kPart;
+    if (lo >= c.hi) break;
+    load_rows<kPer>(a, r, base, lo + threadIdx.x * kPer, c.hi, rows);
   }
 }
 
@@ -272,26 +528,39 @@ struct MoveArgs {
   int blocks;              // workgroups of a (sequence, head)
 };
 
-// Thread: one 16-byte chunk of K and V of a move.
-__global__ __launch_bounds__(kThreads) void evict_move_kernel(EvictArgs a, MoveArgs t) {
+// Thread: 16-byte chunks of K and V of moved rows, kMoves at a time.
+constexpr int kMoveThreads = 256;
+__global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a, MoveArgs t) {
+  constexpr int kMoves = 4;
   const int bh = blockIdx.x / t.blocks, x = blockIdx.x - bh * t.blocks;
   const int n = a.moves[bh];
   if (n == 0) return;
   const RowInfo r = row_info(a, bh);
   const int64_t base = (int64_t)bh * a.C;
   const int64_t off = r.b * t.seq + (bh % a.Hkv) * t.head;
-  const int64_t total = (int64_t)n * t.chunks;
-  for (int64_t i = (int64_t)x * kThreads + threadIdx.x; i < total; i += (int64_t)t.blocks * kThreads) {
-    const int mv = (int)(i / t.chunks), ch = (int)(i - (int64_t)mv * t.chunks);
-    const int dst = a.holes[(int64_t)bh * a.half + mv], src = a.movers[(int64_t)bh * a.half + mv];
-    const int64_t so = off + src * t.row + 16 * ch, d = off + dst * t.row + 16 * ch;
-    const uint4 kx = *reinterpret_cast<const uint4*>(t.k + so);
-    const uint4 vx = *reinterpret_cast<const uint4*>(t.v + so);
-    *reinterpret_cast<uint4*>(t.k + d) = kx;
-    *reinterpret_cast<uint4*>(t.v + d) = vx;
-    if (ch == 0) {
-      a.w_out[base + dst] = a.w[base + src];
-      a.pos_out[base + dst] = position(a, r, base, src);
+  const int64_t total = (int64_t)n * t.chunks, step = (int64_t)t.blocks * kMoveThreads;
+  for (int64_t i0 = (int64_t)x * kMoveThreads + threadIdx.x; i0 < total; i0 += kMoves * step) {
+    int64_t d[kMoves];
+    u32x4 kx[kMoves], vx[kMoves];
+#pragma unroll
+    for (int e = 0; e < kMoves; ++e) {
+      const int64_t i = min(i0 + e * step, total - 1);  // past the end: the last again, not stored
+      const int mv = (int)(i / t.chunks), ch = (int)(i - (int64_t)mv * t.chunks);
+      const int dst = a.holes[(int64_t)bh * a.half + mv], src = a.movers[(int64_t)bh * a.half + mv];
+      const int64_t s = off + src * t.row + 16 * ch;
+      d[e] = off + dst * t.row + 16 * ch;
+      kx[e] = *reinterpret_cast<const u32x4*>(t.k + s);
+      vx[e] = *reinterpret_cast<const u32x4*>(t.v + s);
+      if (ch == 0 && i0 + e * step < total) {
+        a.w_out[base + dst] = a.w[base + src];
+        a.pos_out[base + dst] = position(a, r, base, src);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < kMoves; ++e) {
+      if (i0 + e * step >= total) continue;
+      *reinterpret_cast<u32x4*>(t.k + d[e]) = kx[e];
+      *reinterpret_cast<u32x4*>(t.v + d[e]) = vx[e];
     }
   }
 }
@@ -315,7 +584,7 @@ __global__ __launch_bounds__(256) void cache_commit_kernel(CommitArgs a) {
   int last = -1, n = 0;
   bool on = true;
   for (int j0 = 0; j0 < a.P && on; j0 += 8) {
-    uint4 x[8];
+    u32x4 x[8];
     int src[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -325,32 +594,39 @@ __global__ __launch_bounds__(256) void cache_commit_kernel(CommitArgs a) {
       if (on) {
         last = p;
         ++n;
-        if (moves && p != j0 + e) x[e] = *reinterpret_cast<const uint4*>(base + p * a.row);
+        if (moves && p != j0 + e) x[e] = *reinterpret_cast<const u32x4*>(base + p * a.row);
       }
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (moves && src[e] >= 0 && src[e] != j0 + e)
-        *reinterpret_cast<uint4*>(base + (j0 + e) * a.row) = x[e];
+        *reinterpret_cast<u32x4*>(base + (j0 + e) * a.row) = x[e];
   }
   if (a.lens_out && hc == 0 && blockIdx.y == 0 && blockIdx.z == 0)
     a.lens_out[b] = past < 0 ? past : past + n;
 }
 
 struct Layout {
-  int chunks_max, half;
-  size_t hist, counts, list, moves, total;
+  int chunk, chunks_max, half;
+  size_t hist, cuts, above, list, moves, total;
 };
 Layout layout_of(int B, int Hkv, int C) {
-  Layout y;
+  Layout y{};
   const size_t bh = (size_t)B * Hkv;
-  y.chunks_max = (C + kChunk - 1) / kChunk + 1;  // whatever the budget
-  y.half = C / 2 + 1;                            // moves: at most min(budget, C - budget)
-  y.hist = bh * kDigits * kBins * 4;
-  y.counts = (bh * y.chunks_max * 8 + 15) / 16 * 16;
-  y.list = (bh * y.half * 4 + 15) / 16 * 16;
-  y.moves = (bh * 4 + 15) / 16 * 16;
-  y.total = y.hist + y.counts + 2 * y.list + y.moves;
+  // Chunks of the long form: some 32 a head, each WG adds up all of them.
+  const int64_t parts = std::min<int64_t>(kParts, (C + 32LL * kPart - 1) / (32LL * kPart));
+  y.chunk = (int)(parts * kPart);
+  y.chunks_max = (int)(((int64_t)C + y.chunk - 1) / y.chunk + 1);  // whatever the budget
+  y.half = C / 2 + 1;  // moves: at most min(budget, C - budget)
+  auto up = [](size_t n) { return (n + 15) / 16 * 16; };
+  if (C > kShortRows) {
+    y.hist = up(kDigits * bh * y.chunks_max * kBins * sizeof(uint16_t));
+    y.cuts = up(bh * kDigits * sizeof(Cut));
+    y.above = up(bh * y.chunks_max * 4);
+  }
+  y.list = up(bh * y.half * 4);
+  y.moves = up(bh * 4);
+  y.total = y.hist + y.cuts + y.above + 2 * y.list + y.moves;
   return y;
 }
 
@@ -368,8 +644,9 @@ hipError_t launch_cache_evict(const EvictProblem& p, void* ws, hipStream_t s) {
   a.budget = p.budget;
   a.sinks = p.sinks;
   a.recent = p.recent;
-  a.chunks_a = (p.budget + kChunk - 1) / kChunk;
-  a.chunks = a.chunks_a + (p.C - p.budget + kChunk - 1) / kChunk;
+  a.chunk = y.chunk;
+  a.chunks_a = (int)(((int64_t)p.budget + y.chunk - 1) / y.chunk);
+  a.chunks = a.chunks_a + (int)(((int64_t)p.C - p.budget + y.chunk - 1) / y.chunk);
   a.lens = p.lens;
   a.kept = p.kept;
   a.ends = p.ends;
@@ -379,22 +656,29 @@ hipError_t launch_cache_evict(const EvictProblem& p, void* ws, hipStream_t s) {
   a.pos_out = p.pos_out;
   a.lens_out = p.lens_out;
   uint8_t* at = static_cast<uint8_t*>(ws);
-  a.hist = reinterpret_cast<uint32_t*>(at);
-  a.counts = reinterpret_cast<int2*>(at += y.hist);
-  a.holes = reinterpret_cast<int32_t*>(at += y.counts);
+  a.hist = reinterpret_cast<uint16_t*>(at);
+  a.cuts = reinterpret_cast<Cut*>(at += y.hist);
+  a.above = reinterpret_cast<int32_t*>(at += y.cuts);
+  a.holes = reinterpret_cast<int32_t*>(at += y.above);
   a.movers = reinterpret_cast<int32_t*>(at += y.list);
   a.moves = reinterpret_cast<int32_t*>(at += y.list);
   a.half = y.half;
-  const dim3 grid((unsigned)(bh * a.chunks)), block(kThreads);
-  if (p.C > p.budget) {
-    const int64_t n = (int64_t)bh * kDigits * kBins;
-    hipLaunchKernelGGL(evict_clear_kernel, dim3((unsigned)((n + kThreads - 1) / kThreads)), block, 0, s,
-                       a.hist, n);
-    for (int pass = 0; pass < kDigits; ++pass)
-      hipLaunchKernelGGL(evict_hist_kernel, grid, block, 0, s, a, pass);
-    hipLaunchKernelGGL(evict_count_kernel, grid, block, 0, s, a);
+  if (p.C <= kShortRows) {
+    auto whole = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)bh), dim3(kShortThreads), 0, s, a);
+    };
+    if (p.C <= kShortRows / 4) whole(evict_short_kernel<4>);
+    else if (p.C <= kShortRows / 2) whole(evict_short_kernel<8>);
+    else whole(evict_short_kernel<16>);
+  } else {
+    const dim3 grid((unsigned)(bh * a.chunks)), block(kThreads);
+    if (p.C > p.budget) {
+      hipLaunchKernelGGL(evict_hist_kernel<0>, grid, block, 0, s, a);
+      hipLaunchKernelGGL(evict_hist_kernel<1>, grid, block, 0, s, a);
+      hipLaunchKernelGGL(evict_hist_kernel<2>, grid, block, 0, s, a);
+    }
+    hipLaunchKernelGGL(evict_plan_kernel, grid, block, 0, s, a);
   }
-  hipLaunchKernelGGL(evict_plan_kernel, grid, block, 0, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.C <= p.budget) return e;
   MoveArgs t;
@@ -405,8 +689,8 @@ hipError_t launch_cache_evict(const EvictProblem& p, void* ws, hipStream_t s) {
   t.head = p.head * p.elem;
   t.chunks = p.D * p.elem / 16;
   const int64_t most = (int64_t)std::min(p.budget, p.C - p.budget) * t.chunks;
-  t.blocks = (int)std::max<int64_t>(1, std::min<int64_t>((most + kThreads - 1) / kThreads, std::max(1, 2048 / bh)));
-  hipLaunchKernelGGL(evict_move_kernel, dim3((unsigned)(bh * t.blocks)), block, 0, s, a, t);
+  t.blocks = (int)std::max<int64_t>(1, std::min<int64_t>((most + kMoveThreads - 1) / kMoveThreads, std::max(1, 2048 / bh)));
+  hipLaunchKernelGGL(evict_move_kernel, dim3((unsigned)(bh * t.blocks)), dim3(kMoveThreads), 0, s, a, t);
   return hipGetLastError();
 }
 
