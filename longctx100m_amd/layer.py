@@ -18,11 +18,12 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
-from typing import Dict, List, Optional, Sequence, Tuple
+from typing import Callable, Dict, List, Optional, Sequence, Tuple
 
 import torch
 
 from . import _lib
+from . import cache as kv
 from . import ring_attention as ra
 from .ring_attention import _dtype_code, _stream
 
@@ -289,12 +290,14 @@ def layer_prefill(x: torch.Tensor, w: Dict[str, torch.Tensor], cfg: ModelConfig,
                   preceding_kv: Sequence[Tuple[torch.Tensor, torch.Tensor]],
                   residual: Optional[torch.Tensor] = None,
                   timers: Optional[Dict[str, list]] = None,
-                  cache: Optional[Tuple[torch.Tensor, torch.Tensor]] = None):
+                  cache: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
+                  observe: Optional[Callable] = None):
     """One decoder layer over this rank's shard x [T, hidden].
 
     ``preceding_kv`` holds the (k, v) [1, T, Hkv, d] shards of ranks 0..rank-1
     (the ring's incoming KV).  ``cache``, when given, is this layer's KV cache
-    ([1, capacity, Hkv, d] K and V) and receives the shard's rotated K and V.  ``residual``, when given, is the previous
+    ([1, capacity, Hkv, d] K and V) and receives the shard's rotated K and V.  ``observe``, when
+    given, is called with the attention's (q [1, T, Hq, d], m, l [1, Hq, T]).  ``residual``, when given, is the previous
     layer's MLP output still to be added to x (the add is fused into this
     layer's first RMSNorm).  Returns (x_after_attention, mlp_out): the layer
     output is their sum, which the next layer's (or the final) RMSNorm forms."""
@@ -328,8 +331,10 @@ def layer_prefill(x: torch.Tensor, w: Dict[str, torch.Tensor], cfg: ModelConfig,
         cache[0][:, :T].copy_(kb)
         cache[1][:, :T].copy_(vb)
     shards = [(qb, pk, pv) for pk, pv in preceding_kv] + [(qb, kb, vb)]
-    attn, _, _ = ra.ring_causal_attention_forward_with_stats(shards, rank)
+    attn, m, l = ra.ring_causal_attention_forward_with_stats(shards, rank)
     tick("attention")
+    if observe is not None:
+        observe(qb, m.view(1, hq, T), l.view(1, hq, T))
     o = torch.matmul(attn.view(T, hq * d), w["wo"].t())
     tick("gemm")
     x2 = torch.empty_like(x)
@@ -419,14 +424,18 @@ def new_cache(cfg: ModelConfig, capacity: int, device, dtype=torch.bfloat16):
 
 
 def model_prefill(ids: torch.Tensor, weights: Dict, cfg: ModelConfig, table: torch.Tensor,
-                  caches=None) -> torch.Tensor:
+                  caches=None, observe: Optional[Callable] = None) -> torch.Tensor:
     """Logits [T, vocab] of a one-rank prefill (embedding, layers, final norm,
-    LM head), filling ``caches`` with each layer's rotated K and V if given."""
+    LM head), filling ``caches`` with each layer's rotated K and V if given.
+    ``observe``, when given, is called with (layer, q, m, l) as layer_prefill
+    calls its own."""
     x = torch.nn.functional.embedding(ids, weights["embed"])
     res = None
     for li, lw in enumerate(weights["layers"]):
         x, res = layer_prefill(x, lw, cfg, table, 0, [], residual=res,
-                               cache=caches[li] if caches is not None else None)
+                               cache=caches[li] if caches is not None else None,
+                               observe=None if observe is None else
+                               lambda q, m, l, li=li: observe(li, q, m, l))
     h = rmsnorm(x, weights["final_norm"], cfg.rms_norm_eps, residual=res)
     return torch.matmul(h, weights["lm_head"].t())
 
@@ -447,6 +456,157 @@ def model_decode_step(token: int, pos: int, weights: Dict, cfg: ModelConfig,
     # (155-161 us against 151 us).
     h = rmsnorm(x, weights["final_norm"], cfg.rms_norm_eps, residual=res)
     return linear(h, weights["lm_head"])
+
+
+# ---------------------------------------------- drafted trees, bounded caches --
+
+def layer_decode_tree(x: torch.Tensor, w: Dict[str, torch.Tensor], cfg: ModelConfig,
+                      rows: torch.Tensor, at: int, past: torch.Tensor, parents: torch.Tensor,
+                      cache: Tuple[torch.Tensor, torch.Tensor],
+                      residual: Optional[torch.Tensor] = None,
+                      workspace: Optional[torch.Tensor] = None,
+                      observe: Optional[Callable] = None):
+    """One decoder layer for a tree of N drafted tokens (x [N, hidden]): their K
+    and V are appended to cache rows at .. at + N - 1 and each token attends to
+    the rows before them, its chain of parents and itself
+    (cache.tree_attention).  ``past`` holds ``at`` and ``parents`` the tree on
+    the device (int32 [1] and [1, N]), ``rows`` the tokens' rows of the RoPE
+    table.  ``observe`` as layer_prefill.  Returns (x_after_attention, mlp_out)
+    as layer_decode."""
+    n = x.shape[0]
+    d, hq, hkv = cfg.head_dim, cfg.num_heads, cfg.num_key_value_heads
+    if residual is not None:
+        xin = torch.empty_like(x)
+        h = rmsnorm(x, w["norm1"], cfg.rms_norm_eps, residual=residual, residual_out=xin)
+    else:
+        xin = x
+        h = rmsnorm(x, w["norm1"], cfg.rms_norm_eps)
+    qkv = linear(h, w["wqkv"])
+    kc, vc = cache
+    q = rope_apply(qkv[:, :hq * d], rows, hq, d).view(1, n, hq, d)
+    rope_apply(qkv[:, hq * d:(hq + hkv) * d], rows, hkv, d, out=kc[0, at:at + n])
+    vc[0, at:at + n].copy_(qkv[:, (hq + hkv) * d:].view(n, hkv, d))
+    attn, m, l = kv.tree_attention(q, kc, vc, past, parents, workspace=workspace)
+    if observe is not None:
+        observe(q, m, l)
+    ao = linear(attn.view(n, hq * d), w["wo"])
+    x2 = torch.empty_like(x)
+    h2 = rmsnorm(xin, w["norm2"], cfg.rms_norm_eps, residual=ao, residual_out=x2)
+    gu = linear(h2, w["wgu"])
+    inter = cfg.intermediate_size
+    a = swiglu(gu[:, :inter], gu[:, inter:])
+    return x2, linear(a, w["wd"])
+
+
+class BoundedCache:
+    """The KV caches of a model's layers for one sequence, decoded by trees of
+    drafted tokens and held to a budget of rows by accumulated attention weight:
+
+        c = BoundedCache(cfg, capacity, device)
+        logits = c.prefill(ids, weights, table)
+        logits = c.decode(draft_ids, parents, weights, table)  # [N, vocab]
+        c.commit(path)           # the nodes that were accepted, root first
+        c.evict(budget)          # e.g. once c.past nears the capacity
+
+    ``past`` rows of each layer are held (in no order once evicted), ``end``
+    tokens have been seen; a new token's RoPE position is ``end`` plus its depth
+    in the tree.  ``weights[layer]`` and ``positions[layer]`` ([1, Hkv, capacity])
+    are the rows' accumulated weights and, up to ``kept`` rows, the positions of
+    the tokens that they hold."""
+
+    def __init__(self, cfg: ModelConfig, capacity: int, device, dtype=torch.bfloat16):
+        self.cfg, self.capacity = cfg, capacity
+        self.caches = new_cache(cfg, capacity, device, dtype)
+        self.layers = kv.Layers.of(self.caches)
+        shape = (1, cfg.num_key_value_heads, capacity)
+        self.weights = [torch.zeros(shape, device=device) for _ in self.caches]
+        self.positions = [torch.zeros(shape, dtype=torch.int32, device=device)
+                          for _ in self.caches]
+        self.past = self.kept = self.end = 0
+        self._device = self.caches[0][0].device
+        self._drafts: List[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = []
+        self._parents: List[int] = []
+
+    def _i32(self, *values: int) -> torch.Tensor:
+        return torch.tensor(values, dtype=torch.int32, device=self._device)
+
+    def prefill(self, ids: torch.Tensor, weights: Dict, table: torch.Tensor,
+                window: int = 512) -> torch.Tensor:
+        """model_prefill of a prompt; its last ``window`` tokens give the rows
+        their first weights."""
+        t = ids.numel()
+        if self.end or t > self.capacity:
+            raise ValueError(f"a prompt of at most {self.capacity} tokens comes first")
+        last = min(window, t)
+        past = self._i32(t - last)
+
+        def observe(li, q, m, l):
+            if last:
+                kv.key_weights(q[:, t - last:].contiguous(), self.caches[li][0], past,
+                               m[..., t - last:].contiguous(), l[..., t - last:].contiguous(),
+                               None, out=self.weights[li])
+
+        logits = model_prefill(ids, weights, self.cfg, table[:t], self.caches, observe)
+        self.past = self.end = t
+        return logits
+
+    def decode(self, ids: torch.Tensor, parents: Sequence[int], weights: Dict,
+               table: torch.Tensor, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Logits [N, vocab] of a tree of drafted tokens (``parents`` as
+        cache.tree_attention's, on the host; at most 256).  The tree stays
+        behind the held rows until :meth:`commit`, or the next call, drops it."""
+        n = ids.numel()
+        if n != len(parents) or not 0 < n <= kv.MAX_TOKENS:
+            raise ValueError(f"a tree has 1 to {kv.MAX_TOKENS} tokens and a parent for each")
+        depths = kv.tree_depths(parents)
+        if self.past + n > self.capacity:
+            raise ValueError(f"{n} tokens behind {self.past} rows exceed the capacity {self.capacity}")
+        if self.end + max(depths) >= table.shape[0]:
+            raise ValueError("the RoPE table ends before the tree")
+        rows = table[self._i32(*[self.end + max(x, 0) for x in depths]).long()]
+        past, tree = self._i32(self.past), self._i32(*parents).view(1, n)
+        self._drafts, self._parents = [], list(parents)
+        x = torch.nn.functional.embedding(ids, weights["embed"])
+        res = None
+        for lw, cache in zip(weights["layers"], self.caches):
+            x, res = layer_decode_tree(x, lw, self.cfg, rows, self.past, past, tree, cache,
+                                       residual=res, workspace=workspace,
+                                       observe=lambda *s: self._drafts.append(s))
+        h = rmsnorm(x, weights["final_norm"], self.cfg.rms_norm_eps, residual=res)
+        return linear(h, weights["lm_head"])
+
+    def commit(self, path: Sequence[int]) -> None:
+        """Keeps the tree's nodes ``path``, a chain from a root down, and drops the
+        others; the kept tokens' attention is added to the rows' weights."""
+        path = list(path)
+        up = -1
+        for p in path:
+            if not 0 <= p < len(self._parents) or self._parents[p] != up:
+                raise ValueError(f"{path} is not a chain of the tree's nodes from a root")
+            up = p
+        if path:
+            past = self._i32(self.past)
+            kv.commit(self.layers, past, self._i32(*path).view(1, -1))
+            at = self._i32(*path).long()
+            for (k, _), w, (q, m, l) in zip(self.caches, self.weights, self._drafts):
+                kv.key_weights(q[:, at], k, past, m[..., at], l[..., at], w, out=w)
+        self.past += len(path)
+        self.end += len(path)
+        self._drafts, self._parents = [], []
+
+    def evict(self, budget: int, sinks: int = 4, recent: int = 64) -> None:
+        """Cuts every layer's cache to ``budget`` rows per KV head (cache.evict);
+        a tree that was not committed is dropped."""
+        self._drafts, self._parents = [], []
+        if self.past <= budget:
+            return
+        lens, kept, ends = (self._i32(x) for x in (self.past, self.kept, self.end))
+        ws = torch.empty(kv.evict_workspace_bytes(self.caches[0][0]), dtype=torch.uint8,
+                         device=self._device)
+        for (k, v), w, p in zip(self.caches, self.weights, self.positions):
+            kv.evict(k, v, w, lens, budget, sinks=sinks, recent=recent, positions=p, kept=kept,
+                     ends=ends, weights_out=w, positions_out=p, workspace=ws)
+        self.past = self.kept = budget
 
 
 def init_model_weights(cfg: ModelConfig, gen: torch.Generator, device, dtype=torch.bfloat16,
