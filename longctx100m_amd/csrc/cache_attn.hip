@@ -452,24 +452,33 @@ __global__ __launch_bounds__(64 * W, NB * W == 1 ? 1 : 2) void cache_stream_kern
 
 // ------------------------------------- the past, bf16, head_dim 128, 33+ rows --
 
-// Many query rows: the matrix cores and the softmax beside them bound it.
-// Workgroup = NW waves x 32 rows that share 64-key tiles of K and V in LDS
-// (tile128.h), filled by LDS DMA; S^T = K Q^T and O^T += V^T P^T on 32 x 32 x 16
-// products.  Iteration j issues the products of S^T for tile j + 1 and beside
-// them, on the VALU, the softmax of tile j, then O^T += V_j^T P_j^T; K runs one
-// tile ahead of V, two buffers each, one barrier per tile.
-// A row's reference
-// maximum is only raised by more than 2^kSlack, so rescaling is rare; the true
-// one is tracked beside it.
-template <int NW, bool NT>
-__global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void cache_tile128_kernel(AttnArgs a) {
-  constexpr int D = 128, BN = 64;
+// Many query rows: the matrix cores and the softmax beside them bound it.  Eight
+// waves of 32 rows over 64-key tiles of K and V in LDS (tile128.h), filled by LDS
+// DMA; S^T = K Q^T and O^T += V^T P^T on 32 x 32 x 16 products.  Iteration j issues
+// the products of S^T for tile j + 1 and beside them, on the VALU, the softmax of
+// tile j, then O^T += V_j^T P_j^T; K runs one tile ahead of V, two buffers each,
+// one barrier per tile.
+//   RW = 8: 256 rows that share every tile.
+//   RW = 4: 128 rows; waves 0-3 take the even tiles, 4-7 the odd ones (buffers of
+//           their own), and the halves meet in LDS: two waves a SIMD, which the
+//           products need to hide their LDS reads (32 tokens of 32/8 heads over
+//           262,000 keys 177 us, with four waves 202).
+// A row's reference maximum is only raised by more than 2^kSlack, so rescaling is
+// rare; the true one is tracked beside it.
+template <int RW, bool NT>
+__global__ __launch_bounds__(512, 1) void cache_tile128_kernel(AttnArgs a) {
+  constexpr int D = 128, BN = 64, KG = 8 / RW;
   constexpr int kTileB = BN * t128::kRowBytes;
   constexpr float kSlack = 8.f;  // log2 units
-  __shared__ __attribute__((aligned(1024))) uint8_t kbuf[2][kTileB];
-  __shared__ __attribute__((aligned(1024))) uint8_t vbuf[2][kTileB];
+  constexpr int kPitch = D + 4;
+  constexpr int kBufs = 4 * KG * kTileB, kPart = KG > 1 ? 32 * RW * kPitch * 4 : 0;
+  static_assert(kPart <= kBufs, "the halves meet in the tiles' buffers");
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[kBufs];
+  __shared__ float2 stat_s[32 * RW];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kg = KG > 1 ? wave >> 2 : 0;  // which tiles
+  const int rw = KG > 1 ? wave & 3 : wave;
   const int kc = lane & 31;  // this lane's row within the wave
   const int hh = lane >> 5;  // which half of each 8-key group the lane holds
   const int slot = blockIdx.x / a.units;
@@ -481,19 +490,25 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void cache_tile128_kernel
 
   const uint16_t* kbase = static_cast<const uint16_t*>(a.k) + s.b * a.seq + hk * a.head;
   const uint16_t* vbase = static_cast<const uint16_t*>(a.v) + s.b * a.seq + hk * a.head;
-  const int ntiles = (s.k1 - s.k0 + BN - 1) / BN;
-  const int r = 32 * (rb * NW + wave) + kc;
+  const int all = (s.k1 - s.k0 + BN - 1) / BN;
+  const int steps = (all + KG - 1) / KG;                 // tiles of the longer half
+  const int ntiles = KG > 1 ? (all - kg + 1) / 2 : all;  // of this wave's
+  const int r = 32 * (rb * RW + rw) + kc;
 
-  t128::RowLoader<BN, NW> ld;
-  ld.init(a.row, wave, lane);
-  auto load = [&](const uint16_t* base, int j, uint32_t lds) {
-    ld.template load<false, NT>(base, a.row, s.k0 + j * BN, s.k1, lds, wave, lane);
+  t128::RowLoader<BN, RW> ld;
+  ld.init(a.row, rw, lane);
+  const uint32_t lds0 = t128::lds_addr(smem) + kg * 4 * kTileB;
+  const uint8_t* const kbuf = smem + kg * 4 * kTileB;
+  const uint8_t* const vbuf = kbuf + 2 * kTileB;
+  // Tile j of K (what = 0) or V (1), if there is one, into buffer buf.
+  auto issue = [&](int what, int j, int buf) {
+    if (j < ntiles)
+      ld.template load<false, NT>(what ? vbase : kbase, a.row, s.k0 + (KG * j + kg) * BN, s.k1,
+                                  lds0 + (2 * what + buf) * kTileB, rw, lane);
   };
-  if (ntiles > 0) {
-    load(kbase, 0, t128::lds_addr(kbuf));
-    load(vbase, 0, t128::lds_addr(vbuf));
-  }
-  if (ntiles > 1) load(kbase, 1, t128::lds_addr(kbuf) + kTileB);
+  issue(0, 0, 0);
+  issue(1, 0, 0);
+  issue(0, 1, 1);
 
   bf16x8 qreg[D / 16];  // lane: row r, dims 16 t + 8 hh .. + 7
   {
@@ -608,34 +623,62 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void cache_tile128_kernel
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  auto stage = [&](int j, f32x16 (&sc)[2], f32x16 (&sn)[2]) {
+  auto stage = [&](int j, auto parity, f32x16 (&sc)[2], f32x16 (&sn)[2]) {
+    constexpr int P = decltype(parity)::value;  // j % 2
     t128::wait_vmem();
     __syncthreads();
-    if (j + 2 < ntiles) load(kbase, j + 2, t128::lds_addr(kbuf) + (j & 1) * kTileB);
-    if (j + 1 < ntiles) load(vbase, j + 1, t128::lds_addr(vbuf) + ((j + 1) & 1) * kTileB);
-    if (j + 1 < ntiles) iteration(std::false_type{}, kbuf[(j + 1) & 1], vbuf[j & 1], sc, sn, BN);
-    else iteration(std::true_type{}, kbuf[0], vbuf[j & 1], sc, sn, s.k1 - s.k0 - j * BN);
+    issue(0, j + 2, P);
+    issue(1, j + 1, P ^ 1);
+    if (j + 1 < ntiles)
+      iteration(std::false_type{}, kbuf + (P ^ 1) * kTileB, vbuf + P * kTileB, sc, sn, BN);
+    else if (j < ntiles)
+      iteration(std::true_type{}, kbuf, vbuf + P * kTileB, sc, sn, s.k1 - s.k0 - (KG * j + kg) * BN);
   };
   f32x16 sa[2], sb[2];
   t128::wait_vmem();
   __syncthreads();
-  if (ntiles > 0) scores_only(kbuf[0], sa);
-  for (int j = 0; j < ntiles; j += 2) {
-    stage(j, sa, sb);
-    if (j + 1 < ntiles) stage(j + 1, sb, sa);
+  if (ntiles > 0) scores_only(kbuf, sa);
+  for (int j = 0; j < steps; j += 2) {
+    stage(j, std::integral_constant<int, 0>{}, sa, sb);
+    if (j + 1 < steps) stage(j + 1, std::integral_constant<int, 1>{}, sb, sa);
   }
 
   // The partial, relative to the true maximum.
-  const float f = mtrue == -INFINITY ? 0.f : fast_exp2(mrun - mtrue);
-  const float lt = xor32_sum(lsum) * f;
+  float f = mtrue == -INFINITY ? 0.f : fast_exp2(mrun - mtrue);
+  float lt = xor32_sum(lsum) * f;
+  float* part = reinterpret_cast<float*>(smem) + (32 * rw + kc) * kPitch + 4 * hh;
+  float wb = 0.f;
+  if constexpr (KG > 1) {  // the odd tiles' half hands over
+    __syncthreads();  // the tiles are done with
+    if (kg == 1) {
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          *reinterpret_cast<f32x4*>(part + 32 * d + 8 * w) =
+              f32x4{o[d][4 * w], o[d][4 * w + 1], o[d][4 * w + 2], o[d][4 * w + 3]} * f;
+      if (hh == 0) stat_s[32 * rw + kc] = make_float2(mtrue, lt);
+    }
+    __syncthreads();
+    if (kg == 1) return;
+    const float2 st = stat_s[32 * rw + kc];
+    const float top = fmaxf(mtrue, st.x);
+    const float wa = mtrue == -INFINITY ? 0.f : fast_exp2(mtrue - top);
+    wb = st.x == -INFINITY ? 0.f : fast_exp2(st.x - top);
+    f *= wa;
+    lt = lt * wa + st.y * wb;
+    mtrue = top;
+  }
   if (r < a.R) {
     const int64_t pr = partial_row(a, r, hk, slot);
 #pragma unroll
     for (int d = 0; d < 4; ++d)
 #pragma unroll
-      for (int w = 0; w < 4; ++w)
-        *reinterpret_cast<f32x4*>(a.po + pr * D + 32 * d + 8 * w + 4 * hh) =
-            f32x4{o[d][4 * w], o[d][4 * w + 1], o[d][4 * w + 2], o[d][4 * w + 3]} * f;
+      for (int w = 0; w < 4; ++w) {
+        f32x4 x = f32x4{o[d][4 * w], o[d][4 * w + 1], o[d][4 * w + 2], o[d][4 * w + 3]} * f;
+        if constexpr (KG > 1) x += *reinterpret_cast<const f32x4*>(part + 32 * d + 8 * w) * wb;
+        *reinterpret_cast<f32x4*>(a.po + pr * D + 32 * d + 8 * w + 4 * hh) = x;
+      }
     if (hh == 0) a.ps[pr] = make_float2(mtrue, lt);
   }
 }
@@ -666,7 +709,7 @@ template <typename T, int NI, int WPR>
 __global__ __launch_bounds__(64 * WPR) void cache_merge_kernel(AttnArgs a) {
   constexpr int kStep = 4 * WPR;                              // splits and keys of a step
   constexpr int kFirst = (WPR == 1 ? 8 : 4) / (NI > 1 ? NI : 2);  // steps of partials read up front
-  constexpr int kKeys = WPR == 1 && NI < 4 ? 4 : 1;
+  constexpr int kKeys = WPR == 1 && NI < 4 ? 4 : 1;               // steps of keys read together
   __shared__ uint16_t chain_s[WPR][kCacheMaxTokens];
   __shared__ float top_s[WPR], l_s[WPR];
   __shared__ f32x4 acc_s[WPR][16 * NI];
@@ -862,6 +905,11 @@ __global__ __launch_bounds__(64 * WPR) void cache_merge_kernel(AttnArgs a) {
 
 // ------------------------------------------------------------------- host --
 
+// Query rows from which a wave each is enough for the chip: more waves a row cost
+// more instructions than they save latency (64 tokens of 32 heads 17 us against
+// 20 with four; 26 tokens 9.8 against 8.8).
+constexpr int64_t kManyRows = 1024;
+
 enum class Form { kFp32, kStream, kTiled };
 
 struct Plan {
@@ -891,11 +939,12 @@ Plan make_plan(const CacheProblem& p) {
     }
   } else {
     x.form = Form::kTiled;
-    x.waves = R <= 64 ? 2 : R <= 128 ? 4 : 8;
-    x.rows = 32 * x.waves;
+    x.waves = 8;
+    x.rows = R <= 128 ? 128 : 256;
   }
   x.units = (int)((R + x.rows - 1) / x.rows * p.Hkv);
-  const int64_t deal = std::max<int64_t>(1, std::min<int64_t>(want / x.units, tiles));
+  // A sequence's last slot is one more than its share, so a batch deals fewer.
+  const int64_t deal = std::max<int64_t>(1, std::min<int64_t>(want / x.units - (p.B - 1), tiles));
   x.slots = (int)(deal + p.B);
   return x;
 }
@@ -962,8 +1011,7 @@ hipError_t launch_cache_attn(const CacheProblem& p, const void* q, const void* k
     else stream(std::integral_constant<int, 128>{});
   } else {
     const bool once = x.units == p.Hkv;  // the cache is read once: L2 need not keep it
-    if (x.waves == 2) prefix(cache_tile128_kernel<2, true>);
-    else if (x.waves == 4) prefix(cache_tile128_kernel<4, true>);
+    if (x.rows == 128) prefix(cache_tile128_kernel<4, true>);
     else if (once) prefix(cache_tile128_kernel<8, true>);
     else prefix(cache_tile128_kernel<8, false>);
   }
@@ -978,7 +1026,7 @@ hipError_t launch_cache_attn(const CacheProblem& p, const void* q, const void* k
     using T = decltype(t);
     constexpr int kNI = decltype(ni)::value;
     if (wide) merge(cache_merge_kernel<T, kNI, 16>, 16);
-    else if (rows < 1024) merge(cache_merge_kernel<T, kNI, 4>, 4);
+    else if (rows < kManyRows) merge(cache_merge_kernel<T, kNI, 4>, 4);
     else merge(cache_merge_kernel<T, kNI, 1>, 1);
   };
   auto merge_type = [&](auto t) {
