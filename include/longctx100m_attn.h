@@ -222,7 +222,8 @@ int lc_attn_bwd_shard_ws(const lc_attn_shape_t* shape, const lc_attn_mask_t* mas
  *   b * seq_stride + j * row_stride + h * head_stride
  * of both K and V (head_dim elements, contiguous), so [B, C, Hkv, D] and
  * [B, Hkv, C, D] caches and slices of larger ones are all described.  Strides
- * are multiples of 16 bytes, K and V 16-byte aligned, row_stride <= 2^24.
+ * are multiples of 16 bytes, K and V 16-byte aligned, row_stride <= 2^24, the
+ * others <= 2^40.
  * past[b] (int32, device) rows of sequence b hold earlier tokens, in any order;
  * the new tokens' K and V are in rows past[b] .. past[b] + tokens - 1, where
  * the caller has put them.  A new token whose row lies at or past capacity is
@@ -310,8 +311,8 @@ int lc_cache_evict(const lc_cache_t* cache, int32_t budget, int32_t sinks, int32
 /* Makes an accepted path of the tree the continuation of every layer's cache:
  * path [B, tokens] (int32, device) holds node numbers in ascending order, and
  * K and V row past[b] + path[b][j] moves to past[b] + j, for each of `layers`
- * caches of the same shape (host arrays of device pointers).  The path ends at
- * the first entry that is not above the one before it (>= 0 the first) or whose
+ * caches of the same shape (host arrays of device pointers), no two of which, K
+ * or V, may share rows.  The path ends at the first entry that is not above the one before it (>= 0 the first) or whose
  * row lies past the capacity, e.g. at a -1.  lens_out[b] = past[b] + the path's
  * length; a sequence with past < 0 keeps it.  lens_out must not overlap past or
  * path.  Here tokens is the path's length, and heads_q is not read. */

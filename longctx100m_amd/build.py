@@ -66,6 +66,13 @@ SCRATCH_LIMITS = {
     "decode_kernel": 0,
     "rmsnorm_kernel": 0,
     "generic_kernel": 24,
+    "cache_prefix32_kernel": 0,
+    "cache_stream_kernel": 0,
+    "cache_tile128_kernel": 0,
+    "cache_merge_kernel": 0,
+    "cache_weights": 0,
+    "cache_commit_kernel": 0,
+    "evict_": 0,
 }
 
 # "Function Name: <kernel>" starts a kernel's block; then "<field> [unit]: value".

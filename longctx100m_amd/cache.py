@@ -226,9 +226,13 @@ class Layers:
         self.ks, self.vs = list(ks), list(vs)
         if not self.ks or len(self.ks) != len(self.vs):
             raise ValueError("Layers needs one k and one v per layer")
-        for k, v in zip(self.ks, self.vs):
-            _kv(k, v)
-            _kv(self.ks[0], k)
+        first = self.ks[0]
+        _kv(first, None)
+        like = (first.shape, first.stride(), first.dtype, first.get_device())
+        if any((t.shape, t.stride(), t.dtype, t.get_device()) != like for t in self.ks + self.vs):
+            raise ValueError("the caches must have the same shape, strides, type and device")
+        if len({t.data_ptr() for t in self.ks + self.vs}) < 2 * len(self.ks):
+            raise ValueError("a cache is listed twice: its rows would be moved twice")
         self._k, self._ka = _lib.ptr_array([t.data_ptr() for t in self.ks])
         self._v, self._va = _lib.ptr_array([t.data_ptr() for t in self.vs])
 

@@ -52,4 +52,20 @@ struct CommitArgs {
 };
 hipError_t launch_cache_commit(const CommitArgs& a, int layers, hipStream_t s);
 
+// Inclusive prefix sum over a wave's lanes with DPP: within the rows of 16 lanes
+// by shifts of 1, 2, 4 and 8, then the last lane of row 0 (2) into row 1 (3),
+// and lane 31 into the upper half.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int dpp_add(int x) {
+  return x + __builtin_amdgcn_update_dpp(0, x, kCtrl, kRows, 0xf, true);
+}
+__device__ __forceinline__ int wave_scan(int x) {
+  x = dpp_add<0x111, 0xf>(x);
+  x = dpp_add<0x112, 0xf>(x);
+  x = dpp_add<0x114, 0xf>(x);
+  x = dpp_add<0x118, 0xf>(x);
+  x = dpp_add<0x142, 0xa>(x);
+  return dpp_add<0x143, 0xc>(x);
+}
+
 }  // namespace lc

@@ -50,7 +50,8 @@ int check_cache(const lc_cache_t* c, bool written, bool queries) {
     return set_error(LC_ERR_UNSUPPORTED, "the cache operators need head_dim %% 16 == 0 and <= 256");
   // A launch holds fewer than 2^32 threads in a dimension, and row indices of
   // one sequence's queries are 32-bit.
-  if ((int64_t)c->batch * c->heads_kv * ((c->capacity + 63LL) / 64) > 1 << 24 ||
+  const int64_t heads = (int64_t)c->batch * c->heads_kv;
+  if (heads > 1 << 21 || heads * ((c->capacity + 63LL) / 64) > 1 << 23 ||
       (queries && (int64_t)c->batch * c->heads_q > 1 << 24) ||
       (queries && (int64_t)c->tokens * c->heads_q > 1 << 30))
     return set_error(LC_ERR_UNSUPPORTED, "the cache or its queries exceed the kernels' grids");
@@ -60,6 +61,8 @@ int check_cache(const lc_cache_t* c, bool written, bool queries) {
     return set_error(LC_ERR_INVALID, "cache strides must be multiples of 16 bytes");
   if (c->row_stride > (int64_t)1 << 24)
     return set_error(LC_ERR_UNSUPPORTED, "cache rows lie more than 2^24 elements apart");
+  if (c->seq_stride > (int64_t)1 << 40 || c->head_stride > (int64_t)1 << 40)
+    return set_error(LC_ERR_UNSUPPORTED, "sequences or heads lie more than 2^40 elements apart");
   if (written) {
     struct Dim {
       int64_t stride, n;
@@ -70,7 +73,7 @@ int check_cache(const lc_cache_t* c, bool written, bool queries) {
       if (x.n == 1) continue;
       if (x.stride < extent)
         return set_error(LC_ERR_INVALID, "rows of a cache that is written must not overlap");
-      extent = x.stride * x.n;
+      extent += x.stride * (x.n - 1);
     }
   }
   return LC_OK;
@@ -99,7 +102,7 @@ int check_attn(const lc_cache_t* c) {
   if (int rc = check_cache(c, false, true)) return rc;
   if (c->tokens > LC_CACHE_MAX_TOKENS)
     return set_error(LC_ERR_UNSUPPORTED, "at most %d new tokens", LC_CACHE_MAX_TOKENS);
-  if ((int64_t)c->batch * c->heads_q * c->tokens > 1 << 24)
+  if ((int64_t)c->batch * c->heads_q * c->tokens > 1 << 22)
     return set_error(LC_ERR_UNSUPPORTED, "the cache or its queries exceed the kernels' grids");
   return LC_OK;
 }
@@ -109,7 +112,7 @@ int check_attn(const lc_cache_t* c) {
 extern "C" {
 
 size_t lc_cache_attn_workspace_bytes(const lc_cache_t* cache) {
-  if (check_attn(cache)) return 0;
+  if (check_attn(cache) || cache->tokens == 0) return 0;
   return lc::cache_attn_bytes(make_problem(cache, nullptr, nullptr));
 }
 
@@ -235,6 +238,8 @@ int lc_cache_commit(const lc_cache_t* cache, int32_t layers, void* const* ks, vo
     if (!ks[i] || !vs[i]) return set_error(LC_ERR_INVALID, "null k or v of layer %d", i);
     if (!aligned(ks[i], 16) || !aligned(vs[i], 16))
       return set_error(LC_ERR_INVALID, "k and v must be 16-byte aligned");
+    if (ks[i] == vs[i])  // its rows would be moved twice
+      return set_error(LC_ERR_INVALID, "k and v of layer %d are the same cache", i);
   }
   if (!aligned(past, 4) || !aligned(path, 4) || !aligned(lens_out, 4))
     return set_error(LC_ERR_INVALID, "past, path and lens_out must be 4-byte aligned");

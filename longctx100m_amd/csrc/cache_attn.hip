@@ -15,8 +15,9 @@
 //
 // The lengths are known on the device only.  The host fixes the number of
 // split slots (and with it the workspace); each workgroup reads the lengths
-// and finds its sequence and key range: slots are dealt out in proportion to
-// the sequences' tiles, so a batch of unequal lengths loads the chip evenly.
+// and finds its sequence and key range: a slot holds `per` tiles, the fewest
+// with which the slots suffice for all sequences, so a batch of unequal
+// lengths loads the chip evenly.
 #include "common.h"
 #include "cache.h"
 #include "kernels.h"
@@ -40,6 +41,7 @@ struct AttnArgs {
   // (m, l), m in log2 units.
   float* po;
   float2* ps;
+  int2* deal;  // [B]: a sequence's first slot and its slots
   const int32_t *past, *parents;
   int B, N, C, Hq, Hkv, D, group, R;  // R: query rows of a KV head
   int slots, units;                   // units: workgroups of a slot
@@ -55,74 +57,76 @@ __device__ __forceinline__ int past_tiles(int past, int C) {
   return max(1, (past_rows(past, C) + kTile - 1) / kTile);
 }
 
-__device__ __forceinline__ int wave_sum_i(int x) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) x += __shfl_xor(x, off, 64);
-  return x;
+__device__ __forceinline__ int wave_sum_i(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
+
+// ceil(t / per) for 0 <= t < 2^24, inv = 1 / per: the product is off by at most
+// one.
+__device__ __forceinline__ int slots_for(int t, int per, float inv) {
+  const int q = (int)((float)t * inv);
+  const int r = t - q * per;
+  return q + (r > 0) + (r > per);
 }
 
-// The slots of the sequences: sequence b has ceil(tiles_b / per) of them, one
-// after another, per = ceil(all tiles / (slots - B)); their number is at most
-// all tiles / per + B <= slots.
-struct Deal {
-  int per;   // tiles of a slot
-  int b;     // the sequence looked for
-  int first; // its first slot
-  int count; // its slots
-};
-// With slot >= 0 the sequence that has it (count = 0: none), otherwise b's.
-__device__ __forceinline__ Deal deal_slots(const int32_t* past, int B, int C, int slots, int slot,
-                                           int b) {
+// Sequences up to which the slots are dealt as tightly as possible.
+constexpr int kTightBatch = 64;
+
+// Tiles of a slot.  One sequence: its share.  Up to kTightBatch: the 64 lanes
+// try 63 sizes from an even share of all tiles to five times it, and the longest
+// sequence's tiles, with which one slot a sequence is enough; the smallest
+// size whose slots suffice is taken.  More sequences have B slots beyond the
+// even shares, and ceil(tiles / per) adds less than one each.
+__device__ __forceinline__ int slot_tiles(const int32_t* past, int B, int C, int slots) {
   const int lane = threadIdx.x & 63;
-  Deal d{};
-  if (B == 1) {
-    const int t = past_tiles(past[0], C);
-    d.per = (t + slots - 2) / (slots - 1);
-    d.count = (t + d.per - 1) / d.per;
-    if (slot >= d.count) d.count = 0;
-    return d;
+  if (B == 1) return (past_tiles(past[0], C) + slots - 1) / slots;
+  if (B > kTightBatch) {
+    int total = 0;
+    for (int b0 = 0; b0 < B; b0 += 64)
+      total += wave_sum_i(b0 + lane < B ? past_tiles(past[b0 + lane], C) : 0);
+    return (total + slots - B - 1) / (slots - B);
   }
-  int total = 0;
-  for (int b0 = 0; b0 < B; b0 += 64)
-    total += wave_sum_i(b0 + lane < B ? past_tiles(past[b0 + lane], C) : 0);
-  d.per = (total + slots - B - 1) / (slots - B);
-  int base = 0;
-  for (int b0 = 0; b0 < B; b0 += 64) {
-    const int n = b0 + lane < B ? (past_tiles(past[b0 + lane], C) + d.per - 1) / d.per : 0;
-    int end = n;  // inclusive scan
+  const int mine = lane < B ? past_tiles(past[lane], C) : 0;
+  int most = mine;
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int x = __shfl_up(end, off, 64);
-      if (lane >= off) end += x;
-    }
-    end += base;
-    const bool hit = slot >= 0 ? slot < end && slot >= end - n : b0 + lane == b;
-    const uint64_t who = __ballot(hit);
-    if (who) {
-      const int at = __ffsll((unsigned long long)who) - 1;
-      d.b = b0 + at;
-      d.count = __shfl(n, at, 64);
-      d.first = __shfl(end, at, 64) - d.count;
-      return d;
-    }
-    base = __shfl(end, 63, 64);
-  }
-  return d;  // a slot without a sequence
+  for (int off = 1; off < 64; off <<= 1) most = max(most, __shfl_xor(most, off, 64));
+  const int even = (wave_sum_i(mine) + slots - 1) / slots;
+  const int size = lane == 63 ? most : even + (int)((int64_t)even * lane / 16);
+  const float inv = 1.f / (float)size;
+  int n = 0;
+  for (int b = 0; b < B; ++b) n += slots_for(__builtin_amdgcn_readlane(mine, b), size, inv);
+  const uint64_t fits = __ballot(n <= slots);  // the last lane's does
+  return __builtin_amdgcn_readlane(size, __ffsll((unsigned long long)fits) - 1);
 }
 
 // The key range of a workgroup.
 struct Share {
   int b, k0, k1;  // keys k0 .. k1 - 1 of sequence b (none: k0 == k1)
-  int rows;       // its whole past
 };
+// Finds the share of a slot; false: it has none.  The first workgroup leaves
+// every sequence's slots for the merge.
 __device__ __forceinline__ bool share_of(const AttnArgs& a, int slot, Share& s) {
-  const Deal d = deal_slots(a.past, a.B, a.C, a.slots, slot, 0);
-  if (d.count == 0) return false;
-  s.b = __builtin_amdgcn_readfirstlane(d.b);
-  s.rows = past_rows(a.past[s.b], a.C);
-  s.k0 = __builtin_amdgcn_readfirstlane((slot - d.first) * d.per * kTile);
-  s.k1 = min(s.k0 + d.per * kTile, s.rows);
-  if (s.k0 > s.k1) s.k0 = s.k1;
+  const int lane = threadIdx.x & 63;
+  const int per = slot_tiles(a.past, a.B, a.C, a.slots);
+  const float inv = 1.f / (float)per;
+  int first = 0, at = -1;  // of sequence at
+  int base = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int b = b0 + lane;
+    const int n = b < a.B ? slots_for(past_tiles(a.past[b], a.C), per, inv) : 0;
+    const int end = base + wave_scan(n);
+    if (blockIdx.x == 0 && threadIdx.x < 64 && b < a.B) a.deal[b] = make_int2(end - n, n);
+    const uint64_t who = __ballot(slot < end && slot >= end - n);
+    if (who) {
+      const int x = __ffsll((unsigned long long)who) - 1;
+      at = b0 + x;
+      first = __builtin_amdgcn_readlane(end - n, x);
+    }
+    base = __builtin_amdgcn_readlane(end, 63);
+  }
+  if (at < 0) return false;
+  s.b = __builtin_amdgcn_readfirstlane(at);
+  const int rows = past_rows(a.past[s.b], a.C);
+  s.k0 = __builtin_amdgcn_readfirstlane(min((slot - first) * per * kTile, rows));
+  s.k1 = __builtin_amdgcn_readfirstlane(min(rows - s.k0, per * kTile)) + s.k0;
   return true;
 }
 
@@ -238,23 +242,34 @@ __global__ __launch_bounds__(256) void cache_prefix32_kernel(AttnArgs a) {
   }
 }
 
-// -------------------------------------------- the past, bf16, up to 32 rows --
+// ------------------------------------------- the past, bf16, a few rows --
 
 // Few query rows: bound by the stream of the cache.  Every wave holds all of
 // the workgroup's 16 * NB rows (Q^T in registers, the B operand) and takes its
 // own 8 KB tiles of K, straight into registers as the A operand of S^T = K Q^T,
 // and of V, through LDS for the transposed reads of O^T += V^T P^T; both one
-// tile ahead and non-temporal.  The W waves of a workgroup take the tiles of
-// their split in turn and meet in LDS.
-template <int D, int NB, int W>
-__global__ __launch_bounds__(64 * W, NB * W == 1 ? 1 : 2) void cache_stream_kernel(AttnArgs a) {
+// tile ahead.  With 64 rows there are registers for one K tile: the next is
+// read once the scores are there.  The four waves of a workgroup take the tiles
+// of their split in turn and meet in LDS.  (Workgroups of one wave, eight on a
+// CU, took 204 us against 190 at 262,000 keys, 8 KV heads of 128 and 8 tokens,
+// and left the merge 2048 partials.)
+// Rows of 128 dims are read non-temporally: one workgroup reads them once, and
+// the partials stay in L2 for the merge: 53 us in all against 56 at 60,000 keys
+// and 4 tokens, 194 against 200 at 262,000 (5.7 TB/s).  Rows of 64 are one cache
+// line of which each load takes half, and may have several row blocks that read
+// them: 30.1 us in all against 35.0 at 60,000 keys and 8 tokens, 112 against 118
+// at 262,000 and 4 (5.0 TB/s), 36 against 49 with 256 query rows at 16,000.
+template <int D, int NB>
+__global__ __launch_bounds__(256, 2) void cache_stream_kernel(AttnArgs a) {
   using C = DecodeTile<D>;
   constexpr int TK = C::TK, MB = C::MB, KS = C::KS, DB = C::DB;
+  constexpr int W = 4;            // waves
+  constexpr bool NT = D == 128;  // non-temporal loads
   constexpr int kRows = 16 * NB;
   constexpr int kStages = 2;
   constexpr int kPitch = D + 4;  // floats per row of a wave's partial
   constexpr int kVBytes = W * kStages * kTileBytes;
-  constexpr int kPartBytes = W > 1 ? W * kRows * kPitch * 4 : 0;
+  constexpr int kPartBytes = W * kRows * kPitch * 4;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[kVBytes > kPartBytes ? kVBytes : kPartBytes];
   __shared__ float msm[W][kRows], lsm[W][kRows];
 
@@ -278,16 +293,17 @@ __global__ __launch_bounds__(64 * W, NB * W == 1 ? 1 : 2) void cache_stream_kern
   const uint32_t vlds = t128::lds_addr(smem) + wave * kStages * kTileBytes;
   const uint8_t* vmem = smem + wave * kStages * kTileBytes;
   auto issue = [&](int j) {  // V tile j into stage j % kStages
-    ld.load(vbase, a.row, kb0 + j * (W * TK), s.k1, vlds + (j % kStages) * kTileBytes, lane);
+    ld.template load<NT>(vbase, a.row, kb0 + j * (W * TK), s.k1, vlds + (j % kStages) * kTileBytes, lane);
   };
   auto kload = [&](int j, bf16x8 (&kr)[MB][KS]) {  // lane (c, g): key 16 mb + c, dims 32 kk + 8 g
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
       const int row = min(kb0 + j * (W * TK) + 16 * mb + c, s.k1 - 1);
 #pragma unroll
-      for (int kk = 0; kk < KS; ++kk)
-        kr[mb][kk] = __builtin_nontemporal_load(
-            reinterpret_cast<const bf16x8*>(kbase + row * a.row + 32 * kk + 8 * g));
+      for (int kk = 0; kk < KS; ++kk) {
+        const bf16x8* at = reinterpret_cast<const bf16x8*>(kbase + row * a.row + 32 * kk + 8 * g);
+        kr[mb][kk] = NT ? __builtin_nontemporal_load(at) : *at;
+      }
     }
   };
 
@@ -330,7 +346,7 @@ __global__ __launch_bounds__(64 * W, NB * W == 1 ? 1 : 2) void cache_stream_kern
     t128::wait_vmem();
     if (j + 1 < ntiles) {
       issue(j + 1);
-      kload(j + 1, kn);
+      if constexpr (NB < 4) kload(j + 1, kn);
     }
     const uint8_t* vt = vmem + (j % kStages) * kTileBytes;
     const int left = s.k1 - (kb0 + j * (W * TK));  // keys of the split from this tile on
@@ -345,6 +361,10 @@ __global__ __launch_bounds__(64 * W, NB * W == 1 ? 1 : 2) void cache_stream_kern
       for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) sc[nb][mb] = mfma16x16x32(kc[mb][kk], qreg[nb][kk], sc[nb][mb]);
+    if constexpr (NB == 4) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (j + 1 < ntiles) kload(j + 1, kc);
+    }
     if (left < TK) {
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
@@ -352,7 +372,7 @@ __global__ __launch_bounds__(64 * W, NB * W == 1 ? 1 : 2) void cache_stream_kern
         for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (16 * mb + 4 * g + i >= left) sc[nb][mb][i] = -INFINITY;
+            if (16 * mb + i >= left - 4 * g) sc[nb][mb][i] = -INFINITY;
     }
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
@@ -393,9 +413,13 @@ __global__ __launch_bounds__(64 * W, NB * W == 1 ? 1 : 2) void cache_stream_kern
       }
     }
   };
-  for (int j = 0; j < ntiles; j += 2) {
-    tile(j, kra, krb);
-    if (j + 1 < ntiles) tile(j + 1, krb, kra);
+  if constexpr (NB == 4) {
+    for (int j = 0; j < ntiles; ++j) tile(j, kra, kra);
+  } else {
+    for (int j = 0; j < ntiles; j += 2) {
+      tile(j, kra, krb);
+      if (j + 1 < ntiles) tile(j + 1, krb, kra);
+    }
   }
 
   auto emit = [&](int r, int d, const f32x4& acc, float L, float M) {
@@ -403,17 +427,6 @@ __global__ __launch_bounds__(64 * W, NB * W == 1 ? 1 : 2) void cache_stream_kern
     *reinterpret_cast<f32x4*>(a.po + pr * D + d) = acc;
     if (d == 0) a.ps[pr] = make_float2(M, L);
   };
-  if constexpr (W == 1) {
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      const float L = group4_sum(lsum[nb]);
-      const int r = rb * kRows + 16 * nb + c;
-      if (r < a.R)
-#pragma unroll
-        for (int db = 0; db < DB; ++db) emit(r, 16 * db + 4 * g, o[nb][db], L, mrow[nb]);
-    }
-    return;
-  }
   // The waves' partials, brought to each row's maximum, meet in LDS.
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
@@ -462,7 +475,9 @@ __global__ __launch_bounds__(64 * W, NB * W == 1 ? 1 : 2) void cache_stream_kern
 //   RW = 4: 128 rows; waves 0-3 take the even tiles, 4-7 the odd ones (buffers of
 //           their own), and the halves meet in LDS: two waves a SIMD, which the
 //           products need to hide their LDS reads (32 tokens of 32/8 heads over
-//           262,000 keys 177 us, with four waves 202).
+//           262,000 keys 190 us, 5.6 TB/s; with four waves 202 to 210).
+// 256 rows take 300 us there (64 tokens, 915 TFLOP/s): the
+// softmax of a tile does not hide behind the products entirely.
 // A row's reference maximum is only raised by more than 2^kSlack, so rescaling is
 // rare; the true one is tracked beside it.
 template <int RW, bool NT>
@@ -490,7 +505,9 @@ __global__ __launch_bounds__(512, 1) void cache_tile128_kernel(AttnArgs a) {
 
   const uint16_t* kbase = static_cast<const uint16_t*>(a.k) + s.b * a.seq + hk * a.head;
   const uint16_t* vbase = static_cast<const uint16_t*>(a.v) + s.b * a.seq + hk * a.head;
-  const int all = (s.k1 - s.k0 + BN - 1) / BN;
+  // In a vector register: as a scalar it makes the compiler merge the loop's
+  // branches, at the price of 336 to 420 bytes of scratch a lane.
+  const int all = opaque((s.k1 - s.k0 + BN - 1) / BN);
   const int steps = (all + KG - 1) / KG;                 // tiles of the longer half
   const int ntiles = KG > 1 ? (all - kg + 1) / 2 : all;  // of this wave's
   const int r = 32 * (rb * RW + rw) + kc;
@@ -703,8 +720,8 @@ __device__ __forceinline__ void store_vec4(T* p, const f32x4& r) {
 // wave.  A row costs few bytes and would cost many memory latencies, so what
 // does not depend on the chain (the first partials) is read before the chain
 // is followed, and the keys and values of kKeys steps together (64 tokens of 32
-// heads over 32 splits, chains of some ten keys: 17.5 us with one step at a
-// time).
+// heads over 32 splits, chains of some ten keys: 16.7 us, 17.5 with one step at
+// a time).
 template <typename T, int NI, int WPR>
 __global__ __launch_bounds__(64 * WPR) void cache_merge_kernel(AttnArgs a) {
   constexpr int kStep = 4 * WPR;                              // splits and keys of a step
@@ -737,14 +754,15 @@ __global__ __launch_bounds__(64 * WPR) void cache_merge_kernel(AttnArgs a) {
 #pragma unroll
   for (int x = 0; x < NI; ++x) qv[x] = load_w<T, 4>(qp, 4 * (j + 16 * x), a.D, true);
 
-  const Deal d = deal_slots(a.past, a.B, a.C, a.slots, -1, b);
-  const int64_t pr0 = ((int64_t)i * a.Hq + h) * a.slots + d.first;
+  const int2 deal = a.deal[b];
+  const int splits = deal.y;
+  const int64_t pr0 = ((int64_t)i * a.Hq + h) * a.slots + deal.x;
   f32x4 po[kFirst][NI];
   float2 ps[kFirst];
 #pragma unroll
   for (int f = 0; f < kFirst; ++f) {
     const int s = kStep * f + 4 * wave + u;
-    const int64_t pr = pr0 + min(s, d.count - 1);
+    const int64_t pr = pr0 + min(s, splits - 1);
     ps[f] = a.ps[pr];
 #pragma unroll
     for (int x = 0; x < NI; ++x) po[f][x] = load_w<float, 4>(a.po + pr * a.D, 4 * (j + 16 * x), a.D, true);
@@ -836,7 +854,7 @@ __global__ __launch_bounds__(64 * WPR) void cache_merge_kernel(AttnArgs a) {
   float top = m;
 #pragma unroll
   for (int f = 0; f < kFirst; ++f) top = fmaxf(top, ps[f].x);  // (a re-read split changes nothing)
-  for (int s = kStep * kFirst + 64 * wave + lane; s < d.count; s += 64 * WPR)
+  for (int s = kStep * kFirst + 64 * wave + lane; s < splits; s += 64 * WPR)
     top = fmaxf(top, a.ps[pr0 + s].x);
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
@@ -855,14 +873,14 @@ __global__ __launch_bounds__(64 * WPR) void cache_merge_kernel(AttnArgs a) {
   }
 #pragma unroll
   for (int f = 0; f < kFirst; ++f) {
-    if (kStep * f + 4 * wave + u >= d.count) continue;
+    if (kStep * f + 4 * wave + u >= splits) continue;
     const float w = exp2f(ps[f].x - muse);  // a split without keys: 0
     l += w * ps[f].y;
 #pragma unroll
     for (int x = 0; x < NI; ++x) acc[x] += po[f][x] * w;
   }
 #pragma unroll(NI == 4 ? 1 : 4)
-  for (int s = kStep * kFirst + 4 * wave + u; s < d.count; s += kStep) {
+  for (int s = kStep * kFirst + 4 * wave + u; s < splits; s += kStep) {
     const int64_t pr = pr0 + s;
     const float2 st = a.ps[pr];
     const float w = exp2f(st.x - muse);
@@ -906,9 +924,20 @@ __global__ __launch_bounds__(64 * WPR) void cache_merge_kernel(AttnArgs a) {
 // ------------------------------------------------------------------- host --
 
 // Query rows from which a wave each is enough for the chip: more waves a row cost
-// more instructions than they save latency (64 tokens of 32 heads 17 us against
-// 20 with four; 26 tokens 9.8 against 8.8).
+// more instructions than they save latency (32 heads: 64 tokens 16.7 us against
+// 18.4 with four, 26 tokens 9.8 against 8.8).
 constexpr int64_t kManyRows = 1024;
+
+// Workgroups for a whole chip, one a CU: each split costs a partial that is
+// written and merged.
+constexpr int64_t kWanted = 256;
+
+// K rows of head_dim 64, bf16, of which a cache of as many (V too) stays in the
+// last-level cache: up to there 33 to 64 query rows take it twice, by two
+// workgroups of 32 rows, which is faster than 64 rows at once with their one K
+// tile in flight: 7.2 us against 9.4 at 8 x 4,000 rows, 26.2 against 28.0 at 8 x
+// 60,000, but 148 against 104 at 8 x 262,000.
+constexpr int64_t kCachedRows = 1 << 19;
 
 enum class Form { kFp32, kStream, kTiled };
 
@@ -925,27 +954,23 @@ Plan make_plan(const CacheProblem& p) {
   const bool bf16 = p.dtype == 1 && !p.precise && (p.D == 64 || p.D == 128);
   Plan x;
   x.waves = 4;
-  int64_t want = 256;  // workgroups
   if (!bf16) {
     x.form = Form::kFp32;
     x.rows = R <= 16 ? 16 : R <= 32 ? 32 : 64;
   } else if (R <= 32 || p.D == 64) {
     x.form = Form::kStream;
-    x.rows = R <= 16 ? 16 : 32;
-    const int64_t units = (R + x.rows - 1) / x.rows * p.Hkv;
-    if (units * p.B <= 16 && tiles * units * p.D >= 64 * 6 * 2048) {
-      x.waves = 1;
-      want = 2048;
-    }
+    x.rows = R <= 16 ? 16 : R <= 32 || (R <= 64 && (int64_t)p.B * p.C * p.Hkv <= kCachedRows) ? 32 : 64;
   } else {
     x.form = Form::kTiled;
     x.waves = 8;
     x.rows = R <= 128 ? 128 : 256;
   }
   x.units = (int)((R + x.rows - 1) / x.rows * p.Hkv);
-  // A sequence's last slot is one more than its share, so a batch deals fewer.
-  const int64_t deal = std::max<int64_t>(1, std::min<int64_t>(want / x.units - (p.B - 1), tiles));
-  x.slots = (int)(deal + p.B);
+  const int64_t slots = std::max<int64_t>(1, std::min<int64_t>(kWanted / x.units, tiles));
+  // A batch of nearly as many sequences as slots, or more, has some left for its
+  // long ones: 39 sequences of 300 keys and one of 16,000 take 59 us, with a slot
+  // each 292.
+  x.slots = (int)(p.B > kTightBatch ? slots + p.B : std::max<int64_t>(slots, p.B > 1 ? p.B + slots / 2 : 1));
   return x;
 }
 
@@ -953,7 +978,7 @@ Plan make_plan(const CacheProblem& p) {
 
 size_t cache_attn_bytes(const CacheProblem& p) {
   const Plan x = make_plan(p);
-  return (size_t)x.slots * p.N * p.Hq * (p.D + 2) * sizeof(float);
+  return (size_t)x.slots * p.N * p.Hq * (p.D + 2) * sizeof(float) + (size_t)p.B * sizeof(int2);
 }
 
 hipError_t launch_cache_attn(const CacheProblem& p, const void* q, const void* k, const void* v,
@@ -969,6 +994,7 @@ hipError_t launch_cache_attn(const CacheProblem& p, const void* q, const void* k
   a.l = l;
   a.po = static_cast<float*>(ws);
   a.ps = reinterpret_cast<float2*>(a.po + prows * p.D);
+  a.deal = reinterpret_cast<int2*>(a.ps + prows);
   a.past = p.past;
   a.parents = p.parents;
   a.B = p.B;
@@ -1000,8 +1026,9 @@ hipError_t launch_cache_attn(const CacheProblem& p, const void* q, const void* k
   };
   auto stream = [&](auto d) {
     constexpr int kD = decltype(d)::value;
-    if (x.waves == 1) x.rows == 16 ? prefix(cache_stream_kernel<kD, 1, 1>) : prefix(cache_stream_kernel<kD, 2, 1>);
-    else x.rows == 16 ? prefix(cache_stream_kernel<kD, 1, 4>) : prefix(cache_stream_kernel<kD, 2, 4>);
+    if (x.rows == 16) prefix(cache_stream_kernel<kD, 1>);
+    else if (x.rows == 32) prefix(cache_stream_kernel<kD, 2>);
+    else if constexpr (kD == 64) prefix(cache_stream_kernel<kD, 4>);
   };
   if (x.form == Form::kFp32) {
     if (p.dtype == 1) fp32(uint16_t{});
@@ -1018,15 +1045,13 @@ hipError_t launch_cache_attn(const CacheProblem& p, const void* q, const void* k
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int64_t rows = (int64_t)p.B * p.N * p.Hq;
-  const bool wide = x.slots - p.B >= 128 && rows <= 256;
   auto merge = [&](auto kernel, int waves) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(64 * waves), 0, st, a);
   };
   auto merge_dim = [&](auto t, auto ni) {
     using T = decltype(t);
     constexpr int kNI = decltype(ni)::value;
-    if (wide) merge(cache_merge_kernel<T, kNI, 16>, 16);
-    else if (rows < kManyRows) merge(cache_merge_kernel<T, kNI, 4>, 4);
+    if (rows < kManyRows) merge(cache_merge_kernel<T, kNI, 4>, 4);
     else merge(cache_merge_kernel<T, kNI, 1>, 1);
   };
   auto merge_type = [&](auto t) {

@@ -31,9 +31,10 @@ template <>
 struct VTile<128> {
   t128::RowLoader<DecodeTile<128>::TK, 1> ld;
   __device__ __forceinline__ void init(int64_t stride, int lane) { ld.init(stride, 0, lane); }
+  template <bool kNt = true>
   __device__ __forceinline__ void load(const uint16_t* base, int64_t stride, int row0, int nrows,
                                        uint32_t lds, int lane) const {
-    ld.load<false, true>(base, stride, row0, nrows, lds, 0, lane);
+    ld.template load<false, kNt>(base, stride, row0, nrows, lds, 0, lane);
   }
   static __device__ __forceinline__ int tr_off(int col0, int lane) { return t128::tr_off(0, col0, lane); }
 };
@@ -49,18 +50,24 @@ struct VTile<64> {
     }
   }
   // Rows at or past nrows re-read the last row (callers mask them).
+  template <bool kNt = true>
   __device__ __forceinline__ void load(const uint16_t* base, int64_t stride, int row0, int nrows,
                                        uint32_t lds, int lane) const {
     if (row0 + 8 * kInst <= nrows) {
       const uint8_t* tb = reinterpret_cast<const uint8_t*>(base + (int64_t)row0 * stride);
 #pragma unroll
-      for (int i = 0; i < kInst; ++i) t128::dma_b128_nt(tb, off[i], lds + 1024 * i);
+      for (int i = 0; i < kInst; ++i) {
+        if constexpr (kNt) t128::dma_b128_nt(tb, off[i], lds + 1024 * i);
+        else t128::dma_b128(tb, off[i], lds + 1024 * i);
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < kInst; ++i) {
         const int r = 8 * i + (lane >> 3);
         const int row = min(row0 + r, nrows - 1);
-        t128::dma_b128_nt(base + (int64_t)row * stride + 8 * ((lane & 7) ^ swz64(r)), lds + 1024 * i);
+        const uint16_t* g = base + (int64_t)row * stride + 8 * ((lane & 7) ^ swz64(r));
+        if constexpr (kNt) t128::dma_b128_nt(g, lds + 1024 * i);
+        else t128::dma_b128(g, lds + 1024 * i);
       }
     }
   }

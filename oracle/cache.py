@@ -93,7 +93,8 @@ def evict(k, v, weights, lens, budget, sinks=0, recent=0, positions=None, kept=N
                 return (2, 0.0, j) if np.isnan(w) else (1, -float(w), j)
 
             keep = sorted(sorted(range(n), key=rank)[:budget])
-            holes = [j for j in range(min(budget, n)) if j not in set(keep)]
+            held = set(keep)
+            holes = [j for j in range(min(budget, n)) if j not in held]
             movers = [j for j in keep if j >= budget]
             assert len(holes) == len(movers)
             for j in keep:

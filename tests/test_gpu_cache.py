@@ -237,6 +237,105 @@ def test_more_sequences_than_a_wave_has_lanes(gpu):
     _check_attention(_run(gpu, q, k, v, past, None, "bf16"), want, q, k, v, "bf16", True)
 
 
+# As ATTENTION: batches of unequal lengths, and the row blocks of head_dim 64.
+UNEQUAL = [
+    (4, 2, 64, "bf16", [30] * 20 + [3000] + [0, -1, 7] * 6, 6, 1, 0, "rows"),
+    (4, 2, 128, "bf16", [100] * 11 + [2500, 64], 9, 0, 2, "heads"),
+    (8, 1, 128, "bf16", [65] * 69 + [2000, -1, 3], 4, 0, 0, "rows"),
+    (2, 2, 32, "fp32", [20] * 63 + [900], 2, 0, 0, "rows"),
+    (4, 1, 64, "bf16", [700, 90], 12, 0, 0, "rows"),     # 48 rows per KV head
+    (4, 1, 64, "bf16", [1300], 16, 2, 0, "heads"),       # 64
+    (4, 1, 64, "bf16", [1300, 128], 17, 2, 0, "rows"),   # 68
+    (3, 3, 64, "bf16", [640], 256, 7, 1, "rows"),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", UNEQUAL)
+def test_unequal_lengths_and_row_blocks(gpu, case):
+    hq, hkv, d, dtype, past, n, pad, extra, layout = case
+    rng = np.random.default_rng(n + d + len(past))
+    q, k, v = _data(rng, len(past), n, max(past) + n + extra, hq, hkv, d, dtype)
+    parents = _tree(rng, len(past), n, pad)
+    want = oc.tree_attention(q, k, v, past, parents)
+    got = _run(gpu, q, k, v, past, parents, dtype, layout)
+    _check_attention(got, want, q, k, v, dtype, dtype == "bf16")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,n", [(4, 12), (4, 4), (4, 40)])
+def test_little_of_a_large_cache(gpu, hq, n):
+    """A short past in a cache too large for the last-level cache; its other rows are NaN."""
+    from longctx100m_amd import cache as kv
+
+    rng = np.random.default_rng(41)
+    past, c, d = 900, 530_000, 64
+    q, k, v = _data(rng, 1, n, past + n, hq, 1, d, "bf16")
+    tk, tv = (_nan(gpu, 1, c, 1, d, dtype=gpu.bfloat16) for _ in range(2))
+    tk[:, :past + n] = _to(gpu, k, "bf16")
+    tv[:, :past + n] = _to(gpu, v, "bf16")
+    got = kv.tree_attention(_to(gpu, q, "bf16"), tk, tv, _i32(gpu, [past]))
+    _check_attention(got, oc.tree_attention(q, k, v, [past]), q, k, v, "bf16", True)
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits(gpu):
+    """Every operator on caches whose sequences, heads and rows lie gigabytes apart."""
+    from longctx100m_amd import cache as kv
+
+    rng = np.random.default_rng(42)
+    b, c, hq, hkv, d, n, past = 2, 80, 4, 2, 64, 8, [72, 41]
+    strides = (2 ** 32 + 64, 2 ** 22, 2 ** 31 + 128, 1)
+    size = sum(s * (x - 1) for s, x in zip(strides, (b, c, hkv, d))) + 1
+    q, k, v = _data(rng, b, n, c, hq, hkv, d, "bf16")
+    big = [gpu.empty(size, dtype=gpu.bfloat16, device="cuda") for _ in range(2)]
+    tk, tv = (x.as_strided((b, c, hkv, d), strides) for x in big)
+    tk.copy_(_to(gpu, k, "bf16"))
+    tv.copy_(_to(gpu, v, "bf16"))
+    parents = _tree(rng, b, n)
+    tq, tpast, tpar = _to(gpu, q, "bf16"), _i32(gpu, past), _i32(gpu, parents)
+    got = kv.tree_attention(tq, tk, tv, tpast, tpar)
+    _check_attention(got, oc.tree_attention(q, k, v, past, parents), q, k, v, "bf16", True)
+    m, l = (x.cpu().numpy() for x in got[1:])
+    for rows in (1, n):  # one token a sequence, and all of them
+        w = kv.key_weights(tq[:, :rows].contiguous(), tk, tpast, got[1][:, :, :rows].contiguous(),
+                           got[2][:, :, :rows].contiguous())
+        want = oc.key_weights(q[:, :rows], k, past, m[:, :, :rows], l[:, :, :rows], None,
+                              np.zeros((b, hkv, c), np.float32))
+        _check_weights(w, want, q, k, m, n * hq)
+    path = [[1, 3, 4, 7] + [-1] * 4, [0, 5] + [-1] * 6]
+    lens = kv.commit(kv.Layers([tk], [tv]), tpast, _i32(gpu, path))
+    ek, ev, en = oc.commit(k, v, past, path)
+    assert gpu.equal(tk.cpu().float(), gpu.tensor(ek)) and lens.tolist() == en
+    weights = rng.random((b, hkv, c), dtype=np.float32)
+    _, _, gn = kv.evict(tk, tv, gpu.tensor(weights).cuda(), lens, 40, sinks=2, recent=6)
+    ek, ev, _, _, fn = oc.evict(ek, ev, weights, en, 40, 2, 6, None, None, None)
+    assert gn.tolist() == fn
+    assert gpu.equal(tk.cpu().float(), gpu.tensor(ek)) and gpu.equal(tv.cpu().float(), gpu.tensor(ev))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_no_tokens(gpu, dtype):
+    """Nothing to attend with; key weights pass the earlier ones on."""
+    from longctx100m_amd import cache as kv
+
+    rng = np.random.default_rng(43)
+    q, k, v = _data(rng, 2, 0, 70, 4, 2, 64, dtype)
+    tq, tk, past = _to(gpu, q, dtype), _to(gpu, k, dtype), _i32(gpu, [66, 3])
+    out, m, l = kv.tree_attention(tq, tk, tk, past)
+    assert out.shape == (2, 0, 4, 64) and m.shape == l.shape == (2, 4, 0)
+    old = gpu.rand(2, 2, 70, device="cuda")
+    hold = gpu.rand(2, 2, 70, device="cuda")
+    got = kv.key_weights(tq, tk, past, m, l, old, out=hold.clone())
+    for x, n in enumerate((66, 3)):
+        assert gpu.equal(got[x, :, :n], old[x, :, :n])
+        assert gpu.equal(got[x, :, n:], hold[x, :, n:])
+    layers = kv.Layers([tk], [tk.clone()])
+    lens = kv.commit(layers, past, gpu.zeros(2, 0, dtype=gpu.int32, device="cuda"))
+    assert lens.tolist() == [66, 3]
+
+
 # ------------------------------------------------------------- key weights --
 
 WEIGHTS = [
@@ -253,6 +352,9 @@ WEIGHTS = [
     (2, 1, 16, "fp32", [33], 9, 0, 0, "slice"),
     (4, 2, 80, "bf16", [70], 33, 0, 0, "rows"),
     (4, 1, 256, "fp32", [129, 64], 11, 0, 0, "rows"),
+    (16, 1, 128, "bf16", [400, 1], 1, 0, 0, "rows"),          # all heads share one KV head
+    (32, 1, 64, "bf16", [400, 64], 3, 0, 0, "rows"),
+    (8, 1, 128, "bf16", [30] * 70 + [1500], 2, 0, 0, "rows"),  # one long sequence among many
 ]
 
 
@@ -356,6 +458,8 @@ EVICT = [
     ([20001], 20011, 3, 16, 5000, 16, 100, "bf16", "rows", 3),
     ([70000], 70000, 1, 16, 33000, 4, 1000, "bf16", "rows", 0),
     ([50], 64, 2, 256, 400, 4, 8, "fp32", "rows", 0),   # more room than rows
+    ([600000], 600000, 1, 16, 250000, 4, 64, "bf16", "rows", 0),
+    ([300000, 5, 270001], 300000, 1, 16, 269000, 0, 9, "bf16", "heads", 0),
 ]
 
 
@@ -600,7 +704,9 @@ def test_python_checks(gpu):
     with pytest.raises(ValueError, match="positions"):
         kv.evict(k, k.clone(), w, past, 4, kept=past)
     with pytest.raises(ValueError, match="same shape"):
-        kv.Layers([k, k], [k, k[:, :4]])
+        kv.Layers([k, k.clone()], [k.clone(), k[:, :4]])
+    with pytest.raises(ValueError, match="listed twice"):
+        kv.Layers([k, k.clone()], [k.clone(), k])
     m = gpu.zeros(1, 4, 2, device="cuda")
     with pytest.raises(ValueError):
         kv.key_weights(q, k, past, m, m, gpu.zeros(1, 2, 9, device="cuda"))

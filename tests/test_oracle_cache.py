@@ -73,15 +73,15 @@ def _cache(**kw):
 
 
 def _calls(lib, c):
-    ks = (ctypes.c_void_p * 1)(P)
-    pp = ctypes.cast(ks, ctypes.POINTER(ctypes.c_void_p))
+    ks, vs = (ctypes.c_void_p * 1)(P), (ctypes.c_void_p * 1)(2 * P)
+    pp, vv = (ctypes.cast(x, ctypes.POINTER(ctypes.c_void_p)) for x in (ks, vs))
     big = 1 << 40
     return {
         "attn": lambda: lib.lc_cache_attn(c, P, None, P, P, P, P, P, P, P, big, None),
         "weights": lambda: lib.lc_cache_weights(c, P, None, P, P, P, P, None, P, None),
         "evict": lambda: lib.lc_cache_evict(c, 10, 1, 1, P, None, None, P, P, P, None, 2 * P,
                                             3 * P, 4 * P, P, big, None),
-        "commit": lambda: lib.lc_cache_commit(c, 1, pp, pp, P, 2 * P, 3 * P, None),
+        "commit": lambda: lib.lc_cache_commit(c, 1, pp, vv, P, 2 * P, 3 * P, None),
     }
 
 
@@ -106,6 +106,8 @@ ALL = ("attn", "weights", "evict", "commit")
     (dict(heads_q=2 << 24), _lib.LC_ERR_UNSUPPORTED, READS),
     (dict(seq_stride=0), _lib.LC_ERR_INVALID, ("evict", "commit")),      # sequences share rows
     (dict(row_stride=64), _lib.LC_ERR_INVALID, ("evict", "commit")),     # rows overlap heads
+    (dict(seq_stride=(1 << 40) + 8), _lib.LC_ERR_UNSUPPORTED, ("attn", "weights", "evict", "commit")),
+    (dict(head_stride=(1 << 40) + 8), _lib.LC_ERR_UNSUPPORTED, ("attn", "weights", "evict", "commit")),
     (dict(head_stride=32), _lib.LC_ERR_INVALID, ("evict", "commit")),
 ])
 def test_cache_refusals(kw, code, who):
@@ -158,13 +160,14 @@ def test_argument_refusals():
     assert ev(pos=2 * P) == inv and ev(po=5 * P) == inv
     assert ev(ws=lib.lc_cache_evict_workspace_bytes(c) - 1) == _lib.LC_ERR_WORKSPACE
     # commit
-    ks = (ctypes.c_void_p * 2)(P, None)
-    pp = ctypes.cast(ks, ctypes.POINTER(ctypes.c_void_p))
-    assert lib.lc_cache_commit(c, 2, pp, pp, P, 2 * P, 3 * P, None) == inv and "layer 1" in err()
-    assert lib.lc_cache_commit(c, -1, pp, pp, P, 2 * P, 3 * P, None) == inv
-    assert lib.lc_cache_commit(c, 1, pp, pp, P, 2 * P, P + 4, None) == inv
-    assert lib.lc_cache_commit(c, 1, pp, pp, P, 2 * P, 2 * P + 28, None) == inv
+    ks, vs = (ctypes.c_void_p * 2)(P, None), (ctypes.c_void_p * 2)(2 * P, 3 * P)
+    pp, vv = (ctypes.cast(x, ctypes.POINTER(ctypes.c_void_p)) for x in (ks, vs))
+    assert lib.lc_cache_commit(c, 2, pp, vv, P, 2 * P, 3 * P, None) == inv and "layer 1" in err()
+    assert lib.lc_cache_commit(c, -1, pp, vv, P, 2 * P, 3 * P, None) == inv
+    assert lib.lc_cache_commit(c, 1, pp, vv, P, 2 * P, P + 4, None) == inv
+    assert lib.lc_cache_commit(c, 1, pp, vv, P, 2 * P, 2 * P + 28, None) == inv
     assert lib.lc_cache_commit(c, 1, None, pp, P, 2 * P, 3 * P, None) == inv
+    assert lib.lc_cache_commit(c, 1, pp, pp, P, 2 * P, 3 * P, None) == inv and "same cache" in err()
 
 
 def test_python_refuses_cpu_tensors():
@@ -190,5 +193,6 @@ def test_workspace_does_not_grow_with_the_capacity_alone():
     lib = _lib.load()
     size = lambda **kw: lib.lc_cache_attn_workspace_bytes(_cache(**kw))  # noqa: E731
     long = dict(capacity=1 << 20, seq_stride=(1 << 20) * 128)
-    assert size(**long) <= size(capacity=1 << 17, seq_stride=(1 << 17) * 128)
+    assert size(**long) == size(capacity=1 << 19, seq_stride=(1 << 19) * 128)
+    assert size(tokens=0) == 0
     assert size(tokens=64, **long) < 64 << 20
