@@ -253,18 +253,17 @@ __global__ __launch_bounds__(256) void cache_prefix32_kernel(AttnArgs a) {
 // of their split in turn and meet in LDS.  (Workgroups of one wave, eight on a
 // CU, took 204 us against 190 at 262,000 keys, 8 KV heads of 128 and 8 tokens,
 // and left the merge 2048 partials.)
-// Rows of 128 dims are read non-temporally: one workgroup reads them once, and
-// the partials stay in L2 for the merge: 53 us in all against 56 at 60,000 keys
+// NT, rows of 128 dims that one workgroup reads once: non-temporal loads, which
+// leave the partials in L2 for the merge: 53 us in all against 56 at 60,000 keys
 // and 4 tokens, 194 against 200 at 262,000 (5.7 TB/s).  Rows of 64 are one cache
-// line of which each load takes half, and may have several row blocks that read
-// them: 30.1 us in all against 35.0 at 60,000 keys and 8 tokens, 112 against 118
-// at 262,000 and 4 (5.0 TB/s), 36 against 49 with 256 query rows at 16,000.
-template <int D, int NB>
+// line of which each load takes half: 30.1 us in all against 35.0 at 60,000 keys
+// and 8 tokens, 112 against 118 at 262,000 and 4 (5.0 TB/s).  Two row blocks
+// find in L2 what the other has read.
+template <int D, int NB, bool NT>
 __global__ __launch_bounds__(256, 2) void cache_stream_kernel(AttnArgs a) {
   using C = DecodeTile<D>;
   constexpr int TK = C::TK, MB = C::MB, KS = C::KS, DB = C::DB;
-  constexpr int W = 4;            // waves
-  constexpr bool NT = D == 128;  // non-temporal loads
+  constexpr int W = 4;  // waves
   constexpr int kRows = 16 * NB;
   constexpr int kStages = 2;
   constexpr int kPitch = D + 4;  // floats per row of a wave's partial
@@ -932,12 +931,13 @@ constexpr int64_t kManyRows = 1024;
 // written and merged.
 constexpr int64_t kWanted = 256;
 
-// K rows of head_dim 64, bf16, of which a cache of as many (V too) stays in the
-// last-level cache: up to there 33 to 64 query rows take it twice, by two
-// workgroups of 32 rows, which is faster than 64 rows at once with their one K
-// tile in flight: 7.2 us against 9.4 at 8 x 4,000 rows, 26.2 against 28.0 at 8 x
-// 60,000, but 148 against 104 at 8 x 262,000.
-constexpr int64_t kCachedRows = 1 << 19;
+// Bytes of K and V, at their capacity, of which enough stays in the caches for 33
+// to 64 query rows to take them twice, by two workgroups of 32 rows.  Beyond,
+// one reads them once.  8 KV heads of 64 and 16 tokens: 26.2 us against 28.0 at
+// 60,000 keys, 148 against 104 at 262,000.  Of 128: 16 tokens 14.5 us in all
+// against 15.8 at 500 keys, 19.0 against 22.1 at 4,000, 25.4 against 28.5 at
+// 16,000, but 70 against 58 at 60,000.
+constexpr int64_t kCachedBytes = 1 << 27;
 
 enum class Form { kFp32, kStream, kTiled };
 
@@ -952,14 +952,15 @@ Plan make_plan(const CacheProblem& p) {
   const int64_t R = (int64_t)p.N * (p.Hq / p.Hkv);
   const int64_t tiles = (int64_t)p.B * ((p.C + kTile - 1) / kTile);
   const bool bf16 = p.dtype == 1 && !p.precise && (p.D == 64 || p.D == 128);
+  const bool cached = (int64_t)p.B * p.C * p.Hkv * p.D * 4 <= kCachedBytes;
   Plan x;
   x.waves = 4;
   if (!bf16) {
     x.form = Form::kFp32;
     x.rows = R <= 16 ? 16 : R <= 32 ? 32 : 64;
-  } else if (R <= 32 || p.D == 64) {
+  } else if (R <= 32 || p.D == 64 || (R <= 64 && cached)) {
     x.form = Form::kStream;
-    x.rows = R <= 16 ? 16 : R <= 32 || (R <= 64 && (int64_t)p.B * p.C * p.Hkv <= kCachedRows) ? 32 : 64;
+    x.rows = R <= 16 ? 16 : R <= 32 || (R <= 64 && cached) ? 32 : 64;
   } else {
     x.form = Form::kTiled;
     x.waves = 8;
@@ -1024,11 +1025,14 @@ hipError_t launch_cache_attn(const CacheProblem& p, const void* q, const void* k
     else if (p.D <= 128) prefix(cache_prefix32_kernel<T, 8>);
     else prefix(cache_prefix32_kernel<T, 16>);
   };
+  const bool once = x.units == p.Hkv;  // the cache is read once: L2 need not keep it
   auto stream = [&](auto d) {
     constexpr int kD = decltype(d)::value;
-    if (x.rows == 16) prefix(cache_stream_kernel<kD, 1>);
-    else if (x.rows == 32) prefix(cache_stream_kernel<kD, 2>);
-    else if constexpr (kD == 64) prefix(cache_stream_kernel<kD, 4>);
+    constexpr bool kNt = kD == 128;
+    if (x.rows == 16) prefix(cache_stream_kernel<kD, 1, kNt>);
+    else if (x.rows == 32 && once) prefix(cache_stream_kernel<kD, 2, kNt>);
+    else if (x.rows == 32) prefix(cache_stream_kernel<kD, 2, false>);
+    else if constexpr (kD == 64) prefix(cache_stream_kernel<kD, 4, false>);
   };
   if (x.form == Form::kFp32) {
     if (p.dtype == 1) fp32(uint16_t{});
@@ -1037,7 +1041,6 @@ hipError_t launch_cache_attn(const CacheProblem& p, const void* q, const void* k
     if (p.D == 64) stream(std::integral_constant<int, 64>{});
     else stream(std::integral_constant<int, 128>{});
   } else {
-    const bool once = x.units == p.Hkv;  // the cache is read once: L2 need not keep it
     if (x.rows == 128) prefix(cache_tile128_kernel<4, true>);
     else if (once) prefix(cache_tile128_kernel<8, true>);
     else prefix(cache_tile128_kernel<8, false>);

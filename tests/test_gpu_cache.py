@@ -245,6 +245,8 @@ UNEQUAL = [
     (2, 2, 32, "fp32", [20] * 63 + [900], 2, 0, 0, "rows"),
     (4, 1, 64, "bf16", [700, 90], 12, 0, 0, "rows"),     # 48 rows per KV head
     (4, 1, 64, "bf16", [1300], 16, 2, 0, "heads"),       # 64
+    (8, 2, 128, "bf16", [1300, 0, 65], 9, 0, 0, "slice"),   # 36
+    (8, 2, 128, "bf16", [700], 16, 1, 3, "heads"),       # 64
     (4, 1, 64, "bf16", [1300, 128], 17, 2, 0, "rows"),   # 68
     (3, 3, 64, "bf16", [640], 256, 7, 1, "rows"),
 ]
