@@ -137,6 +137,8 @@ __device__ __forceinline__ int64_t partial_row(const AttnArgs& a, int r, int hk,
 
 // ------------------------------------------------- the past, fp32 products --
 
+// fp32, precise bf16 and other head dims, on the fp32 matrix cores (13 tokens of
+// 2 x 9/3 heads of 64 over 2,047 keys: 11 us).
 // Waves of a workgroup: wave_rows blocks of 16 rows, each by 4 / wave_rows
 // waves that take the 16-key tiles in turn and meet in LDS.
 template <typename T, int NJ>
@@ -250,9 +252,10 @@ __global__ __launch_bounds__(256) void cache_prefix32_kernel(AttnArgs a) {
 // and of V, through LDS for the transposed reads of O^T += V^T P^T; both one
 // tile ahead.  With 64 rows there are registers for one K tile: the next is
 // read once the scores are there.  The four waves of a workgroup take the tiles
-// of their split in turn and meet in LDS.  (Workgroups of one wave, eight on a
-// CU, took 204 us against 190 at 262,000 keys, 8 KV heads of 128 and 8 tokens,
-// and left the merge 2048 partials.)
+// of their split in turn and meet in LDS.  (2,048 workgroups of one wave, the
+// slots of a KV head next to each other, gain with up to 16 rows and 262,000 keys
+// alone, 174 us against 193 for one token; up to 120,000 keys the merge of their
+// partials costs what they gain, and with 32 rows they gain nothing.)
 // NT, rows of 128 dims that one workgroup reads once: non-temporal loads, which
 // leave the partials in L2 for the merge: 53 us in all against 56 at 60,000 keys
 // and 4 tokens, 194 against 200 at 262,000 (5.7 TB/s).  Rows of 64 are one cache

@@ -173,10 +173,10 @@ __device__ __forceinline__ Seq seq_of(const WeightArgs& a, int b) {
 
 // Few query rows: bound by the stream of K.  A wave holds the rows (Q as the A
 // operand of S = Q K^T) and streams 64-key tiles straight into registers as the
-// B operand, one tile ahead and non-temporal.  A lane then has one key and four
-// rows of each product: the sum over rows is four adds and two lane swaps.
-// One-wave workgroups, the KV heads of a key range next to each other (their
-// rows are adjacent in memory).
+// B operand, one tile ahead.  A lane then has one key and four rows of each
+// product: the sum over rows is four adds and two lane swaps.  One-wave
+// workgroups, the key ranges of a KV head next to each other.  One token of 32/8
+// heads of 128 over 262,144 keys (537 MB): 101 us, 5.3 TB/s.
 template <int D>
 __global__ __launch_bounds__(64) void cache_weights_stream_kernel(WeightArgs a) {
   constexpr int KS = D / 32, MB = 4;
@@ -289,8 +289,17 @@ struct QTile {
 // stream past them, 64 to a wave, in registers one tile ahead; no barrier after
 // the start.  S = Q K^T (32 x 32 x 16): a lane has one key and 16 rows of each
 // product, whose statistics are broadcast from LDS.  Rows that give nothing
-// are zeros with lse = inf (p = 0); a tile of such rows alone is left out.
+// are zeros with lse = inf (p = 0); a tile of such rows alone is left out.  32/8
+// heads of 128 over 262,000 keys: 8 tokens 118 us (4.5 TB/s), 26 130, 64 164 (670
+// TFLOP/s).  Non-temporal loads of K, which each workgroup reads once too, took
+// 182 there.
 constexpr int kHeldRows = 256;
+// With two 64-key tiles or fewer for each of the chip's 1,024 waves the rows
+// pass by the keys faster than the keys by more than 64 rows (32/8 heads of 128:
+// 64 tokens over 4,000 keys 13.1 us against 22.3, 26 over 16,000 17.4 against
+// 18.9); with more keys not (26 over 32,000 28.7 against 23.8, 64 over 262,000 252
+// against 164), nor with fewer rows (16 tokens over 4,000 keys 11.4 against 10.0).
+constexpr int64_t kFewKeys = 1 << 17;
 template <int D>
 __global__ __launch_bounds__(256, 2) void cache_weights_rows_kernel(WeightArgs a) {
   using Q = QTile<D>;
@@ -414,7 +423,8 @@ __global__ __launch_bounds__(256, 2) void cache_weights_rows_kernel(WeightArgs a
 // operand of S^T = K Q^T); the tokens of one query head after the other pass
 // through LDS, kTok at a time, two buffers.  A lane has one query row and 16
 // keys of each product, so a row's statistics are one register and a key's sum
-// stays in its lane until the end.
+// stays in its lane until the end.  512 tokens of 32/8 heads of 128 behind 32,000
+// keys: 154 us, 880 TFLOP/s.
 template <int D>
 __global__ __launch_bounds__(256, 2) void cache_weights_tile_kernel(WeightArgs a) {
   using Q = QTile<D>;
@@ -656,9 +666,11 @@ hipError_t launch_cache_weights(const CacheProblem& p, const void* q, const void
     constexpr int kD = decltype(d)::value;
     const int64_t heads = (int64_t)p.B * p.Hkv, tiles = (p.C + 63) / 64;
     // As many workgroups as the chip holds, in which the lengths are dealt out.
+    // Up to 16 rows: one token over 262,000 keys 107 us against 117 with the rows
+    // in LDS, four over 4,000 5.6 against 6.5.
     if (a.R <= 16)
       launch(cache_weights_stream_kernel<kD>, std::min(std::max<int64_t>(1, 2048 / heads), tiles), 64);
-    else if (a.R <= kHeldRows && p.N <= 64)
+    else if (a.R <= kHeldRows && p.N <= 64 && (a.R <= 64 || heads * p.C > kFewKeys))
       launch(cache_weights_rows_kernel<kD>, std::min(std::max<int64_t>(1, 512 / heads), (tiles + 3) / 4), 256);
     else
       launch(cache_weights_tile_kernel<kD>, (p.C + 255) / 256, 256);

@@ -357,6 +357,8 @@ WEIGHTS = [
     (16, 1, 128, "bf16", [400, 1], 1, 0, 0, "rows"),          # all heads share one KV head
     (32, 1, 64, "bf16", [400, 64], 3, 0, 0, "rows"),
     (8, 1, 128, "bf16", [30] * 70 + [1500], 2, 0, 0, "rows"),  # one long sequence among many
+    (8, 2, 128, "bf16", [150], 40, 3, 66000, "rows"),         # 160 rows, a large cache
+    (8, 2, 64, "bf16", [300, 64], 33, 0, 33000, "heads"),
 ]
 
 
