@@ -338,6 +338,30 @@ def test_no_tokens(gpu, dtype):
     assert lens.tolist() == [66, 3]
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,n,dtype", [(128, 3, "bf16"), (128, 40, "bf16"), (64, 20, "bf16"),
+                                       (64, 4, "fp32")])
+def test_lengths_beyond_the_capacity(gpu, d, n, dtype):
+    """A past that counts more rows than there are: its tokens have no place, and
+    every row is a past one."""
+    from longctx100m_amd import cache as kv
+
+    rng = np.random.default_rng(44)
+    past, c = [2 ** 31 - 1, 90, 200, 199], 200
+    q, k, v = _data(rng, 4, n, c, 4, 2, d, dtype)
+    got = _run(gpu, q, k, v, past, None, dtype)
+    want = oc.tree_attention(q, k, v, past)
+    assert not np.isfinite(want[1][0]).any() and np.isfinite(want[1][3]).any()
+    _check_attention(got, want, q, k, v, dtype, dtype == "bf16")
+    old = rng.random((4, 2, c), dtype=np.float32)
+    m, l = (x.cpu().numpy() for x in got[1:])
+    w = kv.key_weights(_to(gpu, q, dtype), _to(gpu, k, dtype), _i32(gpu, past), *got[1:],
+                       gpu.tensor(old).cuda())
+    want = oc.key_weights(q, k, past, m, l, old, np.zeros_like(old))
+    _check_weights(w, want, q, k, m, 4 * n)
+    assert np.array_equal(w[0].cpu().numpy(), old[0])
+
+
 # ------------------------------------------------------------- key weights --
 
 WEIGHTS = [
@@ -512,6 +536,66 @@ def test_evict(gpu, case, ties):
             else:
                 assert (gw[x, :, n:] == 0).all() and (gp[x, :, n:] == 0).all()
                 np.testing.assert_array_equal(tw.cpu().numpy(), w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("c", [70, 20000])
+def test_evict_extremes(gpu, c):
+    """Lengths and kept counts beyond the cache, infinities and NaN of both signs."""
+    from longctx100m_amd import cache as kv
+
+    rng = np.random.default_rng(45)
+    lens, kept, ends = [2 ** 31 - 1, c, -5, c - 1], [c + 9, 2 ** 31 - 1, 4, -1], [c + 50, c, 0, 7]
+    _, k, v = _data(rng, 4, 1, c, 2, 2, 16, "bf16")
+    w = rng.choice(np.array([-np.inf, np.inf, np.nan, -np.nan, -0.0, 0.0, 3e38, -3e38, 1e-45, -1e-45],
+                            np.float32), (4, 2, c))
+    pos = rng.integers(0, c + 40, (4, 2, c)).astype(np.int32)
+    budget, sinks, recent = c - 30, 5, 20
+    want = oc.evict(k, v, w, lens, budget, sinks, recent, pos, kept, ends)
+    tk, tv = _to(gpu, k, "bf16"), _to(gpu, v, "bf16")
+    got = kv.evict(tk, tv, gpu.tensor(w).cuda(), _i32(gpu, lens), budget, sinks=sinks,
+                   recent=recent, positions=gpu.tensor(pos).cuda(), kept=_i32(gpu, kept),
+                   ends=_i32(gpu, ends))
+    assert got[2].tolist() == want[4]
+    np.testing.assert_array_equal(tk.float().cpu().numpy(), want[0])
+    np.testing.assert_array_equal(tv.float().cpu().numpy(), want[1])
+    for x, n in enumerate(want[4]):
+        np.testing.assert_array_equal(got[0][x, :, :n].cpu().numpy(), want[2][x, :, :n])
+        np.testing.assert_array_equal(got[1][x, :, :n].cpu().numpy(), want[3][x, :, :n])
+
+
+@pytest.mark.gpu
+def test_other_operators_on_two_streams(gpu):
+    """Weights, evictions and commits that overlap, each on tensors of its own."""
+    from longctx100m_amd import cache as kv
+
+    rng = np.random.default_rng(46)
+    c, n = 20000, 8
+    runs = []
+    for _ in range(2):
+        q, k, v = _data(rng, 1, n, c, 8, 2, 64, "bf16")
+        runs.append((_to(gpu, q, "bf16"), _to(gpu, k, "bf16"), _to(gpu, v, "bf16")))
+
+    def go(q, k, v):
+        k, v = k.clone(), v.clone()
+        past = _i32(gpu, [c - n])
+        _, m, l = kv.tree_attention(q, k, v, past)
+        w = kv.key_weights(q, k, past, m, l)
+        lens = kv.commit(kv.Layers([k], [v]), past, _i32(gpu, [[1, 2, 5, -1]]))
+        return (k, v, *kv.evict(k, v, w, lens, 12000, sinks=4, recent=30))
+
+    alone = [go(*r) for r in runs]
+    gpu.cuda.synchronize()
+    streams = [gpu.cuda.Stream(), gpu.cuda.Stream()]
+    outs = [[], []]
+    for _ in range(5):
+        for i in (0, 1):
+            with gpu.cuda.stream(streams[i]):
+                outs[i].append(go(*runs[i]))
+    gpu.cuda.synchronize()
+    for i in (0, 1):
+        for got in outs[i]:
+            assert all(gpu.equal(x, y) for x, y in zip(got, alone[i]))
 
 
 # ------------------------------------------------------------------ commit --
