@@ -465,7 +465,7 @@ __global__ __launch_bounds__(256, 2) void cache_stream_kernel(AttnArgs a) {
   }
 }
 
-// ------------------------------------- the past, bf16, head_dim 128, 33+ rows --
+// ---------------------------------- the past, bf16, head_dim 128, many rows --
 
 // Many query rows: the matrix cores and the softmax beside them bound it.  Eight
 // waves of 32 rows over 64-key tiles of K and V in LDS (tile128.h), filled by LDS
@@ -934,13 +934,17 @@ constexpr int64_t kManyRows = 1024;
 // written and merged.
 constexpr int64_t kWanted = 256;
 
-// Bytes of K and V, at their capacity, of which enough stays in the caches for 33
-// to 64 query rows to take them twice, by two workgroups of 32 rows.  Beyond,
-// one reads them once.  8 KV heads of 64 and 16 tokens: 26.2 us against 28.0 at
-// 60,000 keys, 148 against 104 at 262,000.  Of 128: 16 tokens 14.5 us in all
-// against 15.8 at 500 keys, 19.0 against 22.1 at 4,000, 25.4 against 28.5 at
-// 16,000, but 70 against 58 at 60,000.
-constexpr int64_t kCachedBytes = 1 << 27;
+// Bytes of K and V, at their capacity, that all row blocks of 32 read together,
+// up to which those are the best form for more rows too: the second block finds
+// in the caches what the first has read, and the waves need not wait for each
+// other.  Beyond, 64, 128 or 256 rows a workgroup read less.  32/8 heads of 128,
+// in all: 16 tokens 18.9 us against 21.8 at 4,000 keys, 30.2 against 33.6 at
+// 24,000, 70 against 58 at 60,000; 26 tokens 21.0 against 25.1 at 4,000, 35.3
+// against 33.2 at 16,000; 64 tokens 21.6 against 28.3 at 500, 30.4 against 40.8 at
+// 4,000, 59 against 53 at 16,000.  Of 64: 16 tokens 26.2 against 28.0 at 60,000
+// keys, 148 against 104 at 262,000; 26 tokens 16.5 against 18.6 at 4,000, 50.7
+// against 43.0 at 60,000.
+constexpr int64_t kBlockBytes = 240 << 20;
 
 enum class Form { kFp32, kStream, kTiled };
 
@@ -955,15 +959,15 @@ Plan make_plan(const CacheProblem& p) {
   const int64_t R = (int64_t)p.N * (p.Hq / p.Hkv);
   const int64_t tiles = (int64_t)p.B * ((p.C + kTile - 1) / kTile);
   const bool bf16 = p.dtype == 1 && !p.precise && (p.D == 64 || p.D == 128);
-  const bool cached = (int64_t)p.B * p.C * p.Hkv * p.D * 4 <= kCachedBytes;
+  const bool blocks = R <= 32 || (R + 31) / 32 * p.B * p.C * p.Hkv * p.D * 4 <= kBlockBytes;
   Plan x;
   x.waves = 4;
   if (!bf16) {
     x.form = Form::kFp32;
     x.rows = R <= 16 ? 16 : R <= 32 ? 32 : 64;
-  } else if (R <= 32 || p.D == 64 || (R <= 64 && cached)) {
+  } else if (blocks || p.D == 64) {
     x.form = Form::kStream;
-    x.rows = R <= 16 ? 16 : R <= 32 || (R <= 64 && cached) ? 32 : 64;
+    x.rows = R <= 16 ? 16 : blocks ? 32 : 64;
   } else {
     x.form = Form::kTiled;
     x.waves = 8;

@@ -264,20 +264,42 @@ def test_unequal_lengths_and_row_blocks(gpu, case):
     _check_attention(got, want, q, k, v, dtype, dtype == "bf16")
 
 
+# hq, hkv, d, past of each sequence, tokens, padding, capacity, layout
+LARGE = [
+    (4, 1, 64, [900], 12, 0, 530_000, "rows"),
+    (4, 1, 64, [900], 4, 1, 530_000, "rows"),
+    (4, 1, 64, [900], 40, 0, 530_000, "heads"),
+    (4, 1, 128, [900], 10, 2, 250_000, "rows"),                    # 40 rows per KV head
+    (32, 8, 128, [2111], 26, 0, 16_000, "rows"),                   # 104
+    (4, 1, 128, [0, 1, 63, 64, 65, 127, 128, 129, -1], 17, 3, 40_000, "rows"),
+    (4, 2, 128, [1, 700], 64, 1, 40_000, "heads"),                 # 128
+    (4, 2, 128, [777], 70, 4, 60_000, "rows"),                     # 140
+    (4, 1, 128, [1200, 0, 65, 128, 40], 64, 5, 30_000, "heads"),   # 256
+    (9, 3, 128, [2300, 64, 191], 85, 0, 10_000, "rows"),           # 255, three heads a KV head
+    (4, 1, 128, [777, 1300], 256, 9, 32_000, "rows"),              # 1,024
+]
+
+
 @pytest.mark.gpu
-@pytest.mark.parametrize("hq,n", [(4, 12), (4, 4), (4, 40)])
-def test_little_of_a_large_cache(gpu, hq, n):
-    """A short past in a cache too large for the last-level cache; its other rows are NaN."""
+@pytest.mark.parametrize("case", LARGE)
+def test_little_of_a_large_cache(gpu, case):
+    """Short pasts in caches of a large capacity, whose other rows are NaN: the
+    forms that read each row once."""
     from longctx100m_amd import cache as kv
 
-    rng = np.random.default_rng(41)
-    past, c, d = 900, 530_000, 64
-    q, k, v = _data(rng, 1, n, past + n, hq, 1, d, "bf16")
-    tk, tv = (_nan(gpu, 1, c, 1, d, dtype=gpu.bfloat16) for _ in range(2))
-    tk[:, :past + n] = _to(gpu, k, "bf16")
-    tv[:, :past + n] = _to(gpu, v, "bf16")
-    got = kv.tree_attention(_to(gpu, q, "bf16"), tk, tv, _i32(gpu, [past]))
-    _check_attention(got, oc.tree_attention(q, k, v, [past]), q, k, v, "bf16", True)
+    hq, hkv, d, past, n, pad, c, layout = case
+    rng = np.random.default_rng(n + d)
+    b, used = len(past), max(past) + n
+    q, k, v = _data(rng, b, n, used, hq, hkv, d, "bf16")
+    if layout == "heads":
+        tk, tv = (_nan(gpu, b, hkv, c, d, dtype=gpu.bfloat16).transpose(1, 2) for _ in range(2))
+    else:
+        tk, tv = (_nan(gpu, b, c, hkv, d, dtype=gpu.bfloat16) for _ in range(2))
+    tk[:, :used] = _to(gpu, k, "bf16")
+    tv[:, :used] = _to(gpu, v, "bf16")
+    parents = _tree(rng, b, n, pad)
+    got = kv.tree_attention(_to(gpu, q, "bf16"), tk, tv, _i32(gpu, past), _i32(gpu, parents))
+    _check_attention(got, oc.tree_attention(q, k, v, past, parents), q, k, v, "bf16", True)
 
 
 @pytest.mark.gpu
