@@ -931,7 +931,10 @@ __global__ __launch_bounds__(64 * WPR) void cache_merge_kernel(AttnArgs a) {
 constexpr int64_t kManyRows = 1024;
 
 // Workgroups for a whole chip, one a CU: each split costs a partial that is
-// written and merged.
+// written and merged.  The fp32 form takes two where it waits for its products
+// and has the registers for them: 64 tokens of 32/8 heads over 16,000 keys, in
+// all, 129 us against 164 at head_dim 64 and 242 against 274 at 128, but 8 tokens
+// of 128 48 against 45, one 40 against 29.
 constexpr int64_t kWanted = 256;
 
 // Bytes of K and V, at their capacity, that all row blocks of 32 read together,
@@ -974,7 +977,9 @@ Plan make_plan(const CacheProblem& p) {
     x.rows = R <= 128 ? 128 : 256;
   }
   x.units = (int)((R + x.rows - 1) / x.rows * p.Hkv);
-  const int64_t slots = std::max<int64_t>(1, std::min<int64_t>(kWanted / x.units, tiles));
+  const bool twice = x.form == Form::kFp32 && (p.D <= 96 || R > 64);
+  const int64_t want = twice ? 2 * kWanted : kWanted;
+  const int64_t slots = std::max<int64_t>(1, std::min<int64_t>(want / x.units, tiles));
   // A batch of nearly as many sequences as slots, or more, has some left for its
   // long ones: 39 sequences of 300 keys and one of 16,000 take 59 us, with a slot
   // each 292.
