@@ -249,6 +249,12 @@ UNEQUAL = [
     (8, 2, 128, "bf16", [700], 16, 1, 3, "heads"),       # 64
     (4, 1, 64, "bf16", [1300, 128], 17, 2, 0, "rows"),   # 68
     (3, 3, 64, "bf16", [640], 256, 7, 1, "rows"),
+    (8, 2, 256, "fp32", [300, 65], 20, 2, 0, "rows"),    # fp32 products, more than 32 rows
+    (8, 2, 112, "bf16", [200, 3], 30, 0, 0, "heads"),
+    (4, 1, 16, "fp32", [129], 40, 0, 0, "rows"),
+    (4, 1, 32, "bf16", [77, 64, 15], 64, 6, 0, "rows"),
+    (12, 3, 128, "fp32", [1000, 0, 17, -1], 17, 1, 0, "slice"),
+    (4, 2, 80, "fp32", [500, 480], 100, 0, 2, "rows"),
 ]
 
 
