@@ -234,7 +234,10 @@ int lc_attn_bwd_shard_ws(const lc_attn_shape_t* shape, const lc_attn_mask_t* mas
  * p.  Any other value, or a chain of parents that meets one, means that the
  * token is not there (padding of a smaller tree).  A token sees the past, its
  * chain of parents and itself; NULL is the chain (each token sees those before
- * it).  Neither the kernels nor the host reads other rows of the cache. */
+ * it).  Neither the kernels nor the host reads other rows of the cache.
+ * Limits (LC_ERR_UNSUPPORTED beyond): batch * heads_kv 2^21, the same times
+ * capacity / 64 (rounded up) 2^23, batch * heads_q 2^24, tokens * heads_q 2^30,
+ * and for lc_cache_attn batch * heads_q * tokens 2^22. */
 typedef struct lc_cache {
   int32_t batch;    /* B */
   int32_t tokens;   /* new tokens of each sequence */

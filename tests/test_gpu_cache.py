@@ -593,6 +593,46 @@ def test_evict_extremes(gpu, c):
 
 
 @pytest.mark.gpu
+def test_long_caches_in_a_graph(gpu):
+    """Attention, weights, commit and an eviction of several launches, captured
+    once and replayed with other tensors, lengths and trees, beside eager calls."""
+    from longctx100m_amd import cache as kv
+
+    rng = np.random.default_rng(47)
+    b, c, n, hq, hkv, d, budget = 2, 18000, 8, 4, 2, 64, 9000
+
+    def inputs(past):
+        q, k, v = (_to(gpu, x, "bf16") for x in _data(rng, b, n, c, hq, hkv, d, "bf16"))
+        w = gpu.tensor(rng.random((b, hkv, c), dtype=np.float32)).cuda()
+        path = [[0, 3, -1, -1], [1, 2, 6, -1]]
+        return [q, k, v, w, _i32(gpu, past), _i32(gpu, _tree(rng, b, n)), _i32(gpu, path)]
+
+    def step(q, k, v, w, past, parents, path, ws):
+        out, m, l = kv.tree_attention(q, k, v, past, parents, workspace=ws[0])
+        kv.key_weights(q, k, past, m, l, w, parents, out=w)
+        lens = kv.commit(kv.Layers([k], [v]), past, path)
+        return (out, m, l, k, v, *kv.evict(k, v, w, lens, budget, sinks=4, recent=60, workspace=ws[1]))
+
+    static = inputs([0, 0])
+    ws = [gpu.empty(s, dtype=gpu.uint8, device="cuda") for s in
+          (kv.tree_attention_workspace_bytes(static[0], static[1]), kv.evict_workspace_bytes(static[1]))]
+    step(*[x.clone() for x in static], ws)
+    gpu.cuda.synchronize()
+    graph = gpu.cuda.CUDAGraph()
+    with gpu.cuda.graph(graph):
+        got = step(*static, ws)
+    for past in ([17000, 3], [17992, 12000], [8995, -1], [400, 17999]):
+        fresh = inputs(past)
+        want = step(*[x.clone() for x in fresh], [w.clone() for w in ws])
+        for x, y in zip(static, fresh):
+            x.copy_(y)
+        graph.replay()
+        gpu.cuda.synchronize()
+        for x, y in zip(got, want):
+            assert gpu.equal(x, y), past
+
+
+@pytest.mark.gpu
 def test_other_operators_on_two_streams(gpu):
     """Weights, evictions and commits that overlap, each on tensors of its own."""
     from longctx100m_amd import cache as kv

@@ -104,6 +104,9 @@ ALL = ("attn", "weights", "evict", "commit")
     (dict(row_stride=1 << 25, seq_stride=1 << 40), _lib.LC_ERR_UNSUPPORTED, ALL),
     (dict(batch=1 << 20, capacity=1 << 20), _lib.LC_ERR_UNSUPPORTED, ALL),
     (dict(heads_q=2 << 24), _lib.LC_ERR_UNSUPPORTED, READS),
+    (dict(batch=1 << 20, heads_kv=4, head_stride=64, row_stride=256), _lib.LC_ERR_UNSUPPORTED, ALL),
+    (dict(tokens=256, batch=1 << 12, heads_q=8), _lib.LC_ERR_UNSUPPORTED, ("attn",)),
+    (dict(tokens=1 << 28, heads_q=8), _lib.LC_ERR_UNSUPPORTED, READS),
     (dict(seq_stride=0), _lib.LC_ERR_INVALID, ("evict", "commit")),      # sequences share rows
     (dict(row_stride=64), _lib.LC_ERR_INVALID, ("evict", "commit")),     # rows overlap heads
     (dict(seq_stride=(1 << 40) + 8), _lib.LC_ERR_UNSUPPORTED, ("attn", "weights", "evict", "commit")),
