@@ -273,7 +273,7 @@ int lc_cache_attn(const lc_cache_t* cache, const int32_t* past, const int32_t* p
  * same rows),
  *   w[h][j] = sum over the query rows of KV head h that see row j of
  *             exp(s - m) / l
- * (a query row with l = 0 or m = -inf gives nothing), added to what was
+ * (a query row with m = -inf or an l that is not above 0 gives nothing), added to what was
  * accumulated before:
  *   weights_out[b][h][j] = weights[b][h][j] + w[h][j]   (j < past[b])
  *   weights_out[b][h][j] = w[h][j]                      (a new token's own row)

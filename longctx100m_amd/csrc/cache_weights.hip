@@ -332,10 +332,11 @@ struct QTile {
 // All query rows of the KV head (at most 64 tokens) stay in LDS and the keys
 // stream past them, 64 to a wave, in registers one tile ahead; no barrier after
 // the start.  S = Q K^T (32 x 32 x 16): a lane has one key and 16 rows of each
-// product, whose statistics are broadcast from LDS.  Rows that give nothing
-// are zeros with lse = inf (p = 0); a tile of such rows alone is left out.  32/8
+// product, whose statistics are broadcast from LDS.  Rows that give nothing are
+// zeros; a tile of such rows alone is left out, and one that has some of them
+// selects (an infinite key makes their scores NaN).  32/8
 // heads of 128 over 262,000 keys: 8 tokens 118 us (4.5 TB/s), 26 130, 64 164 (670
-// TFLOP/s).  Non-temporal loads of K, which each workgroup reads once too, took
+// TFLOP/s), of which five are padding 178, 171 without the selection.  Non-temporal loads of K, which each workgroup reads once too, took
 // 182 there.
 constexpr int kHeldRows = 256;
 // With two 64-key tiles or fewer for each of the chip's 1,024 waves the rows
@@ -353,7 +354,7 @@ __global__ __launch_bounds__(256, 2) void cache_weights_rows_kernel(WeightArgs a
   __shared__ __attribute__((aligned(16))) uint64_t bits_s[kHeldRows];
   __shared__ uint64_t seen[64];
   __shared__ int par[64];
-  __shared__ int live_s;  // one bit for each tile of 32 rows
+  __shared__ int live_s, dead_s;  // one bit for each tile of 32 rows: has rows that give something, nothing
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kc = lane & 31, hh = lane >> 5;
@@ -379,7 +380,7 @@ __global__ __launch_bounds__(256, 2) void cache_weights_rows_kernel(WeightArgs a
   if (j0 < j1) kload(j0, kra);
 
   build_bits(seen, par, a.parents ? a.parents + (int64_t)b * a.N : nullptr, a.N, sq.there);
-  if (threadIdx.x == 0) live_s = 0;
+  if (threadIdx.x == 0) live_s = dead_s = 0;
   __syncthreads();
   const int tiles = (a.R + 31) / 32;
   {  // a row of each thread
@@ -390,7 +391,7 @@ __global__ __launch_bounds__(256, 2) void cache_weights_rows_kernel(WeightArgs a
     const uint64_t bits = r < a.R && gives(m, l) ? seen[tk] : 0;
     lse_s[r] = bits != 0 ? row_lse(m, l) : INFINITY;
     bits_s[r] = bits;
-    if (bits != 0) atomicOr(&live_s, 1 << (r >> 5));
+    atomicOr(bits != 0 ? &live_s : &dead_s, 1 << (r >> 5));
   }
   __syncthreads();
   for (int x = threadIdx.x; x < 32 * tiles * Q::kLanes; x += 256) {
@@ -404,6 +405,7 @@ __global__ __launch_bounds__(256, 2) void cache_weights_rows_kernel(WeightArgs a
   }
   __syncthreads();
   const int live = __builtin_amdgcn_readfirstlane(live_s);
+  const int whole = ~__builtin_amdgcn_readfirstlane(dead_s);
 
   int qoff[KS];
 #pragma unroll
@@ -429,11 +431,18 @@ __global__ __launch_bounds__(256, 2) void cache_weights_rows_kernel(WeightArgs a
 #pragma unroll
       for (int w = 0; w < 4; ++w) lse[w] = *reinterpret_cast<const f32x4*>(lse_s + 32 * t + 8 * w + 4 * hh);
       if (key0 + 64 <= sq.past) {
+        auto add = [&](auto select) {
 #pragma unroll
-        for (int v = 0; v < 16; ++v)
+          for (int v = 0; v < 16; ++v)
 #pragma unroll
-          for (int mb = 0; mb < 2; ++mb)
-            sum[mb][v & 3] += fast_exp2(fmaf(s[mb][v], a.sl2, -lse[v >> 2][v & 3]));
+            for (int mb = 0; mb < 2; ++mb) {
+              const float x = lse[v >> 2][v & 3];
+              const float p = fast_exp2(fmaf(s[mb][v], a.sl2, -x));
+              sum[mb][v & 3] += decltype(select)::value && x == INFINITY ? 0.f : p;
+            }
+        };
+        if (whole >> t & 1) add(std::false_type{});
+        else add(std::true_type{});
       } else {
 #pragma unroll
         for (int v = 0; v < 16; ++v) {

@@ -1,0 +1,61 @@
+"""Infinities and NaN in the caches of the KV-cache operators, in every form of
+the kernels, against the float64 oracle (tolerances: test_gpu_cache.py)."""
+
+import numpy as np
+import pytest
+
+from oracle import cache as oc
+from tests.conftest import bf16_round
+from tests.test_gpu_cache import _check_weights, _data, _i32, _to, _tree
+
+pytestmark = pytest.mark.gpu
+
+
+# hq, hkv, d, tokens, capacity, dtype: query rows of a KV head and the form that takes them
+@pytest.mark.parametrize("hq,hkv,d,n,c,dtype", [
+    (4, 2, 128, 8, 170, "bf16"),      # 16: in registers
+    (4, 2, 128, 13, 170, "bf16"),     # 26: in LDS, one tile of 32
+    (4, 2, 64, 20, 170, "bf16"),      # 40
+    (4, 2, 128, 32, 170, "bf16"),     # 64, no filler
+    (8, 2, 128, 50, 70000, "bf16"),   # 200
+    (8, 2, 64, 64, 70000, "bf16"),    # 256
+    (8, 2, 128, 64, 300, "bf16"),     # 256, streamed
+    (4, 2, 64, 150, 300, "bf16"),     # 300
+    (4, 2, 64, 20, 170, "fp32"),
+])
+@pytest.mark.parametrize("tree", [True, False], ids=["tree", "chain"])
+def test_rows_that_give_nothing_give_no_nan(gpu, hq, hkv, d, n, c, dtype, tree):
+    """An infinite key gives those rows that give nothing (padding, l not above 0,
+    m = -inf) a NaN or infinite score, and every other row -inf: its weight is 0."""
+    from longctx100m_amd import cache as kv
+
+    rng = np.random.default_rng(n + d)
+    past = [130]
+    q, k, v = _data(rng, 1, n, past[0] + n, hq, hkv, d, dtype)
+    q[..., 3] = -np.abs(q[..., 3]) - 1
+    q = bf16_round(q) if dtype == "bf16" else q  # what the kernel is given
+    parents = _tree(rng, 1, n, 3) if tree else None
+    _, m, l = oc.tree_attention(q, k, v, past, parents)
+    m, l = m.astype(np.float32), l.astype(np.float32)
+    for i, h in ((5, 1), (6, 0), (7, hq - 1)):
+        q[0, i, h, 3] = (0, 2, 1)[i - 5]
+    l[0, 1, 5] = 0.0
+    l[0, 0, 6] = np.nan
+    m[0, hq - 1, 7] = -np.inf
+    if tree:
+        q[0, n - 3:, :, 3] = (0, 1, -1)[n % 3]
+    k[0, [20, 70, 129], :, 3] = np.inf
+    zeros = np.zeros((1, hkv, past[0] + n), np.float32)
+    want = oc.key_weights(q, k, past, m, l, None, zeros, parents)
+    assert (want[0, :, [20, 70, 129]] == 0).all()
+    tk = gpu.zeros(1, c, hkv, d, dtype=gpu.bfloat16 if dtype == "bf16" else gpu.float32,
+                   device="cuda")
+    tk[:, :past[0] + n] = _to(gpu, k, dtype)
+    args = (_i32(gpu, past), gpu.tensor(m).cuda(), gpu.tensor(l).cuda(), None, _i32(gpu, parents))
+    got = kv.key_weights(_to(gpu, q, dtype), tk, *args)[..., :past[0] + n]
+    _check_weights(got, want, q, k, m, n * hq)
+    tk[0, 40, 1, 7] = float("nan")  # a seen key: NaN in its own weight alone
+    got = kv.key_weights(_to(gpu, q, dtype), tk, *args)[..., :past[0] + n]
+    assert np.isnan(got[0, 1, 40].item())
+    got[0, 1, 40] = float(want[0, 1, 40])
+    _check_weights(got, want, q, k, m, n * hq)
