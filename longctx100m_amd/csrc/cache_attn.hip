@@ -8,9 +8,10 @@
 //   1. a prefix kernel attends all R = N * Hq / Hkv query rows of a KV head to
 //      a split of the past, without any mask, and leaves an unnormalised
 //      partial (o, m, l) per row and split;
-//   2. cache_merge_kernel, a wave per row, follows the row's chain, takes its
+//   2. cache_merge_kernel, one or four waves per row, follows the row's chain, takes its
 //      few keys with fp32 dot products and merges them with the partials.
-// No product with a masked probability exists, so what stands in a row that a
+// Neither multiplies a row of the cache by a masked probability (a tile that the
+// past ends in is filled up with rows of zeros), so what stands in a row that a
 // token does not see cannot reach it, whatever it is.
 //
 // The lengths are known on the device only.  The host fixes the number of
@@ -32,6 +33,10 @@ namespace lc {
 namespace {
 
 constexpr int kTile = 64;  // keys by which the past is dealt out
+
+// What the rows of a V tile behind the past hold: their probabilities are zeros,
+// but the past's last row again would make 0 * inf of an infinity in it.
+__device__ const uint4 kZeroRow = {0u, 0u, 0u, 0u};
 
 struct AttnArgs {
   const void *q, *k, *v;
@@ -295,7 +300,8 @@ __global__ __launch_bounds__(256, 2) void cache_stream_kernel(AttnArgs a) {
   const uint32_t vlds = t128::lds_addr(smem) + wave * kStages * kTileBytes;
   const uint8_t* vmem = smem + wave * kStages * kTileBytes;
   auto issue = [&](int j) {  // V tile j into stage j % kStages
-    ld.template load<NT>(vbase, a.row, kb0 + j * (W * TK), s.k1, vlds + (j % kStages) * kTileBytes, lane);
+    ld.template load<NT>(vbase, a.row, kb0 + j * (W * TK), s.k1, vlds + (j % kStages) * kTileBytes, lane,
+                          &kZeroRow);
   };
   auto kload = [&](int j, bf16x8 (&kr)[MB][KS]) {  // lane (c, g): key 16 mb + c, dims 32 kk + 8 g
 #pragma unroll
@@ -523,7 +529,7 @@ __global__ __launch_bounds__(512, 1) void cache_tile128_kernel(AttnArgs a) {
   auto issue = [&](int what, int j, int buf) {
     if (j < ntiles)
       ld.template load<false, NT>(what ? vbase : kbase, a.row, s.k0 + (KG * j + kg) * BN, s.k1,
-                                  lds0 + (2 * what + buf) * kTileB, rw, lane);
+                                  lds0 + (2 * what + buf) * kTileB, rw, lane, &kZeroRow);
   };
   issue(0, 0, 0);
   issue(1, 0, 0);

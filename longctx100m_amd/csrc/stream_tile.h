@@ -33,8 +33,8 @@ struct VTile<128> {
   __device__ __forceinline__ void init(int64_t stride, int lane) { ld.init(stride, 0, lane); }
   template <bool kNt = true>
   __device__ __forceinline__ void load(const uint16_t* base, int64_t stride, int row0, int nrows,
-                                       uint32_t lds, int lane) const {
-    ld.template load<false, kNt>(base, stride, row0, nrows, lds, 0, lane);
+                                       uint32_t lds, int lane, const void* filler = nullptr) const {
+    ld.template load<false, kNt>(base, stride, row0, nrows, lds, 0, lane, filler);
   }
   static __device__ __forceinline__ int tr_off(int col0, int lane) { return t128::tr_off(0, col0, lane); }
 };
@@ -49,10 +49,11 @@ struct VTile<64> {
       off[i] = (uint32_t)(r * stride * 2 + 16 * ((lane & 7) ^ swz64(r)));
     }
   }
-  // Rows at or past nrows re-read the last row (callers mask them).
+  // Rows at or past nrows re-read the last row (callers mask them), or 16 bytes
+  // at filler.
   template <bool kNt = true>
   __device__ __forceinline__ void load(const uint16_t* base, int64_t stride, int row0, int nrows,
-                                       uint32_t lds, int lane) const {
+                                       uint32_t lds, int lane, const void* filler = nullptr) const {
     if (row0 + 8 * kInst <= nrows) {
       const uint8_t* tb = reinterpret_cast<const uint8_t*>(base + (int64_t)row0 * stride);
 #pragma unroll
@@ -66,6 +67,7 @@ struct VTile<64> {
         const int r = 8 * i + (lane >> 3);
         const int row = min(row0 + r, nrows - 1);
         const uint16_t* g = base + (int64_t)row * stride + 8 * ((lane & 7) ^ swz64(r));
+        if (filler != nullptr && row0 + r >= nrows) g = static_cast<const uint16_t*>(filler);
         if constexpr (kNt) t128::dma_b128_nt(g, lds + 1024 * i);
         else t128::dma_b128(g, lds + 1024 * i);
       }

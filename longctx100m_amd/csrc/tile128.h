@@ -121,7 +121,8 @@ __device__ __forceinline__ void dma_b32(const void* g, uint32_t lds) {
 // 4 rows.  The per-lane byte offsets inside a tile and the wave's LDS offset
 // are computed once; a tile that lies fully inside the matrix is issued from
 // a uniform base pointer plus those offsets, the last (partial) tile re-reads
-// row nrows - 1 for rows past the end (finite data; callers mask those rows).
+// row nrows - 1 for rows past the end (finite data; callers mask those rows),
+// or 16 bytes at `filler` (zeros) where that is given.
 template <int ROWS, int NW>
 struct RowLoader {
   static_assert(ROWS % (4 * NW) == 0, "4 rows per wave instruction");
@@ -145,7 +146,8 @@ struct RowLoader {
   // that no other workgroup reads again.
   template <bool kTracked = false, bool kNt = false>
   __device__ __forceinline__ void load(const uint16_t* base, int64_t stride, int row0, int nrows,
-                                       uint32_t lds, int wave, int lane) const {
+                                       uint32_t lds, int wave, int lane,
+                                       const void* filler = nullptr) const {
     if (row0 + ROWS <= nrows) {
       const uint8_t* tb = reinterpret_cast<const uint8_t*>(base + (int64_t)row0 * stride);
 #pragma unroll
@@ -166,6 +168,7 @@ struct RowLoader {
         int grow = row0 + r;
         grow = grow < nrows ? grow : nrows - 1;
         const uint16_t* g = base + (int64_t)grow * stride + chunk * 8;
+        if (filler != nullptr && row0 + r >= nrows) g = static_cast<const uint16_t*>(filler);
         const uint32_t dst = lds + wave_lds + i * NW * 4 * kRowBytes;
         if constexpr (kTracked)
           __builtin_amdgcn_global_load_lds(g, (lds_void*)(uintptr_t)dst, 16, 0, 0);

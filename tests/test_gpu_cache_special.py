@@ -6,7 +6,7 @@ import pytest
 
 from oracle import cache as oc
 from tests.conftest import bf16_round
-from tests.test_gpu_cache import _check_weights, _data, _i32, _to, _tree
+from tests.test_gpu_cache import _check_attention, _check_weights, _data, _i32, _nan, _to, _tree
 
 pytestmark = pytest.mark.gpu
 
@@ -59,3 +59,51 @@ def test_rows_that_give_nothing_give_no_nan(gpu, hq, hkv, d, n, c, dtype, tree):
     assert np.isnan(got[0, 1, 40].item())
     got[0, 1, 40] = float(want[0, 1, 40])
     _check_weights(got, want, q, k, m, n * hq)
+
+
+# hq, hkv, d, past of each sequence, tokens, padding, capacity, dtype
+@pytest.mark.parametrize("hq,hkv,d,past,n,pad,c,dtype", [
+    (32, 8, 128, [130, 1, 31], 3, 0, 200, "bf16"),
+    (8, 2, 64, [65, 700, 129], 4, 1, 710, "bf16"),
+    (8, 2, 128, [1201, 33], 8, 0, 1300, "bf16"),
+    (9, 3, 64, [300, 7, 190], 9, 2, 400, "bf16"),
+    (4, 1, 64, [900], 12, 0, 530_000, "bf16"),
+    (4, 1, 128, [900, 65], 10, 2, 120_000, "bf16"),
+    (4, 2, 128, [777], 70, 4, 60_000, "bf16"),
+    (4, 1, 128, [777, 1301], 160, 9, 48_000, "bf16"),
+    (8, 2, 80, [130, 17], 9, 0, 200, "bf16"),
+    (9, 3, 64, [300, 7], 9, 2, 400, "fp32"),
+])
+def test_infinities_in_a_tile_that_the_past_ends_in(gpu, hq, hkv, d, past, n, pad, c, dtype):
+    """An infinite value in the past's last row makes its column infinite, a NaN one
+    NaN, and no other; an infinite key that all rows score -inf has no part."""
+    from longctx100m_amd import cache as kv
+
+    rng = np.random.default_rng(n + d)
+    b, used = len(past), max(past) + n
+    q, k, v = _data(rng, b, n, used, hq, hkv, d, dtype)
+    q[..., 3] = -np.abs(q[..., 3]) - 1
+    q = bf16_round(q) if dtype == "bf16" else q
+    for x in range(b):
+        if past[x] > 1:
+            k[x, past[x] - 2, :, 3] = np.inf
+    parents = _tree(rng, b, n, pad)
+    eo, em, el = oc.tree_attention(q, k, v, past, parents)
+    there = np.isfinite(em[:, 0])
+    for x in range(b):
+        v[x, past[x] - 1, :, 7], v[x, past[x] - 1, :, d - 1] = np.inf, -np.inf
+        v[x, past[x] - 1, :, 5] = np.nan
+    tk, tv = (_nan(gpu, b, c, hkv, d, dtype=gpu.bfloat16 if dtype == "bf16" else gpu.float32)
+              for _ in range(2))
+    tk[:, :used], tv[:, :used] = _to(gpu, k, dtype), _to(gpu, v, dtype)
+    for precise in ((False, True) if dtype == "bf16" and c < 1000 else (False,)):
+        o, m, l = kv.tree_attention(_to(gpu, q, dtype), tk, tv, _i32(gpu, past),
+                                    _i32(gpu, parents), precise=precise)
+        col = o.float().cpu().numpy()
+        assert (col[there][..., 7] == np.inf).all() and (col[there][..., d - 1] == -np.inf).all()
+        assert np.isnan(col[there][..., 5]).all()
+        o, want = o.clone(), eo.copy()
+        for x in (5, 7, d - 1):
+            o[..., x], want[..., x] = 0, 0
+        _check_attention((o, m, l), (want, em, el), q, k, v, dtype,
+                         dtype == "bf16" and not precise)
