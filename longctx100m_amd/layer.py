@@ -581,7 +581,8 @@ class BoundedCache:
         path = list(path)
         up = -1
         for p in path:
-            if not 0 <= p < len(self._parents) or self._parents[p] != up:
+            # (a token whose parent is not before it is padding)
+            if not up < p < len(self._parents) or self._parents[p] != up:
                 raise ValueError(f"{path} is not a chain of the tree's nodes from a root")
             up = p
         if path:

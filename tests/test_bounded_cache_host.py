@@ -1,0 +1,65 @@
+"""What layer.BoundedCache decides on the host: which trees and paths it takes
+and what a refused call leaves behind.  The kernels are replaced by recorders,
+so this runs without a GPU."""
+
+import pytest
+import torch
+
+from longctx100m_amd import layer as ly
+
+
+class Recorder:
+    """Stands for longctx100m_amd.cache: notes the calls that reach it."""
+
+    def __init__(self, real):
+        self.real, self.calls = real, []
+
+    def __getattr__(self, name):
+        if name in ("tree_depths", "MAX_TOKENS"):
+            return getattr(self.real, name)
+        return lambda *a, **kw: self.calls.append(name)
+
+
+def _bounded(monkeypatch, past=10, capacity=100, layers=2):
+    kv = Recorder(ly.kv)
+    monkeypatch.setattr(ly, "kv", kv)
+    c = object.__new__(ly.BoundedCache)
+    c.cfg = ly.ModelConfig(hidden_size=64, num_heads=4, num_key_value_heads=2,
+                           intermediate_size=64, num_layers=layers, vocab_size=50)
+    c.capacity, c.past, c.kept, c.end = capacity, past, 0, past
+    c.caches = ly.new_cache(c.cfg, capacity, "cpu", torch.float32)
+    c.layers = None
+    c.weights = [torch.zeros(1, 2, capacity) for _ in c.caches]
+    c.positions = [torch.zeros(1, 2, capacity, dtype=torch.int32) for _ in c.caches]
+    c._device = torch.device("cpu")
+    c._drafts, c._parents = [], []
+    return c, kv
+
+
+def _drafted(c, parents):
+    """As after a decode of this tree."""
+    n = len(parents)
+    c._parents = list(parents)
+    c._drafts = [(torch.zeros(1, n, 4, 16), torch.zeros(1, 4, n), torch.ones(1, 4, n))
+                 for _ in c.caches]
+
+
+@pytest.mark.parametrize("parents,path", [
+    ([-1, 2, 0], [0, 2, 1]),        # node 1 names a later node: padding
+    ([1, -1], [1, 0]),
+    ([-1, 1, 0], [0, 1]),           # node 1 names itself
+    ([-1, 3, 0, 2], [0, 2, 3, 1]),
+    ([-1, -2, 0], [1]),
+    ([-1, 0, 1], [0, 2]),
+    ([-1, 0, 1], [1]),
+    ([-1, 0], [0, -1]),
+    ([-1, 0], [0, 2]),
+])
+def test_commit_refuses_paths_through_padding(monkeypatch, parents, path):
+    c, kv = _bounded(monkeypatch)
+    _drafted(c, parents)
+    with pytest.raises(ValueError, match="chain"):
+        c.commit(path)
+    assert kv.calls == [] and (c.past, c.end) == (10, 10)
+    c.commit([parents.index(-1)])  # the tree is still there
+    assert kv.calls == ["commit", "key_weights", "key_weights"] and (c.past, c.end) == (11, 11)
