@@ -561,9 +561,10 @@ class BoundedCache:
         depths = kv.tree_depths(parents)
         if self.past + n > self.capacity:
             raise ValueError(f"{n} tokens behind {self.past} rows exceed the capacity {self.capacity}")
-        if self.end + max(depths) >= table.shape[0]:
+        at = [self.end + max(x, 0) for x in depths]
+        if max(at) >= table.shape[0]:
             raise ValueError("the RoPE table ends before the tree")
-        rows = table[self._i32(*[self.end + max(x, 0) for x in depths]).long()]
+        rows = table[self._i32(*at).long()]
         past, tree = self._i32(self.past), self._i32(*parents).view(1, n)
         self._drafts, self._parents = [], list(parents)
         x = torch.nn.functional.embedding(ids, weights["embed"])

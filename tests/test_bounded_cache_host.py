@@ -63,3 +63,13 @@ def test_commit_refuses_paths_through_padding(monkeypatch, parents, path):
     assert kv.calls == [] and (c.past, c.end) == (10, 10)
     c.commit([parents.index(-1)])  # the tree is still there
     assert kv.calls == ["commit", "key_weights", "key_weights"] and (c.past, c.end) == (11, 11)
+
+
+@pytest.mark.parametrize("parents", [[-2], [5, -2], [-1, -2], [-1, 0]])
+def test_decode_refuses_a_table_that_ends_at_the_tree(monkeypatch, parents):
+    """Padding takes a row of the table too, where its tree has no other node."""
+    c, kv = _bounded(monkeypatch, past=20)
+    table = torch.zeros(20 + max(ly.kv.tree_depths(parents) + [0]), 2, 8)
+    with pytest.raises(ValueError, match="RoPE"):
+        c.decode(torch.zeros(len(parents), dtype=torch.long), parents, {}, table)
+    assert kv.calls == [] and c.past == 20
