@@ -566,15 +566,18 @@ class BoundedCache:
             raise ValueError("the RoPE table ends before the tree")
         rows = table[self._i32(*at).long()]
         past, tree = self._i32(self.past), self._i32(*parents).view(1, n)
-        self._drafts, self._parents = [], list(parents)
+        self._drafts, self._parents = [], []  # the rows of an earlier tree go
+        drafts = []
         x = torch.nn.functional.embedding(ids, weights["embed"])
         res = None
         for lw, cache in zip(weights["layers"], self.caches):
             x, res = layer_decode_tree(x, lw, self.cfg, rows, self.past, past, tree, cache,
                                        residual=res, workspace=workspace,
-                                       observe=lambda *s: self._drafts.append(s))
+                                       observe=lambda *s: drafts.append(s))
         h = rmsnorm(x, weights["final_norm"], self.cfg.rms_norm_eps, residual=res)
-        return linear(h, weights["lm_head"])
+        logits = linear(h, weights["lm_head"])
+        self._drafts, self._parents = drafts, list(parents)  # every layer has its rows
+        return logits
 
     def commit(self, path: Sequence[int]) -> None:
         """Keeps the tree's nodes ``path``, a chain from a root down, and drops the

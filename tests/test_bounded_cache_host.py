@@ -73,3 +73,31 @@ def test_decode_refuses_a_table_that_ends_at_the_tree(monkeypatch, parents):
     with pytest.raises(ValueError, match="RoPE"):
         c.decode(torch.zeros(len(parents), dtype=torch.long), parents, {}, table)
     assert kv.calls == [] and c.past == 20
+
+
+def test_a_decode_that_fails_leaves_no_tree(monkeypatch):
+    """A tree whose rows not every layer has cannot be committed, nor the one
+    before it, whose rows are overwritten; a call that is refused leaves it."""
+    c, kv = _bounded(monkeypatch)
+    _drafted(c, [-1, 0])
+    layers = []
+
+    def one_layer(x, *a, observe=None, **kw):
+        layers.append(x)
+        if len(layers) > 1:
+            raise RuntimeError("out of memory")
+        observe(torch.zeros(1, 3, 4, 16), torch.zeros(1, 4, 3), torch.ones(1, 4, 3))
+        return x, x
+
+    monkeypatch.setattr(ly, "layer_decode_tree", one_layer)
+    ids, table = torch.zeros(3, dtype=torch.long), torch.zeros(100, 2, 8)
+    weights = {"embed": torch.zeros(50, 64), "layers": [{}, {}]}
+    with pytest.raises(ValueError, match="parent"):
+        c.decode(ids, [-1, 0], weights, table)
+    assert len(c._parents) == len(c._drafts) == 2
+    with pytest.raises(RuntimeError, match="memory"):
+        c.decode(ids, [-1, 0, 0], weights, table)
+    for path in ([0], [0, 1], [0, 2]):
+        with pytest.raises(ValueError, match="chain"):
+            c.commit(path)
+    assert kv.calls == [] and c.past == 10
