@@ -602,8 +602,12 @@ class BoundedCache:
     def evict(self, budget: int, sinks: int = 4, recent: int = 64) -> None:
         """Cuts every layer's cache to ``budget`` rows per KV head (cache.evict);
         a tree that was not committed is dropped."""
+        over = self.past > budget
+        if over and (budget <= 0 or min(sinks, recent) < 0 or sinks + recent > budget):
+            raise ValueError(f"a budget of {budget} rows must be positive and hold {sinks} sinks and "
+                             f"{recent} recent rows")
         self._drafts, self._parents = [], []
-        if self.past <= budget:
+        if not over:
             return
         lens, kept, ends = (self._i32(x) for x in (self.past, self.kept, self.end))
         ws = torch.empty(kv.evict_workspace_bytes(self.caches[0][0]), dtype=torch.uint8,

@@ -101,3 +101,24 @@ def test_a_decode_that_fails_leaves_no_tree(monkeypatch):
         with pytest.raises(ValueError, match="chain"):
             c.commit(path)
     assert kv.calls == [] and c.past == 10
+
+
+@pytest.mark.parametrize("kw", [dict(budget=0), dict(budget=-3), dict(budget=20, recent=17),
+                                dict(budget=20, sinks=-1, recent=2), dict(budget=39, recent=-1)])
+def test_evict_refuses_before_it_drops_the_tree(monkeypatch, kw):
+    c, kv = _bounded(monkeypatch, past=40)
+    _drafted(c, [-1, 0])
+    with pytest.raises(ValueError, match="budget"):
+        c.evict(**kw)
+    assert kv.calls == [] and (c.past, c.kept) == (40, 0)
+    c.commit([0, 1])
+    assert c.past == 42
+
+
+def test_evict_within_the_budget_drops_the_tree(monkeypatch):
+    c, kv = _bounded(monkeypatch, past=40)
+    _drafted(c, [-1, 0])
+    c.evict(40)
+    assert kv.calls == [] and (c.past, c.kept) == (40, 0)
+    with pytest.raises(ValueError, match="chain"):
+        c.commit([0])
