@@ -107,3 +107,30 @@ def test_infinities_in_a_tile_that_the_past_ends_in(gpu, hq, hkv, d, past, n, pa
             o[..., x], want[..., x] = 0, 0
         _check_attention((o, m, l), (want, em, el), q, k, v, dtype,
                          dtype == "bf16" and not precise)
+
+
+# hq, hkv, d, tokens, capacity: forms, each with several tiles of keys a wave
+@pytest.mark.parametrize("hq,hkv,d,n,c", [
+    (4, 1, 128, 4, 120_000), (4, 1, 128, 8, 120_000), (4, 1, 64, 8, 120_000),
+    (4, 1, 64, 16, 530_000),
+    (4, 1, 128, 10, 250_000), (4, 1, 128, 32, 130_000),   # 128 rows in two halves
+    (4, 1, 128, 64, 70_000), (4, 1, 128, 256, 70_000),    # 256 rows
+])
+def test_the_largest_probability_is_not_rounded(gpu, hq, hkv, d, n, c):
+    """Probabilities go to the matrix cores in bf16, relative to their row's largest
+    so far: where one key has nearly all of a row's weight, its value comes out
+    exactly.  Here key 133 has it, and a key of the tiles before has 2^-5 of that
+    at most and the same value; the others have less than 2^-26 together.  The
+    rounding of the small ones (2^-8 each) moves the output by 2^-13 of the value,
+    less than half a step (2^-9 at least), which is the output's rounding."""
+    from longctx100m_amd import cache as kv
+
+    gen = gpu.Generator(device="cuda").manual_seed(n + d)
+    k = gpu.full((1, c, hkv, d), -3.0, device="cuda")
+    k[:, 5], k[:, 133] = 0.625 if d == 128 else 0.5, 1.0
+    v = gpu.randn(1, c, hkv, d, generator=gen, device="cuda").bfloat16()
+    v[:, 5] = v[:, 133]
+    scale = 1 + gpu.arange(n * hq, device="cuda") % 32 / 128
+    q = scale.view(1, n, hq, 1).expand(-1, -1, -1, d)
+    out, _, _ = kv.tree_attention(q.bfloat16().contiguous(), k.bfloat16(), v, _i32(gpu, [c - n]))
+    assert gpu.equal(out, v[:, 133:134].expand(-1, n, -1, -1).repeat(1, 1, hq, 1))
