@@ -60,6 +60,14 @@ def _opt(t, shape, dtype, device: int, name: str) -> Optional[int]:
     return None if t is None else _buf(t, shape, dtype, device, name)
 
 
+def _int32(x: int, name: str) -> int:
+    """An argument of the C ABI's int32_t, which ctypes would cut to its low bits."""
+    x = int(x)
+    if not -2 ** 31 <= x < 2 ** 31:
+        raise ValueError(f"{name} is beyond 32 bits: {x}")
+    return x
+
+
 def _kv(k: torch.Tensor, v: Optional[torch.Tensor]) -> int:
     """Checks a cache; returns its device."""
     for t, name in ((k, "k"), (v, "v")):
@@ -81,6 +89,9 @@ def _kv(k: torch.Tensor, v: Optional[torch.Tensor]) -> int:
 def _describe(k: torch.Tensor, tokens: int, heads_q: int, precise: bool = False) -> _lib.Cache:
     b, c, hkv, d = k.shape
     sb, sr, sh, _ = k.stride()
+    if max(b, c, hkv, d, tokens, heads_q) >= 2 ** 31:  # as _int32
+        raise ValueError(f"{tokens} tokens of {heads_q} heads over a cache {tuple(k.shape)}: "
+                         "a size is beyond 32 bits")
     return _lib.Cache(b, tokens, c, heads_q, hkv, d, _dtype_code(k),
                       _lib.LC_FLAG_PRECISE if precise else 0,
                       # the stride of a dimension of one is never used, and may be anything
@@ -212,7 +223,8 @@ def evict(k: torch.Tensor, v: torch.Tensor, weights: torch.Tensor, lens: torch.T
     lib = _lib.load()
     desc = _describe(k, 0, 0)
     workspace = _workspace(workspace, lib.lc_cache_evict_workspace_bytes, desc, dev)
-    _call(dev, lib.lc_cache_evict, desc, int(budget), int(sinks), int(recent), *ptrs,
+    _call(dev, lib.lc_cache_evict, desc, _int32(budget, "budget"), _int32(sinks, "sinks"),
+          _int32(recent, "recent"), *ptrs,
           workspace.data_ptr(), workspace.numel() * workspace.element_size())
     return weights_out, positions_out, lens_out
 
