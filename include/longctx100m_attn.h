@@ -235,6 +235,11 @@ int lc_attn_bwd_shard_ws(const lc_attn_shape_t* shape, const lc_attn_mask_t* mas
  * token is not there (padding of a smaller tree).  A token sees the past, its
  * chain of parents and itself; NULL is the chain (each token sees those before
  * it).  Neither the kernels nor the host reads other rows of the cache.
+ * The lengths are known on the device only, so kernels and grids are chosen by
+ * the capacity: short sequences in a cache of a much larger capacity take the
+ * kernels that suit long ones.  Where the caller knows a bound on past[b] +
+ * tokens, lc_cache_attn may be given that as the capacity (the other entries
+ * have arrays of capacity entries a head).
  * Limits (LC_ERR_UNSUPPORTED beyond): batch * heads_kv 2^21, the same times
  * capacity / 64 (rounded up) 2^23, batch * heads_q 2^24, tokens * heads_q 2^30,
  * and for lc_cache_attn batch * heads_q * tokens 2^22. */
@@ -261,6 +266,10 @@ typedef struct lc_cache {
  * aligned); a second kernel merges them with the token's own chain, which it
  * computes in fp32.  What a token does not see never enters its result, not
  * even as a product with zero: infinities and NaN stay where they are.
+ * bf16 with head_dim 64 or 128: the past's probabilities are rounded to bf16 for
+ * the product with V on the bf16 matrix cores (scores, sums and the accumulated
+ * output are fp32); LC_FLAG_PRECISE keeps them in fp32, in the slower kernels
+ * that the other types and head_dims take.
  * Calls that overlap need a workspace each. */
 #define LC_CACHE_MAX_TOKENS 256
 size_t lc_cache_attn_workspace_bytes(const lc_cache_t* cache);
@@ -315,8 +324,9 @@ int lc_cache_evict(const lc_cache_t* cache, int32_t budget, int32_t sinks, int32
  * path [B, tokens] (int32, device) holds node numbers in ascending order, and
  * K and V row past[b] + path[b][j] moves to past[b] + j, for each of `layers`
  * caches of the same shape (host arrays of device pointers), no two of which, K
- * or V, may share rows.  The path ends at the first entry that is not above the one before it (>= 0 the first) or whose
- * row lies past the capacity, e.g. at a -1.  lens_out[b] = past[b] + the path's
+ * or V, may share rows.  The path ends at the first entry that is not above the
+ * one before it (>= 0 the first) or whose row lies past the capacity, e.g. at a
+ * -1.  lens_out[b] = past[b] + the path's
  * length; a sequence with past < 0 keeps it.  lens_out must not overlap past or
  * path.  Here tokens is the path's length, and heads_q is not read. */
 int lc_cache_commit(const lc_cache_t* cache, int32_t layers, void* const* ks, void* const* vs,

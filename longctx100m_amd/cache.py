@@ -16,6 +16,10 @@ one marks a batch slot without a sequence.  The new tokens' K and V are in rows
 a tree: -1 hangs token i off the past, p < i off token p, anything else is
 padding; None is a chain.
 
+Kernels are chosen by the capacity: of a cache that is far from full, pass
+``k[:, :bound]`` and ``v[:, :bound]`` to :func:`tree_attention` where a bound on the
+rows, new tokens included, is known.
+
 Everything runs on the current stream of the tensors' device, nothing
 synchronises, and lengths, trees and paths are read on the device only, so a
 captured graph can be replayed with others.  Calls that overlap need a
@@ -123,8 +127,9 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, past: torc
 
     q [B, N, Hq, D]; returns (out [B, N, Hq, D] in q's type, m, l [B, Hq, N]
     fp32), the statistics as those of ``ring_attention.fwd_shard``.  Padded
-    tokens have out = 0, m = -inf, l = 0.  ``precise`` takes bf16 inputs
-    through the fp32-math kernels."""
+    tokens have out = 0, m = -inf, l = 0.  bf16 caches of head_dim 64 or 128 round
+    the past's probabilities to bf16 for the product with v; ``precise`` takes
+    bf16 inputs through the fp32-math kernels, which do not."""
     dev = _kv(k, v)
     b, n, hq, d = _queries(q, k)
     stats = (b, hq, n)
@@ -157,7 +162,7 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, past: torch.Tensor, m: torch.T
                 precise: bool = False) -> torch.Tensor:
     """The attention weight that each cached row receives from the new tokens,
     added to ``weights``: [B, Hkv, C] fp32, summed over the query heads of a KV
-    head.
+    head.  Query rows with m = -inf or an l that is not above 0 give nothing.
 
     m, l [B, Hq, N] are the statistics of the tokens' attention
     (:func:`tree_attention`, or a forward over the same rows).  Rows < past get

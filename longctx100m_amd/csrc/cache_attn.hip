@@ -951,7 +951,9 @@ constexpr int64_t kWanted = 256;
 // in all: 16 tokens 18.9 us against 21.8 at 4,000 keys, 30.2 against 33.6 at
 // 24,000, 70 against 58 at 60,000; 26 tokens 21.0 against 25.1 at 4,000, 35.3
 // against 33.2 at 16,000; 64 tokens 21.6 against 28.3 at 500, 30.4 against 40.8 at
-// 4,000, 59 against 53 at 16,000.  Of 64: 16 tokens 26.2 against 28.0 at 60,000
+// 4,000, 59 against 53 at 16,000.  (The capacity decides: 64 tokens over 500 keys
+// take 31 us in a cache of 564 rows, 35 in a larger one, 26 over 4,000 23 and 27.)
+// Of 64: 16 tokens 26.2 against 28.0 at 60,000
 // keys, 148 against 104 at 262,000; 26 tokens 16.5 against 18.6 at 4,000, 50.7
 // against 43.0 at 60,000.
 constexpr int64_t kBlockBytes = 240 << 20;

@@ -35,8 +35,10 @@ constexpr int kPer = 16;                // rows of a thread of the long form
 constexpr int kThreads = 512;           // of a workgroup of it
 constexpr int kPart = kThreads * kPer;  // rows that it holds at a time
 constexpr int kParts = 7;               // at most: a chunk's histogram has 16-bit bins
-// Rows of the short form: at most 16,000 rows of eight heads take it 21 us where
-// the long form's launches take 34, 4,000 11 against 31.
+// Capacity of the short form: at most 16,000 rows of eight heads take it 21 us where
+// the long form's launches take 34, 4,000 11 against 31.  (The lengths are not
+// known on the host: 4,000 rows in a capacity of 32,768 take the 32 of the long
+// form, in one of 262,144 46.)
 constexpr int kShortRows = 1024 * 16;
 // Chunks (of K and V, 16 bytes each) up to which the planning workgroup of the
 // short form moves them itself, which saves a launch: 100 of 4,300 rows of 256
