@@ -486,9 +486,9 @@ __global__ __launch_bounds__(256, 2) void cache_stream_kernel(AttnArgs a) {
 //   RW = 4: 128 rows; waves 0-3 take the even tiles, 4-7 the odd ones (buffers of
 //           their own), and the halves meet in LDS: two waves a SIMD, which the
 //           products need to hide their LDS reads (32 tokens of 32/8 heads over
-//           262,000 keys 190 us, 5.6 TB/s; with four waves 202 to 210).
-// 256 rows take 300 us there (64 tokens, 915 TFLOP/s): the
-// softmax of a tile does not hide behind the products entirely.
+//           262,000 keys 209 us with the merge; with four waves 12 to 20 more).
+// 256 rows take 317 us there (64 tokens, 867 TFLOP/s, with the merge): the softmax
+// of a tile does not hide behind the products entirely.
 // Probabilities go to the products in bf16 (their sum stays fp32), relative to the
 // row's exact running maximum, so the largest so far is not rounded: a relative
 // error of 1.73e-3 at 26 tokens over 16,000 keys, 1.64e-3 of it the output's own
