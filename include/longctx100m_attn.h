@@ -282,8 +282,8 @@ int lc_cache_attn(const lc_cache_t* cache, const int32_t* past, const int32_t* p
  * same rows),
  *   w[h][j] = sum over the query rows of KV head h that see row j of
  *             exp(s - m) / l
- * (a query row with m = -inf or an l that is not above 0 gives nothing), added to what was
- * accumulated before:
+ * (a query row with m = -inf or an l that is not above 0 gives nothing), added
+ * to what was accumulated before:
  *   weights_out[b][h][j] = weights[b][h][j] + w[h][j]   (j < past[b])
  *   weights_out[b][h][j] = w[h][j]                      (a new token's own row)
  * weights (NULL: zeros) and weights_out are [B, heads_kv, capacity] fp32 and
@@ -326,8 +326,7 @@ int lc_cache_evict(const lc_cache_t* cache, int32_t budget, int32_t sinks, int32
  * caches of the same shape (host arrays of device pointers), no two of which, K
  * or V, may share rows.  The path ends at the first entry that is not above the
  * one before it (>= 0 the first) or whose row lies past the capacity, e.g. at a
- * -1.  lens_out[b] = past[b] + the path's
- * length; a sequence with past < 0 keeps it.  lens_out must not overlap past or
+ * -1.  lens_out[b] = past[b] + the path's length; a sequence with past < 0 keeps it.  lens_out must not overlap past or
  * path.  Here tokens is the path's length, and heads_q is not read. */
 int lc_cache_commit(const lc_cache_t* cache, int32_t layers, void* const* ks, void* const* vs,
                     const int32_t* past, const int32_t* path, int32_t* lens_out, void* stream);

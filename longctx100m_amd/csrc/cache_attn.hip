@@ -8,8 +8,9 @@
 //   1. a prefix kernel attends all R = N * Hq / Hkv query rows of a KV head to
 //      a split of the past, without any mask, and leaves an unnormalised
 //      partial (o, m, l) per row and split;
-//   2. cache_merge_kernel, one or four waves per row, follows the row's chain, takes its
-//      few keys with fp32 dot products and merges them with the partials.
+//   2. cache_merge_kernel, one or four waves per row, follows the row's chain,
+//      takes its few keys with fp32 dot products and merges them with the
+//      partials.
 // Neither multiplies a row of the cache by a masked probability (a tile that the
 // past ends in is filled up with rows of zeros), so what stands in a row that a
 // token does not see cannot reach it, whatever it is.

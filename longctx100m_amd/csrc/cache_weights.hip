@@ -337,10 +337,10 @@ struct QTile {
 // the start.  S = Q K^T (32 x 32 x 16): a lane has one key and 16 rows of each
 // product, whose statistics are broadcast from LDS.  Rows that give nothing are
 // zeros; a tile of such rows alone is left out, and one that has some of them
-// selects (an infinite key makes their scores NaN).  32/8
-// heads of 128 over 262,000 keys: 8 tokens 118 us (4.5 TB/s), 26 130, 64 164 (670
-// TFLOP/s), of which five are padding 178, 171 without the selection.  Non-temporal loads of K, which each workgroup reads once too, took
-// 182 there.
+// selects (an infinite key makes their scores NaN).  32/8 heads of 128 over
+// 262,000 keys: 8 tokens 118 us (4.5 TB/s), 26 130, 64 164 (670 TFLOP/s), of which
+// five are padding 178, 171 without the selection.  Non-temporal loads of K, which
+// each workgroup reads once too, took 182 there.
 constexpr int kHeldRows = 256;
 // With two 64-key tiles or fewer for each of the chip's 1,024 waves the rows
 // pass by the keys faster than the keys by more than 64 rows (32/8 heads of 128:
@@ -357,7 +357,7 @@ __global__ __launch_bounds__(256, 2) void cache_weights_rows_kernel(WeightArgs a
   __shared__ __attribute__((aligned(16))) uint64_t bits_s[kHeldRows];
   __shared__ uint64_t seen[64];
   __shared__ int par[64];
-  __shared__ int live_s, dead_s;  // one bit for each tile of 32 rows: has rows that give something, nothing
+  __shared__ int live_s, dead_s;  // a bit for each tile of 32 rows that has some that give something, nothing
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kc = lane & 31, hh = lane >> 5;
