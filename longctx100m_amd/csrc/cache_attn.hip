@@ -22,6 +22,7 @@
 // lengths loads the chip evenly.
 #include "common.h"
 #include "cache.h"
+#include "deal.h"
 #include "kernels.h"
 #include "stream_tile.h"
 #include "tile128.h"
@@ -32,8 +33,6 @@
 
 namespace lc {
 namespace {
-
-constexpr int kTile = 64;  // keys by which the past is dealt out
 
 // What the rows of a V tile behind the past hold: their probabilities are zeros,
 // but the past's last row again would make 0 * inf of an infinity in it.
@@ -56,84 +55,11 @@ struct AttnArgs {
   float sl2;
 };
 
-// Rows of the past and the tiles they take, at least one (so that every
-// sequence has a slot).
+// Rows of a sequence's past.
 __device__ __forceinline__ int past_rows(int past, int C) { return max(0, min(past, C)); }
-__device__ __forceinline__ int past_tiles(int past, int C) {
-  return max(1, (past_rows(past, C) + kTile - 1) / kTile);
-}
 
-__device__ __forceinline__ int wave_sum_i(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
-
-// ceil(t / per) for 0 <= t < 2^24, inv = 1 / per: the product is off by at most
-// one.
-__device__ __forceinline__ int slots_for(int t, int per, float inv) {
-  const int q = (int)((float)t * inv);
-  const int r = t - q * per;
-  return q + (r > 0) + (r > per);
-}
-
-// Sequences up to which the slots are dealt as tightly as possible.
-constexpr int kTightBatch = 64;
-
-// Tiles of a slot.  One sequence: its share.  Up to kTightBatch: the 64 lanes
-// try 63 sizes from an even share of all tiles to five times it, and the longest
-// sequence's tiles, with which one slot a sequence is enough; the smallest
-// size whose slots suffice is taken.  More sequences have B slots beyond the
-// even shares, and ceil(tiles / per) adds less than one each.
-__device__ __forceinline__ int slot_tiles(const int32_t* past, int B, int C, int slots) {
-  const int lane = threadIdx.x & 63;
-  if (B == 1) return (past_tiles(past[0], C) + slots - 1) / slots;
-  if (B > kTightBatch) {
-    int total = 0;
-    for (int b0 = 0; b0 < B; b0 += 64)
-      total += wave_sum_i(b0 + lane < B ? past_tiles(past[b0 + lane], C) : 0);
-    return (total + slots - B - 1) / (slots - B);
-  }
-  const int mine = lane < B ? past_tiles(past[lane], C) : 0;
-  int most = mine;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) most = max(most, __shfl_xor(most, off, 64));
-  const int even = (wave_sum_i(mine) + slots - 1) / slots;
-  const int size = lane == 63 ? most : even + (int)((int64_t)even * lane / 16);
-  const float inv = 1.f / (float)size;
-  int n = 0;
-  for (int b = 0; b < B; ++b) n += slots_for(__builtin_amdgcn_readlane(mine, b), size, inv);
-  const uint64_t fits = __ballot(n <= slots);  // the last lane's does
-  return __builtin_amdgcn_readlane(size, __ffsll((unsigned long long)fits) - 1);
-}
-
-// The key range of a workgroup.
-struct Share {
-  int b, k0, k1;  // keys k0 .. k1 - 1 of sequence b (none: k0 == k1)
-};
-// Finds the share of a slot; false: it has none.  The first workgroup leaves
-// every sequence's slots for the merge.
 __device__ __forceinline__ bool share_of(const AttnArgs& a, int slot, Share& s) {
-  const int lane = threadIdx.x & 63;
-  const int per = slot_tiles(a.past, a.B, a.C, a.slots);
-  const float inv = 1.f / (float)per;
-  int first = 0, at = -1;  // of sequence at
-  int base = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int b = b0 + lane;
-    const int n = b < a.B ? slots_for(past_tiles(a.past[b], a.C), per, inv) : 0;
-    const int end = base + wave_scan(n);
-    if (blockIdx.x == 0 && threadIdx.x < 64 && b < a.B) a.deal[b] = make_int2(end - n, n);
-    const uint64_t who = __ballot(slot < end && slot >= end - n);
-    if (who) {
-      const int x = __ffsll((unsigned long long)who) - 1;
-      at = b0 + x;
-      first = __builtin_amdgcn_readlane(end - n, x);
-    }
-    base = __builtin_amdgcn_readlane(end, 63);
-  }
-  if (at < 0) return false;
-  s.b = __builtin_amdgcn_readfirstlane(at);
-  const int rows = past_rows(a.past[s.b], a.C);
-  s.k0 = __builtin_amdgcn_readfirstlane(min((slot - first) * per * kTile, rows));
-  s.k1 = __builtin_amdgcn_readfirstlane(min(rows - s.k0, per * kTile)) + s.k0;
-  return true;
+  return share_of([&](int b) { return past_rows(a.past[b], a.C); }, a.B, a.slots, a.deal, slot, s);
 }
 
 // Where the partial of query row r of KV head hk goes.

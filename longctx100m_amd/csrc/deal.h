@@ -1,0 +1,95 @@
+// How the keys of a ragged batch are dealt over the workgroups, on the device:
+// the host fixes the number of slots (and with it a workspace), the lengths are
+// read here.  A slot holds `per` tiles of one sequence, the fewest with which the
+// slots suffice for all, so a batch of unequal lengths loads the chip evenly.
+//
+// rows(b) is the number of keys of sequence b, below 2^30.
+#pragma once
+
+#include "cache.h"
+#include "common.h"
+
+namespace lc {
+
+constexpr int kTile = 64;  // keys by which a sequence is dealt out
+
+// Tiles of a sequence, at least one (so that every sequence has a slot).
+__device__ __forceinline__ int tiles_of(int rows) { return max(1, (rows + kTile - 1) / kTile); }
+
+__device__ __forceinline__ int wave_sum_i(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
+
+// ceil(t / per) for 0 <= t < 2^24, inv = 1 / per: the product is off by at most
+// one.
+__device__ __forceinline__ int slots_for(int t, int per, float inv) {
+  const int q = (int)((float)t * inv);
+  const int r = t - q * per;
+  return q + (r > 0) + (r > per);
+}
+
+// Sequences up to which the slots are dealt as tightly as possible.
+constexpr int kTightBatch = 64;
+
+// Tiles of a slot.  One sequence: its share.  Up to kTightBatch: the 64 lanes
+// try 63 sizes from an even share of all tiles to five times it, and the longest
+// sequence's tiles, with which one slot a sequence is enough; the smallest
+// size whose slots suffice is taken.  More sequences have B slots beyond the
+// even shares, and ceil(tiles / per) adds less than one each.
+template <typename Rows>
+__device__ __forceinline__ int slot_tiles(const Rows& rows, int B, int slots) {
+  const int lane = threadIdx.x & 63;
+  if (B == 1) return (tiles_of(rows(0)) + slots - 1) / slots;
+  if (B > kTightBatch) {
+    int total = 0;
+    for (int b0 = 0; b0 < B; b0 += 64)
+      total += wave_sum_i(b0 + lane < B ? tiles_of(rows(b0 + lane)) : 0);
+    return (total + slots - B - 1) / (slots - B);
+  }
+  const int mine = lane < B ? tiles_of(rows(lane)) : 0;
+  int most = mine;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) most = max(most, __shfl_xor(most, off, 64));
+  const int even = (wave_sum_i(mine) + slots - 1) / slots;
+  const int size = lane == 63 ? most : even + (int)((int64_t)even * lane / 16);
+  const float inv = 1.f / (float)size;
+  int n = 0;
+  for (int b = 0; b < B; ++b) n += slots_for(__builtin_amdgcn_readlane(mine, b), size, inv);
+  const uint64_t fits = __ballot(n <= slots);  // the last lane's does
+  return __builtin_amdgcn_readlane(size, __ffsll((unsigned long long)fits) - 1);
+}
+
+// The key range of a workgroup.
+struct Share {
+  int b, k0, k1;  // keys k0 .. k1 - 1 of sequence b (none: k0 == k1)
+};
+// Finds the share of a slot; false: it has none.  The first workgroup leaves
+// every sequence's first slot and its slots in deal [B].
+template <typename Rows>
+__device__ __forceinline__ bool share_of(const Rows& rows, int B, int slots, int2* deal, int slot,
+                                         Share& s) {
+  const int lane = threadIdx.x & 63;
+  const int per = slot_tiles(rows, B, slots);
+  const float inv = 1.f / (float)per;
+  int first = 0, at = -1;  // of sequence at
+  int base = 0;
+  for (int b0 = 0; b0 < B; b0 += 64) {
+    const int b = b0 + lane;
+    const int n = b < B ? slots_for(tiles_of(rows(b)), per, inv) : 0;
+    const int end = base + wave_scan(n);
+    if (blockIdx.x == 0 && threadIdx.x < 64 && b < B) deal[b] = make_int2(end - n, n);
+    const uint64_t who = __ballot(slot < end && slot >= end - n);
+    if (who) {
+      const int x = __ffsll((unsigned long long)who) - 1;
+      at = b0 + x;
+      first = __builtin_amdgcn_readlane(end - n, x);
+    }
+    base = __builtin_amdgcn_readlane(end, 63);
+  }
+  if (at < 0) return false;
+  s.b = __builtin_amdgcn_readfirstlane(at);
+  const int n = rows(s.b);
+  s.k0 = __builtin_amdgcn_readfirstlane(min((slot - first) * per * kTile, n));
+  s.k1 = __builtin_amdgcn_readfirstlane(min(n - s.k0, per * kTile)) + s.k0;
+  return true;
+}
+
+}  // namespace lc
