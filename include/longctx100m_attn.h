@@ -331,6 +331,79 @@ int lc_cache_evict(const lc_cache_t* cache, int32_t budget, int32_t sinks, int32
 int lc_cache_commit(const lc_cache_t* cache, int32_t layers, void* const* ks, void* const* vs,
                     const int32_t* past, const int32_t* path, int32_t* lens_out, void* stream);
 
+/* ---- a paged cache in 8 bits -------------------------------------------------- */
+
+/* Many sequences share a pool of pages.  A page holds page_rows tokens of all KV
+ * heads: K as e4m3 codes (OCP: 448 the largest, no infinities) [pages, heads_kv,
+ * page_rows, head_dim], V as [pages, heads_kv, head_dim, page_rows], and for each
+ * page and head one scale for K and one for V [pages, heads_kv] fp32.  What a code
+ * stands for is code * scale; scales are powers of two from 2^-126 on.
+ * Row r of sequence b lies in row r % page_rows of page table[b][r / page_rows]
+ * (int32 [batch, table_width], device).  An entry outside 0 .. pages - 1, and any
+ * row from table_width * page_rows on, is no page: nothing is written there and
+ * nobody sees its rows.  Pages may stand in several tables (a shared prefix), but
+ * a page that an append writes to must be one sequence's alone.
+ * past[b] (int32, device) rows stand before the new tokens; < 0: no sequence.
+ * counts[b] (int32, device; NULL: tokens) of the call's tokens are there, the
+ * others are padding; it is clipped to [0, tokens].  New token i is row past + i. */
+typedef struct lc_paged {
+  int32_t batch;
+  int32_t tokens;   /* new tokens of a sequence, at most */
+  int32_t heads_q;
+  int32_t heads_kv;
+  int32_t head_dim; /* a multiple of 16, <= 256 */
+  int32_t dtype;    /* of q, k, v and out */
+  int32_t pages;
+  int32_t page_rows;   /* 16, 32, 64 or 128 */
+  int32_t table_width;
+  uint32_t flags;      /* 0 */
+} lc_paged_t;
+
+/* Strides, in elements, of a tensor [batch, tokens, heads, head_dim] whose rows
+ * are contiguous, e.g. columns of a fused projection. */
+typedef struct lc_rows {
+  int64_t seq_stride;
+  int64_t token_stride;
+  int64_t head_stride;
+} lc_rows_t;
+
+struct lc_rotary; /* longctx100m_layer.h */
+
+/* Appends the new tokens' K, turned to positions past + i (rotary NULL: as it is;
+ * rotary_dim must be a multiple of 16), and V to the pages, and writes their
+ * turned queries to q_out (contiguous; may be q; both NULL: no queries).  All of
+ * it is computed in fp32; K is not rounded to dtype before it is rounded to e4m3
+ * (nearest even).
+ * A page's scale for K (V) is the smallest power of two with which the magnitudes
+ * of what it has been given, finite ones, are at most 448.  The first row of a
+ * page starts it anew; when later rows raise it, the earlier rows' codes are
+ * rounded to the new scale (exact but below 2^-6 of it).  Infinities and NaN are
+ * stored as NaN.  Rows behind the new ones, padded tokens' rows and their q_out
+ * stay as they are.
+ * Reads batch, tokens, heads_q (with q), heads_kv, head_dim, dtype, pages,
+ * page_rows and table_width. */
+int lc_paged_append(const lc_paged_t* cache, const struct lc_rotary* rotary, const int32_t* table,
+                    const int32_t* past, const int32_t* counts, const void* q,
+                    const lc_rows_t* q_rows, void* q_out, const void* k, const lc_rows_t* k_rows,
+                    const void* v, const lc_rows_t* v_rows, void* k_pages, void* v_pages,
+                    float* k_scales, float* v_scales, void* stream);
+
+/* Attention of the new tokens, whose rows are in the cache already, from one token
+ * to a whole prompt: token i sees rows 0 .. past + i.  q and out are contiguous
+ * [batch, tokens, heads_q, head_dim] in dtype, m and l [batch, heads_q, tokens]
+ * fp32 (each may be NULL) as lc_attn_fwd_shard's statistics.  A token that is
+ * padding, or sees no row, has out = 0, m = -inf, l = 0.
+ * Products with q are exact in K; sums are fp32.  With bf16 queries the
+ * probabilities are rounded to bf16 for the product with V, relative to the row's
+ * running maximum; with fp32 queries they are not.  What stands in a row that a
+ * token does not see does not reach it, NaN included.
+ * The workspace belongs to the call until it has run. */
+size_t lc_paged_attn_workspace_bytes(const lc_paged_t* cache);
+int lc_paged_attn(const lc_paged_t* cache, const int32_t* table, const int32_t* past,
+                  const int32_t* counts, const void* q, const void* k_pages, const void* v_pages,
+                  const float* k_scales, const float* v_scales, void* out, float* m, float* l,
+                  void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- emulated ring (one GPU, ordered loop over KV shards in HBM) ------------ */
 
 /* Ring geometry: world equal shards of local_tokens tokens. */

@@ -74,6 +74,34 @@ int lc_rope_apply(int32_t dtype, int64_t tokens, int32_t heads, int32_t head_dim
                   const float* table, const void* src, int64_t src_token_stride, void* dst,
                   void* stream);
 
+/* Rotary positions at any positions, forward and backward: pair i of the first
+ * rotary_dim dims of a head turns by position * inv_freq[i],
+ *   (y1, y2) = factor (x1 cos - x2 sin, x2 cos + x1 sin),
+ * the pair being dims (i, i + rotary_dim / 2), or (2i, 2i + 1) if interleaved;
+ * dims from rotary_dim on stay.  Beside lc_rope_table / lc_rope_apply, whose
+ * angles are the reference's fp32 ones: here a frequency is a 64-bit fraction of
+ * a turn, so an angle is off by |position| 2^-65 turns at most, 2^-38 at 10^8. */
+typedef struct lc_rotary {
+  int32_t head_dim;      /* <= 256 */
+  int32_t rotary_dim;    /* even, <= head_dim */
+  int32_t interleaved;   /* 0 or 1 */
+  float factor;          /* of cos and sin */
+  const uint64_t* turns; /* [rotary_dim / 2], device: lc_rotary_turns' */
+} lc_rotary_t;
+
+/* inv_freq / 2 pi in units of 2^-64 turns, whole turns left out (host arrays). */
+int lc_rotary_turns(int32_t pairs, const double* inv_freq, uint64_t* turns);
+
+/* Turns x [batch, tokens, heads, head_dim] (by strides, head_dim contiguous) into
+ * out; inverse = 1: by the opposite angles, which makes it the backward pass, dx
+ * of dy.  positions [batch, tokens] (int64, device, any sign) or NULL: pos0 +
+ * token.  fp32, rounded to dtype at the end.  out may be x with the same strides,
+ * or lie apart from it. */
+int lc_rotary_apply(const lc_rotary_t* rotary, int32_t dtype, int64_t batch, int64_t tokens,
+                    int32_t heads, const int64_t* positions, int64_t pos0, int32_t inverse,
+                    const void* x, const lc_rows_t* x_rows, void* out, const lc_rows_t* out_rows,
+                    void* stream);
+
 /* SwiGLU gate (model.rs:323-327; src/longctx100m/model.py SwiGLU):
  *   out = dtype(dtype(silu(gate)) * up),  silu(g) = g / (1 + exp(-g)) in fp32.  gate and up are [rows, cols] with row
  * strides (e.g. the two halves of one fused gate/up projection); out is

@@ -120,8 +120,42 @@ class GemvFused(ctypes.Structure):
     ]
 
 
+class Paged(ctypes.Structure):
+    _fields_ = [
+        ("batch", c_int32),
+        ("tokens", c_int32),
+        ("heads_q", c_int32),
+        ("heads_kv", c_int32),
+        ("head_dim", c_int32),
+        ("dtype", c_int32),
+        ("pages", c_int32),
+        ("page_rows", c_int32),
+        ("table_width", c_int32),
+        ("flags", c_uint32),
+    ]
+
+
+class Rows(ctypes.Structure):
+    _fields_ = [
+        ("seq_stride", c_int64),
+        ("token_stride", c_int64),
+        ("head_stride", c_int64),
+    ]
+
+
+class Rotary(ctypes.Structure):
+    _fields_ = [
+        ("head_dim", c_int32),
+        ("rotary_dim", c_int32),
+        ("interleaved", c_int32),
+        ("factor", ctypes.c_float),
+        ("turns", c_void_p),
+    ]
+
+
 _vpp = POINTER(c_void_p)
 _S, _M, _R, _C = POINTER(Shape), POINTER(Mask), POINTER(RingDesc), POINTER(Cache)
+_P, _T, _W = POINTER(Paged), POINTER(Rotary), POINTER(Rows)
 
 # name -> (restype, argtypes); exactly the entry points the header declares.
 SIGNATURES = {
@@ -155,6 +189,10 @@ SIGNATURES = {
                                c_void_p]),
     "lc_cache_commit": (c_int, [_C, c_int32, _vpp, _vpp, c_void_p, c_void_p, c_void_p,
                                 c_void_p]),
+    "lc_paged_append": (c_int, [_P, _T, c_void_p, c_void_p, c_void_p, c_void_p, _W, c_void_p,
+                                c_void_p, _W, c_void_p, _W, *[c_void_p] * 5]),
+    "lc_paged_attn_workspace_bytes": (c_size_t, [_P]),
+    "lc_paged_attn": (c_int, [_P, *[c_void_p] * 12, c_size_t, c_void_p]),
     "lc_ring_fwd_workspace_bytes": (c_size_t, [_R]),
     "lc_ring_bwd_workspace_bytes": (c_size_t, [_R]),
     "lc_ring_bwd_ds_workspace_bytes": (c_size_t, [_R]),
@@ -175,6 +213,9 @@ SIGNATURES = {
     "lc_rope_table": (c_int, [POINTER(Rope), c_int64, c_int64, c_void_p, c_void_p]),
     "lc_rope_apply": (c_int, [c_int32, c_int64, c_int32, c_int32, c_void_p, c_void_p, c_int64,
                               c_void_p, c_void_p]),
+    "lc_rotary_turns": (c_int, [c_int32, c_void_p, c_void_p]),
+    "lc_rotary_apply": (c_int, [_T, c_int32, c_int64, c_int64, c_int32, c_void_p, c_int64, c_int32,
+                                c_void_p, _W, c_void_p, _W, c_void_p]),
     "lc_swiglu": (c_int, [c_int32, c_int64, c_int32, c_void_p, c_int64, c_void_p, c_int64,
                           c_void_p, c_void_p]),
     "lc_gemv": (c_int, [c_int32, c_int64, c_int32, c_void_p, c_int64, c_void_p, c_void_p,

@@ -73,6 +73,10 @@ SCRATCH_LIMITS = {
     "cache_weights": 0,
     "cache_commit_kernel": 0,
     "evict_": 0,
+    "rotary_": 0,
+    "paged_append_kernel": 0,
+    "paged_stream_kernel": 0,
+    "paged_merge_kernel": 0,
 }
 
 # "Function Name: <kernel>" starts a kernel's block; then "<field> [unit]: value".

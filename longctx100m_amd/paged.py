@@ -1,0 +1,186 @@
+"""A paged KV cache in 8 bits: appending tokens, their keys rotated on the way,
+and attention over it (lc_paged_* of include/longctx100m_attn.h).
+
+The reference keeps no cache (src/longctx100m/distributed_infer.py:185-219
+recomputes the prefill for every token); ``layer.new_cache`` and ``cache`` keep
+one sequence's, or a batch's, in rows of their own.  Here many sequences share a
+pool of pages (:class:`Pages`) and take them as they grow, at half of bf16's
+bytes: e4m3 codes, with a power-of-two scale for each page and KV head.
+
+``table`` (int32 ``[B, W]``, on the GPU) lists each sequence's pages: row r of its
+cache is row r % rows of page table[b, r // rows].  An entry outside the pool is
+no page.  ``past`` (int32 ``[B]``) counts the rows before the call's new tokens, a
+negative one marks a batch slot without a sequence; ``counts`` (int32 ``[B]``)
+tells how many of the call's N tokens a sequence has (None: all).  New token i
+is row and position past + i.  :func:`append` writes the new rows, after which
+:func:`attention` lets each token see the rows up to its own.
+
+Everything runs on the current stream of the tensors' device, nothing
+synchronises, and tables and lengths are read on the device only, so a
+captured graph can be replayed with others.  The kernels of an attention are
+chosen by the table's width: where a bound on the rows is known, pass
+``table[:, :bound].contiguous()``.  Calls that overlap need a ``workspace`` each
+(without one, a tensor of the current stream is allocated).
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from .cache import _buf, _call, _opt, _workspace
+from .ring_attention import _dtype_code
+from .rotary import Rotary, heads_of
+
+PAGE_ROWS = (16, 32, 64, 128)
+
+
+class Pages:
+    """The pool of a layer: ``k`` [pages, Hkv, rows, D] and ``v`` [pages, Hkv, D, rows]
+    in float8_e4m3fn, ``k_scale`` and ``v_scale`` [pages, Hkv] fp32.  A row's K is its
+    codes times its page's scale."""
+
+    def __init__(self, pages: int, rows: int, kv_heads: int, head_dim: int, device="cuda"):
+        def codes(*shape):
+            return torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+
+        self._set(codes(pages, kv_heads, rows, head_dim), codes(pages, kv_heads, head_dim, rows),
+                  torch.zeros(pages, kv_heads, device=device), torch.zeros(pages, kv_heads, device=device))
+
+    @classmethod
+    def of(cls, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> "Pages":
+        """A pool in tensors that are there already."""
+        p = cls.__new__(cls)
+        p._set(k, v, k_scale, v_scale)
+        return p
+
+    def _set(self, k, v, k_scale, v_scale):
+        for t in (k, v, k_scale, v_scale):
+            if not isinstance(t, torch.Tensor) or not t.is_contiguous():
+                raise ValueError("a pool is contiguous tensors")
+        if k.dim() != 4 or v.dim() != 4 or any(t.dtype is not torch.float8_e4m3fn for t in (k, v)):
+            raise ValueError("pages must be float8_e4m3fn tensors [pages, kv_heads, rows, head_dim] and "
+                             "[pages, kv_heads, head_dim, rows]")
+        n, h, rows, d = k.shape
+        if v.shape != (n, h, d, rows) or any(t.shape != (n, h) or t.dtype is not torch.float32
+                                             for t in (k_scale, v_scale)):
+            raise ValueError("v must be [pages, kv_heads, head_dim, rows], and the scales fp32 [pages, kv_heads]")
+        if any(t.device != k.device for t in (v, k_scale, v_scale)):
+            raise ValueError("a pool lives on one device")
+        if rows not in PAGE_ROWS:
+            raise ValueError(f"a page has {PAGE_ROWS} rows, got {rows}")
+        if max(n, h, d) >= 2 ** 31 or min(n, h, d) == 0:
+            raise ValueError(f"a pool of shape {tuple(k.shape)}")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.count, self.kv_heads, self.rows, self.head_dim = n, h, rows, d
+        self._ptrs = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
+
+    def device(self) -> int:
+        if not self.k.is_cuda:
+            raise ValueError("tensors must live on the GPU (device pointers are passed to HIP)")
+        return self.k.get_device()
+
+
+def _describe(pages: Pages, table: torch.Tensor, x: torch.Tensor, heads_q: int) -> _lib.Paged:
+    b, n = x.shape[:2]
+    if not isinstance(table, torch.Tensor) or table.dim() != 2:
+        raise ValueError("table must be a [batch, pages of a sequence] tensor")
+    if max(b, n, heads_q, table.shape[1]) >= 2 ** 31:
+        raise ValueError(f"{n} tokens of {heads_q} heads in {b} sequences: a size is beyond 32 bits")
+    return _lib.Paged(b, n, heads_q, pages.kv_heads, pages.head_dim, _dtype_code(x), pages.count, pages.rows,
+                      table.shape[1], 0)
+
+
+def _lengths(table, past, counts, b: int, dev: int) -> Tuple[int, int, Optional[int]]:
+    return (_buf(table, (b, table.shape[1]), torch.int32, dev, "table"),
+            _buf(past, (b,), torch.int32, dev, "past"), _opt(counts, (b,), torch.int32, dev, "counts"))
+
+
+def _rows(t, like: torch.Tensor, heads: int, d: int, dev: int, name: str) -> _lib.Rows:
+    if not isinstance(t, torch.Tensor) or t.dim() != 4 or t.dtype is not like.dtype or \
+            t.get_device() != dev or t.shape != (*like.shape[:2], heads, d):
+        raise ValueError(f"{name} must be a [batch, tokens, {heads}, {d}] tensor of one type on cuda:{dev}")
+    return heads_of(t, name)
+
+
+def append(pages: Pages, table: torch.Tensor, past: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
+           counts: Optional[torch.Tensor] = None, rotary: Optional[Rotary] = None,
+           q: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Appends the new tokens' k and v [B, N, Hkv, D] (bf16 or fp32, any strides with
+    contiguous D, e.g. columns of a fused projection) to the pages, k rotated to
+    positions past + i by ``rotary``.  With ``q`` [B, N, Hq, D] the tokens' queries are
+    rotated too and returned (``q_out``, contiguous, may be q; padded tokens' rows
+    in it are left alone, and are not written in one made here).
+
+    The pages that new rows lie in must be their sequence's alone.  Their scales
+    rise as needed, which rounds codes of earlier rows in them again: to the
+    same value, but for values below 2^-6 of the scale.  Infinities and NaN are
+    stored as NaN."""
+    dev = pages.device()
+    if not isinstance(k, torch.Tensor) or k.dim() != 4:
+        raise ValueError("k must be a [batch, tokens, heads, head_dim] tensor")
+    d, hkv = pages.head_dim, pages.kv_heads
+    ks, vs = _rows(k, k, hkv, d, dev, "k"), _rows(v, k, hkv, d, dev, "v")
+    hq, qs = 0, None
+    if q is not None:
+        if not isinstance(q, torch.Tensor) or q.dim() != 4:
+            raise ValueError("q must be a [batch, tokens, heads, head_dim] tensor")
+        hq = q.shape[2]
+        qs = _rows(q, k, hq, d, dev, "q")
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
+        _buf(q_out, q.shape, q.dtype, dev, "q_out")
+    elif q_out is not None:
+        raise ValueError("q_out comes with q")
+    desc = _describe(pages, table, k, hq)
+    if desc.batch == 0 or desc.tokens == 0:
+        return q_out
+    _call(dev, _lib.load().lc_paged_append, desc, rotary.on(dev) if rotary is not None else None,
+          *_lengths(table, past, counts, desc.batch, dev), q.data_ptr() if q is not None else None, qs,
+          q_out.data_ptr() if q is not None else None, k.data_ptr(), ks, v.data_ptr(), vs, *pages._ptrs)
+    return q_out
+
+
+def _queries(q, pages: Pages, dev: int) -> None:
+    if not isinstance(q, torch.Tensor) or q.dim() != 4 or not q.is_contiguous() or q.get_device() != dev:
+        raise ValueError(f"q must be a contiguous [batch, tokens, heads, head_dim] tensor on cuda:{dev}")
+    if q.shape[3] != pages.head_dim:
+        raise ValueError("q and the pages must agree in head_dim")
+
+
+def attention_workspace_bytes(q: torch.Tensor, pages: Pages, table: torch.Tensor) -> int:
+    """Workspace of :func:`attention` for queries, pools and tables of these shapes."""
+    _queries(q, pages, pages.device())
+    return int(_lib.load().lc_paged_attn_workspace_bytes(_describe(pages, table, q, q.shape[2])))
+
+
+def attention(q: torch.Tensor, pages: Pages, table: torch.Tensor, past: torch.Tensor, *,
+              counts: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+              m: Optional[torch.Tensor] = None, l: Optional[torch.Tensor] = None,
+              workspace: Optional[torch.Tensor] = None):
+    """Attention of N new tokens of each sequence, appended before, over the rows up
+    to their own: one token, drafts, or a whole prompt.
+
+    q [B, N, Hq, D] (bf16 or fp32); returns (out [B, N, Hq, D] in q's type, m, l
+    [B, Hq, N] fp32), the statistics as those of ``ring_attention.fwd_shard``.
+    Padded tokens, and those that see no row, have out = 0, m = -inf, l = 0.
+    bf16 queries round the probabilities to bf16 for the product with v, fp32
+    ones do not."""
+    dev = pages.device()
+    _queries(q, pages, dev)
+    b, n, hq, _ = q.shape
+    stats = (b, hq, n)
+    out = torch.empty_like(q) if out is None else out
+    m = torch.empty(stats, dtype=torch.float32, device=dev) if m is None else m
+    l = torch.empty(stats, dtype=torch.float32, device=dev) if l is None else l
+    ptrs = (q.data_ptr(), *pages._ptrs, _buf(out, q.shape, q.dtype, dev, "out"),
+            _buf(m, stats, torch.float32, dev, "m"), _buf(l, stats, torch.float32, dev, "l"))
+    desc = _describe(pages, table, q, hq)
+    if b == 0 or n == 0:
+        return out, m, l
+    lib = _lib.load()
+    workspace = _workspace(workspace, lib.lc_paged_attn_workspace_bytes, desc, dev)
+    _call(dev, lib.lc_paged_attn, desc, *_lengths(table, past, counts, b, dev), *ptrs, workspace.data_ptr(),
+          workspace.numel() * workspace.element_size())
+    return out, m, l
