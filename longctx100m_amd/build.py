@@ -76,6 +76,7 @@ SCRATCH_LIMITS = {
     "rotary_": 0,
     "paged_append_kernel": 0,
     "paged_stream_kernel": 0,
+    "paged_tile_kernel": 0,
     "paged_merge_kernel": 0,
 }
 

@@ -33,11 +33,13 @@ constexpr int kTightBatch = 64;
 // try 63 sizes from an even share of all tiles to five times it, and the longest
 // sequence's tiles, with which one slot a sequence is enough; the smallest
 // size whose slots suffice is taken.  More sequences have B slots beyond the
-// even shares, and ceil(tiles / per) adds less than one each.
+// even shares, and ceil(tiles / per) adds less than one each.  As many slots as
+// sequences: a slot is a whole sequence.
 template <typename Rows>
 __device__ __forceinline__ int slot_tiles(const Rows& rows, int B, int slots) {
   const int lane = threadIdx.x & 63;
   if (B == 1) return (tiles_of(rows(0)) + slots - 1) / slots;
+  if (slots == B) return 1 << 24;
   if (B > kTightBatch) {
     int total = 0;
     for (int b0 = 0; b0 < B; b0 += 64)

@@ -48,6 +48,7 @@ struct AttnArgs {
   int group, R;
   int slots, units;  // units: workgroups of a slot
   int shift;         // log2 of a page's rows
+  bool direct;       // a slot is a whole sequence: results in place of partials
   float sl2;
 };
 
@@ -96,6 +97,85 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
 // The lowest n bytes of a word (n may be out of 0 .. 4).
 __device__ __forceinline__ uint32_t low_bytes(int n) { return n >= 4 ? ~0u : n <= 0 ? 0u : (1u << 8 * n) - 1u; }
 
+// Values in a tile that not every row sees wholly go to the products without what
+// no row sees (`left` of 16 keys are seen) and without NaN, which times a masked
+// probability, a zero, would be NaN.  True: there was some, which the rows that
+// see it get by patch_nan.
+__device__ __forceinline__ bool clean_values(uint4& w, int left) {
+  uint32_t x[4] = {w.x, w.y, w.z, w.w}, any = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[i] &= low_bytes(left - 4 * i);
+    const uint32_t n = nan_bytes(x[i]);
+    x[i] &= ~((n >> 7) * 0xffu);
+    any |= n;
+  }
+  w = make_uint4(x[0], x[1], x[2], x[3]);
+  return any != 0;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_vec4(T* p, const f32x4& r) {
+  if constexpr (sizeof(T) == 4) store4(p, nullptr, r);
+  else store4(nullptr, p, r);
+}
+
+// 1 / l for a row's sum: 0 for a row that saw nothing, NaN for one that saw NaN.
+__device__ __forceinline__ float inverse_sum(float l) { return l > 0.f ? 1.f / l : l; }
+
+// The statistics of query row r (token r / group) of sequence b and KV head hk:
+// its maximum in log2 units, and its sum.
+__device__ __forceinline__ void store_stats(const AttnArgs& a, int b, int hk, int r, float top, float l) {
+  const int64_t si = ((int64_t)b * a.p.Hq + hk * a.group + r % a.group) * a.p.N + r / a.group;
+  if (a.m) a.m[si] = top == -INFINITY ? top : top * kLn2;
+  if (a.l) a.l[si] = l;
+}
+
+// A run of 16 tiles (64 groups of 16 keys) of a walk, lane x with group x: its
+// page (-1: none, or no key below `end`) and the page's scales.  The next run's
+// are on their way during this one, the scales half a run after the pages that
+// they follow from.
+struct PageRun {
+  int page, next;
+  float ks, vs, nks, nvs;
+
+  __device__ __forceinline__ void look(const AttnArgs& a, const int32_t* table, int t, int end) {
+    const int64_t key = 64 * (int64_t)t + 16 * (threadIdx.x & 63);
+    next = -1;
+    if (key < end) next = page_of(table, a.p.width, a.p.pool.pages, key >> a.shift);
+  }
+  __device__ __forceinline__ void scales(const AttnArgs& a, int hk) {
+    nks = nvs = 1.f;  // (of no page: finite, its values are taken as zeros)
+    if (next >= 0) {
+      const int64_t u = (int64_t)next * a.p.pool.Hkv + hk;
+      nks = a.p.pool.ks[u];
+      nvs = a.p.pool.vs[u];
+    }
+  }
+  __device__ __forceinline__ void turn() {
+    page = next;
+    ks = nks;
+    vs = nvs;
+  }
+};
+
+// Calls put(n) for those of a row's dims dim(0) .. dim(N - 1) in which a value of the
+// keys key0 .. key1 - 1 is NaN.
+template <int N, typename Dim, typename Put>
+__device__ __forceinline__ void patch_nan(const AttnArgs& a, const int32_t* table, int hk, int key0, int key1,
+                                          const Dim& dim, const Put& put) {
+  const Pool& pool = a.p.pool;
+#pragma unroll 1
+  for (int key = key0; key < key1; ++key) {
+    const int page = page_of(table, a.p.width, pool.pages, key >> a.shift);
+    if (page < 0) continue;
+    const uint8_t* v = pool.v + ((((int64_t)page * pool.Hkv + hk) * pool.D) << a.shift) + (key & ((1 << a.shift) - 1));
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      if (dim(n) < pool.D && (v[(int64_t)dim(n) << a.shift] & 0x7f) == 0x7f) put(n);
+  }
+}
+
 // ------------------------------------------------------- a few query rows --
 
 // Every wave holds all of the workgroup's 16 * NB rows and walks a run of the
@@ -130,6 +210,8 @@ __global__ __launch_bounds__(256, DP * PARTS > 192 ? 1 : 2) void paged_stream_ke
   const int all = last >= first && k1 > s.k0 ? (k1 - s.k0 + 63) / 64 : 0;
   const int per = (all + W - 1) / W;
   const int t0 = s.k0 / 64 + min(wave * per, all), t1 = s.k0 / 64 + min((wave + 1) * per, all);
+  const int clear = past + first + 1;  // keys that all rows see
+  bool strange = false;                // NaN among the values of tiles beyond
 
   // Rows of this lane: c of each 16; the keys they see.
   bf16x8 q[PARTS][NB][2 * KJ];
@@ -156,21 +238,11 @@ __global__ __launch_bounds__(256, DP * PARTS > 192 ? 1 : 2) void paged_stream_ke
     }
   }
 
-  // The pages of the next 16 tiles: lane x has that of keys 16 x .. 16 x + 15 of
-  // them, the page's two scales, and the row in it.
-  int pages = -1;
-  float kscale = 0.f, vscale = 0.f;
-  auto look = [&](int t) {
-    const int64_t key = 64 * (int64_t)t + 16 * lane;
-    pages = -1;
-    kscale = vscale = 1.f;  // (of no page: finite, its values are taken as zeros)
-    if (key < k1) pages = page_of(table, a.p.width, pool.pages, key >> a.shift);
-    if (pages >= 0) {
-      const int64_t u = (int64_t)pages * pool.Hkv + hk;
-      kscale = pool.ks[u];
-      vscale = pool.vs[u];
-    }
-  };
+  PageRun run;
+  if (t0 < t1) {
+    run.look(a, table, t0, k1);
+    run.scales(a, hk);
+  }
   const int64_t head_bytes = (int64_t)D << a.shift;
   uint4 kr[4][KJ], vr[DB];
   auto base = [&](const uint8_t* p, int page) {
@@ -179,7 +251,7 @@ __global__ __launch_bounds__(256, DP * PARTS > 192 ? 1 : 2) void paged_stream_ke
   auto kload = [&](int t) {
     const int x = 4 * (t - t0 & 15) + (c >> 2);
     const int row = (64 * t + 16 * (c >> 2)) & ((1 << a.shift) - 1);
-    const uint8_t* p = base(pool.k, __shfl(pages, x, 64)) + (row + (c & 3)) * D;
+    const uint8_t* p = base(pool.k, __shfl(run.page, x, 64)) + (row + (c & 3)) * D;
 #pragma unroll
     for (int mb = 0; mb < 4; ++mb)
 #pragma unroll
@@ -191,7 +263,7 @@ __global__ __launch_bounds__(256, DP * PARTS > 192 ? 1 : 2) void paged_stream_ke
   auto vload = [&](int t) {
     const int x = 4 * (t - t0 & 15) + g;
     const int row = (64 * t + 16 * g) & ((1 << a.shift) - 1);
-    const uint8_t* p = base(pool.v, __shfl(pages, x, 64)) + ((int64_t)c << a.shift) + row;
+    const uint8_t* p = base(pool.v, __shfl(run.page, x, 64)) + ((int64_t)c << a.shift) + row;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
       vr[db] = *reinterpret_cast<const uint4*>(p + ((int64_t)(EXACT || 16 * db < D ? 16 * db : 0) << a.shift));
@@ -207,16 +279,17 @@ __global__ __launch_bounds__(256, DP * PARTS > 192 ? 1 : 2) void paged_stream_ke
     lsum[nb] = 0.f;
   }
 
+  if (t0 < t1) {
+    run.turn();
+    kload(t0);
+    vload(t0);
+    run.look(a, table, t0 + 16, k1);
+  }
   for (int t = t0; t < t1; ++t) {
-    if ((t - t0 & 15) == 0) {
-      look(t);
-      kload(t);
-      vload(t);
-    }
     const int x = 4 * (t - t0 & 15);
-    const float ks = __shfl(kscale, x + (c >> 2), 64);  // of the lane's K
-    const float vs = __shfl(vscale, x + g, 64);         // of its V
-    const int page = __shfl(pages, x + g, 64);
+    const float ks = __shfl(run.ks, x + (c >> 2), 64);  // of the lane's K
+    const float vs = __shfl(run.vs, x + g, 64);         // of its V
+    const int page = __shfl(run.page, x + g, 64);
     f32x4 sc[NB][4];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
@@ -235,23 +308,30 @@ __global__ __launch_bounds__(256, DP * PARTS > 192 ? 1 : 2) void paged_stream_ke
             sc[nb][mb] = mfma16x16x32(k1, q[p][nb][2 * j + 1], sc[nb][mb]);
           }
       }
-    const bool more = t + 1 < t1 && (t + 1 - t0 & 15) != 0;
-    if (more) kload(t + 1);
+    const bool more = t + 1 < t1;
+    if (more) {
+      const int step = t + 1 - t0 & 15;
+      if (step == 0) {
+        run.turn();
+        run.look(a, table, t + 17, k1);
+      } else if (step == 8) {
+        run.scales(a, hk);
+      }
+      kload(t + 1);
+    }
 
     // A tile that not every row sees wholly, or with a page that there is not.
-    const bool edge = 64 * (t + 1) > past + 1 || __any(page < 0);
-    bool strange = false;  // NaN among the values of such a tile
-    if (edge) {
+    const bool edge = 64 * (t + 1) > clear;
+    if (edge || __any(page < 0)) {
       const int left = page < 0 ? 0 : k1 - (64 * t + 16 * g);  // values that some row sees
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
-        vr[db].x &= low_bytes(left);
-        vr[db].y &= low_bytes(left - 4);
-        vr[db].z &= low_bytes(left - 8);
-        vr[db].w &= low_bytes(left - 12);
-        strange = strange || (nan_bytes(vr[db].x) | nan_bytes(vr[db].y) | nan_bytes(vr[db].z) | nan_bytes(vr[db].w));
+        if (edge) {
+          strange |= clean_values(vr[db], left);
+        } else if (left <= 0) {
+          vr[db] = make_uint4(0u, 0u, 0u, 0u);
+        }
       }
-      strange = __any(strange);
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         const int see = page < 0 ? 0 : lim[nb] - (64 * t + 16 * g);
@@ -294,23 +374,7 @@ __global__ __launch_bounds__(256, DP * PARTS > 192 ? 1 : 2) void paged_stream_ke
       for (int nb = 0; nb < NB; ++nb) split8<PARTS>(sc[nb][2 * k2], sc[nb][2 * k2 + 1], pb[nb]);
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
-        uint32_t w0 = k2 ? vr[db].z : vr[db].x, w1 = k2 ? vr[db].w : vr[db].y;
-        if (strange) {
-          // A NaN must reach the rows that see it and no other: counted by itself.
-          const uint32_t n0 = nan_bytes(w0), n1 = nan_bytes(w1);
-          const uint32_t f0 = (n0 >> 7) * 0xffu, f1 = (n1 >> 7) * 0xffu;
-          const bf16x8 is = bf16_of(f0 & 0x38383838u, f1 & 0x38383838u, 1.f);  // 1 where NaN
-          w0 &= ~f0;
-          w1 &= ~f1;
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            const f32x4 n = mfma16x16x32(is, pb[nb][0], f32x4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (n[i] > 0.f) o[nb][db][i] = NAN;
-          }
-        }
-        const bf16x8 v = bf16_of(w0, w1, vs);
+        const bf16x8 v = bf16_of(k2 ? vr[db].z : vr[db].x, k2 ? vr[db].w : vr[db].y, vs);
 #pragma unroll
         for (int p = PARTS - 1; p >= 0; --p)
 #pragma unroll
@@ -319,6 +383,13 @@ __global__ __launch_bounds__(256, DP * PARTS > 192 ? 1 : 2) void paged_stream_ke
     }
     if (more) vload(t + 1);
   }
+
+  if (__any(strange))
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+      patch_nan<4 * DB>(
+          a, table, hk, max(64 * t0, clear & ~63), min(64 * t1, lim[nb]),
+          [&](int n) { return 16 * (n >> 2) + 4 * g + (n & 3); }, [&](int n) { o[nb][n >> 2][n & 3] = NAN; });
 
   // The waves' partials, brought to each row's maximum, meet in LDS.
 #pragma unroll
@@ -352,19 +423,339 @@ __global__ __launch_bounds__(256, DP * PARTS > 192 ? 1 : 2) void paged_stream_ke
       L += lsm[w][rr];
       M = fmaxf(M, msm[w][rr]);
     }
-    const int64_t pr = partial_row(a, r, hk, slot);
-    *reinterpret_cast<f32x4*>(a.po + pr * D + d) = acc;
-    if (d == 0) a.ps[pr] = make_float2(M, L);
+    if (a.direct) {
+      const int64_t qi = ((int64_t)s.b * a.p.N + r / a.group) * a.p.Hq + hk * a.group + r % a.group;
+      const bool there = r / a.group < count;
+      store_vec4(static_cast<T*>(a.out) + qi * D + d, there ? acc * inverse_sum(L) : f32x4{0.f, 0.f, 0.f, 0.f});
+      if (d == 0) store_stats(a, s.b, hk, r, there ? M : -INFINITY, there ? L : 0.f);
+    } else {
+      const int64_t pr = partial_row(a, r, hk, slot);
+      *reinterpret_cast<f32x4*>(a.po + pr * D + d) = acc;
+      if (d == 0) a.ps[pr] = make_float2(M, L);
+    }
+  }
+}
+
+// ------------------------------------------------------ many query rows --
+
+// Bound by the products and the softmax beside them.  Eight waves of 32 rows share
+// 64-key tiles of K and V^T, which the threads read from the pages as codes, 16
+// bytes at a time, one tile ahead, and write to LDS as bf16: converted once for
+// 256 rows.  Iteration j issues the products of S^T for tile j + 1 and beside
+// them, on the VALU, the softmax of tile j, then O^T += V_j^T P_j^T; K runs one tile
+// ahead of V, two buffers each, one barrier per tile.
+// v_mfma_f32_32x32x16_bf16 (common.h): a lane's scores are those of row l % 32 with
+// keys 8 (v / 4) + 4 h + v % 4, h = l / 32.  V^T rows are kept with each 16 keys in
+// the order 0-3, 8-11, 4-7, 12-15, so that the eight of a lane half are one 16-byte
+// read, and P^T needs no shuffle.
+// Chunks of 16 bytes of an LDS row of 128 bytes are XOR-swizzled by (row / 2) % 8, for
+// reads without bank conflicts (tile128.h has the lane groups of a ds_read_b128).
+template <int D>
+__global__ __launch_bounds__(512, 1) void paged_tile_kernel(AttnArgs a) {
+  constexpr int BN = 64, RW = 8, KT = D / 16, DB = D / 32;  // products of S over the dims; 32-dim blocks
+  constexpr int kTileB = BN * D * 2;
+  constexpr int kStageK = 4 * D;  // threads that stage K: all 512, or (D = 64) the first half
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * kTileB];
+  __shared__ uint32_t nan_s[RW];  // whether a wave has met NaN in V
+  uint8_t* const kbuf = smem;
+  uint8_t* const vbuf = smem + 2 * kTileB;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kc = lane & 31, hh = lane >> 5;
+  const int slot = blockIdx.x / a.units;
+  const int unit = blockIdx.x - slot * a.units;
+  const Pool& pool = a.p.pool;
+  const int hk = unit % pool.Hkv;
+  const int rb = a.units / pool.Hkv - 1 - unit / pool.Hkv;  // the longest walks first
+  Share s;
+  if (!share_of([&](int b) { return keys_of(a, b); }, a.p.B, a.slots, a.deal, slot, s)) return;
+
+  const int past = a.p.past[s.b];
+  const int count = new_tokens(a.p.counts, a.p.N, s.b, past);
+  const int32_t* table = a.p.table + (int64_t)s.b * a.p.width;
+  constexpr int kRows = 32 * RW;
+  // The keys of the workgroup's rows, and those of the wave's.
+  const int first = rb * kRows / a.group, last = min((rb * kRows + kRows - 1) / a.group, count - 1);
+  const int k1 = last >= first ? min(s.k1, past + last + 1) : s.k0;
+  const int t0 = s.k0 / BN;
+  const int ntiles = opaque(k1 > s.k0 ? (k1 - s.k0 + BN - 1) / BN : 0);
+  const int wfirst = (rb * kRows + 32 * wave) / a.group;
+  const int wlast = min((rb * kRows + 32 * wave + 31) / a.group, count - 1);
+  const int wk1 = wlast >= wfirst ? min(k1, past + wlast + 1) : s.k0;
+  const int nt_w = opaque(wk1 > s.k0 ? (wk1 - s.k0 + BN - 1) / BN : 0);
+  const int clear = past + wfirst + 1;     // keys that every row of the wave sees
+  const int all_clear = past + first + 1;  // and every row of the workgroup
+  bool strange = false;                    // NaN among the values of tiles beyond
+
+  const int r = rb * kRows + 32 * wave + kc, i = r / a.group;
+  const bool ok = r < a.R && i < count;
+  const int lim = ok ? past + i + 1 : 0;
+
+  // Staging: a thread's piece of K is 16 dims of a row, of V 16 keys of a dim.
+  const bool do_k = D == 128 || tid < kStageK, do_v = D == 128 || tid >= kStageK;
+  const int krow = tid / (D / 16), kch = tid % (D / 16);
+  const int vdim = (D == 128 ? tid : tid - kStageK) >> 2, vg = tid & 3;
+  const int kg = __builtin_amdgcn_readfirstlane(krow >> 4) & 3;  // (uniform in the wave)
+  const int64_t head_bytes = (int64_t)D << a.shift;
+  const int page_mask = (1 << a.shift) - 1;
+  const int kdst = krow * 2 * D + 16 * ((2 * kch) ^ (D == 128 ? t128::swz(krow) : (krow >> 1) & 7));
+  const int vdst = vdim * 128 + 16 * ((2 * vg) ^ ((vdim >> 1) & 7));
+  PageRun run;
+  uint4 kw, vw;
+  float kscale, vscale;
+  uint32_t gone = 0, gone_next = 0;  // of V's last two tiles, bit g: keys 16 g .. have no page
+  // Tile j of K is read before that of V, and turns to a new run one tile earlier.
+  auto kload = [&](int j) {
+    if (j >= ntiles) return;
+    if ((j & 15) == 8) run.scales(a, hk);
+    const bool ahead = (j & 15) == 0;
+    const int x = 4 * (j & 15) + kg;
+    const int page = max(__builtin_amdgcn_readlane(ahead ? run.next : run.page, x), 0);
+    kscale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ahead ? run.nks : run.ks), x));
+    if (do_k) {
+      const int row = (BN * (t0 + j) + 16 * kg & page_mask) + (krow & 15);
+      kw = *reinterpret_cast<const uint4*>(pool.k + ((int64_t)page * pool.Hkv + hk) * head_bytes + row * D + 16 * kch);
+    }
+  };
+  auto vload = [&](int j) {
+    gone = gone_next;
+    if (j >= ntiles) return;
+    if ((j & 15) == 0) {
+      run.turn();
+      run.look(a, table, t0 + j + 16, k1);
+    }
+    const int x = 4 * (j & 15);
+    gone_next = (uint32_t)(__ballot(run.page < 0) >> x) & 15u;
+    vscale = __shfl(run.vs, x + vg, 64);
+    const int page = max(__shfl(run.page, x + vg, 64), 0);
+    if (do_v) {
+      const int row = BN * (t0 + j) + 16 * vg & page_mask;
+      vw = *reinterpret_cast<const uint4*>(pool.v + ((int64_t)page * pool.Hkv + hk) * head_bytes +
+                                           ((int64_t)vdim << a.shift) + row);
+    }
+  };
+  auto kwrite = [&](int j, auto parity) {  // parity: j % 2
+    if (j >= ntiles || !do_k) return;
+    uint8_t* const b = kbuf + decltype(parity)::value * kTileB;
+    *reinterpret_cast<bf16x8*>(b + kdst) = bf16_of(kw.x, kw.y, kscale);
+    *reinterpret_cast<bf16x8*>(b + (kdst ^ 16)) = bf16_of(kw.z, kw.w, kscale);
+  };
+  auto vwrite = [&](int j, auto parity) {
+    constexpr int P = decltype(parity)::value;
+    if (j >= ntiles) return;
+    if (!do_v) return;
+    const bool none = gone_next >> vg & 1;
+    if (BN * (t0 + j) + BN > all_clear)
+      strange |= clean_values(vw, none ? 0 : k1 - (BN * (t0 + j) + 16 * vg));
+    else if (none)
+      vw = make_uint4(0u, 0u, 0u, 0u);
+    *reinterpret_cast<bf16x8*>(vbuf + P * kTileB + vdst) = bf16_of(vw.x, vw.z, vscale);
+    *reinterpret_cast<bf16x8*>(vbuf + P * kTileB + (vdst ^ 16)) = bf16_of(vw.y, vw.w, vscale);
+  };
+  constexpr std::integral_constant<int, 0> even{};
+  constexpr std::integral_constant<int, 1> odd{};
+  if (ntiles > 0) {
+    run.look(a, table, t0, k1);
+    run.scales(a, hk);
+    kload(0);
+    kwrite(0, even);
+    vload(0);
+    vwrite(0, even);
+    kload(1);
+    kwrite(1, odd);
+    vload(1);
+    kload(2);
+  }
+
+  bf16x8 qreg[KT];  // lane: row r, dims 16 t + 8 hh .. + 7
+  {
+    const int64_t qi = ((int64_t)s.b * a.p.N + (ok ? i : 0)) * a.p.Hq + hk * a.group + r % a.group;
+    const uint16_t* qrow = static_cast<const uint16_t*>(a.q) + qi * D;
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      qreg[t] = *reinterpret_cast<const bf16x8*>(qrow + 16 * t + 8 * hh);
+      if (!ok) qreg[t] = bf16x8{};
+    }
+  }
+  const int koff = opaque(D == 128 ? t128::row_chunk_off(kc, hh) : kc * 128 + 16 * (hh ^ ((kc >> 1) & 7)));
+  const int voff = opaque(kc * 128 + 16 * (hh ^ ((kc >> 1) & 7)));
+  auto kread = [&](const uint8_t* kt, int n) {  // S step n: t = n / 2, mb = n % 2
+    return *reinterpret_cast<const bf16x8*>(kt + (koff ^ 32 * (n >> 1)) + (n & 1) * 32 * 2 * D);
+  };
+  auto vread = [&](const uint8_t* vt, int n) {  // PV step n: u = n / DB, dims 32 (n % DB) ..
+    return *reinterpret_cast<const bf16x8*>(vt + (voff ^ 32 * (n / DB)) + (n % DB) * 32 * 128);
+  };
+
+  f32x16 o[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) o[d] = f32x16{};
+  float mrun = -INFINITY;  // log2 units, shared by the lanes l, l ^ 32
+  float lsum = 0.f;        // lane-partial, relative to mrun
+
+  auto scores_only = [&](const uint8_t* kt, f32x16 (&x)[2]) {
+    bf16x8 A[2] = {kread(kt, 0), kread(kt, 1)};
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < 2 * KT; ++n) {
+      x[n & 1] = mfma32x32x16(A[n & 1], qreg[n >> 1], n < 2 ? f32x16{} : x[n & 1]);
+      if (n + 2 < 2 * KT) A[n & 1] = kread(kt, n + 2);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // Tile j: klim, the lane's keys of it (less 4 hh); gone, bit g: no page for its
+  // keys 16 g .. (both read if MASKED only).
+  auto iteration = [&](auto masked_tag, auto next_tag, const uint8_t* kt, const uint8_t* vt, f32x16 (&sc)[2],
+                       f32x16 (&sn)[2], int klim, uint32_t gone) {
+    constexpr bool MASKED = decltype(masked_tag)::value;
+    constexpr bool NEXT = decltype(next_tag)::value;
+    constexpr int S = 16;  // steps; 2 KT of them with a product
+    constexpr int kEvery = S / (2 * KT);
+    bf16x8 A[2], B[2], pb[4];
+    if constexpr (NEXT) {
+      A[0] = kread(kt, 0);
+      A[1] = kread(kt, 1);
+    }
+    float pmax = -INFINITY, muse = 0.f;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int st = 0; st < S; ++st) {
+      if constexpr (NEXT)
+        if (st % kEvery == 0) {
+          const int n = st / kEvery;
+          sn[n & 1] = mfma32x32x16(A[n & 1], qreg[n >> 1], n < 2 ? f32x16{} : sn[n & 1]);
+          if (n + 2 < 2 * KT) A[n & 1] = kread(kt, n + 2);
+        }
+      if (st < 4) {  // the maximum, 8 scores per step
+#pragma unroll
+        for (int e = 8 * st; e < 8 * st + 8; ++e) {
+          const int mb = e >> 4, v = e & 15;
+          if constexpr (MASKED)
+            if (32 * mb + 8 * (v >> 2) + (v & 3) >= klim || (gone >> (2 * mb + (v >> 3)) & 1)) sc[mb][v] = -INFINITY;
+          pmax = fmaxf(pmax, sc[mb][v]);
+        }
+      }
+      if (st == 7) {
+        const float mx = xor32_max(pmax) * a.sl2;
+        if (__any(mx > mrun)) {
+          const float alpha = mx > mrun ? fast_exp2(mrun - mx) : 1.f;  // mrun = -inf: 0
+          mrun = fmaxf(mrun, mx);
+          lsum *= alpha;
+#pragma unroll
+          for (int d = 0; d < DB; ++d) o[d] *= alpha;
+        }
+        muse = mrun == -INFINITY ? 0.f : mrun;
+      }
+      if (st >= 8) {  // probabilities, 4 per step
+#pragma unroll
+        for (int e = 4 * (st - 8); e < 4 * (st - 8) + 4; ++e) {
+          const int mb = e >> 4, v = e & 15;
+          const float p = fast_exp2(fmaf(sc[mb][v], a.sl2, -muse));
+          lsum += p;
+          sc[mb][v] = p;
+        }
+      }
+      if (st == 11 || st == 15) {  // B operands of keys 32 mb .. 32 mb + 31
+        const int mb = (st - 11) >> 2;
+#pragma unroll
+        for (int u2 = 0; u2 < 2; ++u2) {
+          const int e0 = 8 * u2;
+          pb[2 * mb + u2] = pack_bf16x8(f32x4{sc[mb][e0], sc[mb][e0 + 1], sc[mb][e0 + 2], sc[mb][e0 + 3]},
+                                        f32x4{sc[mb][e0 + 4], sc[mb][e0 + 5], sc[mb][e0 + 6], sc[mb][e0 + 7]});
+        }
+      }
+      if (st == 14) B[0] = vread(vt, 0);
+      if (st == 15) B[1] = vread(vt, 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int n = 0; n < 4 * DB; ++n) {
+      o[n % DB] = mfma32x32x16(B[n & 1], pb[n / DB], o[n % DB]);
+      if (n + 2 < 4 * DB) B[n & 1] = vread(vt, n + 2);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // Step j of the workgroup: tiles j + 2 of K and j + 1 of V to LDS, the next ones on
+  // their way.  Returns tile j's groups without a page.
+  auto stage = [&](int j, auto parity) {
+    constexpr int P = decltype(parity)::value;  // j % 2
+    __syncthreads();
+    kwrite(j + 2, parity);
+    vwrite(j + 1, std::integral_constant<int, P ^ 1>{});
+    const uint32_t none = gone;
+    vload(j + 2);
+    kload(j + 3);
+    return none;
+  };
+  auto masked = [&](int j, auto parity, auto next, f32x16 (&sc)[2], f32x16 (&sn)[2], uint32_t none) {
+    constexpr int P = decltype(parity)::value;
+    iteration(std::true_type{}, next, kbuf + (P ^ 1) * kTileB, vbuf + P * kTileB, sc, sn,
+              opaque(lim - BN * (t0 + j) - 4 * hh), none);
+  };
+  auto step = [&](int j, auto parity, f32x16 (&sc)[2], f32x16 (&sn)[2]) {
+    constexpr int P = decltype(parity)::value;
+    const uint32_t none = stage(j, parity);
+    if (BN * (t0 + j) + BN > clear || none != 0)
+      masked(j, parity, std::true_type{}, sc, sn, none);
+    else
+      iteration(std::false_type{}, std::true_type{}, kbuf + (P ^ 1) * kTileB, vbuf + P * kTileB, sc, sn, 0, 0);
+  };
+  f32x16 sa[2], sb[2];
+  __syncthreads();
+  int j = 0;
+  if (nt_w > 0) {
+    scores_only(kbuf, sa);
+    for (; j + 2 < nt_w; j += 2) {
+      step(j, even, sa, sb);
+      step(j + 1, odd, sb, sa);
+    }
+    if (j + 1 < nt_w) {
+      step(j, even, sa, sb);
+      ++j;
+      masked(j, odd, std::false_type{}, sb, sa, stage(j, odd));
+    } else {
+      masked(j, even, std::false_type{}, sa, sb, stage(j, even));
+    }
+    ++j;
+  }
+  for (; j < ntiles; ++j) {  // what the other waves' rows see beyond
+    if (j & 1) stage(j, odd);
+    else stage(j, even);
+  }
+
+  const uint64_t any = __ballot(strange);
+  if (lane == 0) nan_s[wave] = any != 0;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < RW; ++w) strange |= nan_s[w] != 0;
+  if (strange)
+    patch_nan<16 * DB>(
+        a, table, hk, max(s.k0, all_clear & ~(BN - 1)), min(k1, lim),
+        [&](int n) { return 32 * (n >> 4) + 8 * ((n & 15) >> 2) + 4 * hh + (n & 3); },
+        [&](int n) { o[n >> 4][n & 15] = NAN; });
+  const float l = xor32_sum(lsum);
+  if (r >= a.R) return;
+  const float f = a.direct ? (ok ? inverse_sum(l) : 0.f) : 1.f;
+  const bool nothing = a.direct ? !ok : mrun == -INFINITY;
+  const int64_t pr = partial_row(a, r, hk, slot);
+  uint16_t* out = static_cast<uint16_t*>(a.out) + (((int64_t)s.b * a.p.N + i) * a.p.Hq + hk * a.group + r % a.group) * D;
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      f32x4 x = f32x4{o[d][4 * w], o[d][4 * w + 1], o[d][4 * w + 2], o[d][4 * w + 3]} * f;
+      if (nothing) x = f32x4{0.f, 0.f, 0.f, 0.f};
+      const int at = 32 * d + 8 * w + 4 * hh;
+      if (a.direct) store4(nullptr, out + at, x);
+      else *reinterpret_cast<f32x4*>(a.po + pr * D + at) = x;
+    }
+  if (hh == 0) {
+    if (a.direct) store_stats(a, s.b, hk, r, ok ? mrun : -INFINITY, ok ? l : 0.f);
+    else a.ps[pr] = make_float2(mrun, l);
   }
 }
 
 // ------------------------------------------------------------- the merge --
-
-template <typename T>
-__device__ __forceinline__ void store_vec4(T* p, const f32x4& r) {
-  if constexpr (sizeof(T) == 4) store4(p, nullptr, r);
-  else store4(nullptr, p, r);
-}
 
 // A wave per query row: lane 16 u + j holds 4-element chunks j, j + 16, .. of
 // the head dim for the u-th of every four splits.
@@ -403,7 +794,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a) {
       acc[x] += load_w<float, 4>(a.po + pr * D, 4 * (j + 16 * x), D, true) * w;
   }
   l = group4_sum(l);
-  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // NaN stays
+  const float inv = inverse_sum(l);
   T* out = static_cast<T*>(a.out) + row * D;
 #pragma unroll
   for (int x = 0; x < NI; ++x) {
@@ -411,18 +802,16 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a) {
     for (int e = 0; e < 4; ++e) acc[x][e] = group4_sum(acc[x][e]);
     if (u == 0 && j + 16 * x < nch) store_vec4<T>(out + 4 * (j + 16 * x), acc[x] * inv);
   }
-  if (lane == 0) {
-    const int64_t si = ((int64_t)b * a.p.Hq + h) * a.p.N + i;
-    if (a.m) a.m[si] = top == -INFINITY ? top : top * kLn2;
-    if (a.l) a.l[si] = l;
-  }
+  if (lane == 0) store_stats(a, b, h / a.group, i * a.group + h % a.group, top, l);
 }
 
 // ------------------------------------------------------------------- host --
 
-constexpr int64_t kWanted = 512;  // workgroups for the chip
+constexpr int64_t kWanted = 512;  // workgroups of the streaming form for the chip
+constexpr int64_t kWantedTiled = 256;
 
 struct Plan {
+  bool tiled;
   int rows;  // of a workgroup
   int units, slots;
 };
@@ -431,10 +820,13 @@ Plan make_plan(const PagedProblem& p) {
   const int64_t R = (int64_t)p.N * (p.Hq / p.pool.Hkv);
   const int64_t tiles = (int64_t)p.B * (((int64_t)p.width * p.pool.rows + kTile - 1) / kTile);
   Plan x;
-  x.rows = 16;
+  x.tiled = p.dtype == 1 && (p.pool.D == 64 || p.pool.D == 128) && R > 64;
+  x.rows = x.tiled ? 256 : 16;
   x.units = (int)((R + x.rows - 1) / x.rows * p.pool.Hkv);
-  const int64_t slots = std::max<int64_t>(1, std::min<int64_t>(kWanted / x.units, tiles));
-  x.slots = (int)(p.B > kTightBatch ? slots + p.B : std::max<int64_t>(slots, p.B > 1 ? p.B + slots / 2 : 1));
+  const int64_t slots =
+      std::max<int64_t>(1, std::min<int64_t>((x.tiled ? kWantedTiled : kWanted) / x.units, tiles));
+  if (slots == 1) x.slots = p.B;
+  else x.slots = (int)(p.B > kTightBatch ? slots + p.B : std::max<int64_t>(slots, p.B > 1 ? p.B + slots / 2 : 1));
   return x;
 }
 
@@ -442,6 +834,7 @@ Plan make_plan(const PagedProblem& p) {
 
 size_t paged_attn_bytes(const PagedProblem& p) {
   const Plan x = make_plan(p);
+  if (x.slots == p.B) return (size_t)p.B * sizeof(int2);
   return (size_t)x.slots * p.N * p.Hq * (p.pool.D + 2) * sizeof(float) + (size_t)p.B * sizeof(int2);
 }
 
@@ -455,17 +848,19 @@ hipError_t launch_paged_attn(const PagedProblem& p, const void* q, void* out, fl
   a.out = out;
   a.m = m;
   a.l = l;
+  a.direct = x.slots == p.B;
+  const int64_t parts = a.direct ? 0 : prows;
   a.po = static_cast<float*>(ws);
-  a.ps = reinterpret_cast<float2*>(a.po + prows * p.pool.D);
-  a.deal = reinterpret_cast<int2*>(a.ps + prows);
+  a.ps = reinterpret_cast<float2*>(a.po + parts * p.pool.D);
+  a.deal = reinterpret_cast<int2*>(a.ps + parts);
   a.group = p.Hq / p.pool.Hkv;
   a.R = p.N * a.group;
   a.slots = x.slots;
   a.units = x.units;
   a.shift = __builtin_ctz((unsigned)p.pool.rows);
   a.sl2 = (float)(1.4426950408889634 / sqrt((double)p.pool.D));
-  auto launch = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(x.slots * x.units)), dim3(256), 0, st, a);
+  auto launch = [&](auto kernel, int threads = 256) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(x.slots * x.units)), dim3(threads), 0, st, a);
   };
   auto by_dim = [&](auto parts) {
     constexpr int P = decltype(parts)::value;
@@ -474,10 +869,12 @@ hipError_t launch_paged_attn(const PagedProblem& p, const void* q, void* out, fl
     else if (p.pool.D < 128) launch(paged_stream_kernel<128, false, 1, P>);
     else launch(paged_stream_kernel<256, false, 1, P>);
   };
-  if (p.dtype == 1) by_dim(std::integral_constant<int, 1>{});
+  if (x.tiled && p.pool.D == 64) launch(paged_tile_kernel<64>, 512);
+  else if (x.tiled) launch(paged_tile_kernel<128>, 512);
+  else if (p.dtype == 1) by_dim(std::integral_constant<int, 1>{});
   else by_dim(std::integral_constant<int, 3>{});
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
+  if (e != hipSuccess || a.direct) return e;
   const int64_t rows = (int64_t)p.B * p.N * p.Hq;
   auto merge = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
