@@ -3,7 +3,7 @@
 // read here.  A slot holds `per` tiles of one sequence, the fewest with which the
 // slots suffice for all, so a batch of unequal lengths loads the chip evenly.
 //
-// rows(b) is the number of keys of sequence b, below 2^30.
+// rows(b) is the number of keys of sequence b, below 2^30; TILE keys are a tile.
 #pragma once
 
 #include "cache.h"
@@ -14,7 +14,10 @@ namespace lc {
 constexpr int kTile = 64;  // keys by which a sequence is dealt out
 
 // Tiles of a sequence, at least one (so that every sequence has a slot).
-__device__ __forceinline__ int tiles_of(int rows) { return max(1, (rows + kTile - 1) / kTile); }
+template <int TILE>
+__device__ __forceinline__ int tiles_of(int rows) {
+  return max(1, (rows + TILE - 1) / TILE);
+}
 
 __device__ __forceinline__ int wave_sum_i(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
 
@@ -35,18 +38,18 @@ constexpr int kTightBatch = 64;
 // size whose slots suffice is taken.  More sequences have B slots beyond the
 // even shares, and ceil(tiles / per) adds less than one each.  As many slots as
 // sequences: a slot is a whole sequence.
-template <typename Rows>
+template <int TILE, typename Rows>
 __device__ __forceinline__ int slot_tiles(const Rows& rows, int B, int slots) {
   const int lane = threadIdx.x & 63;
-  if (B == 1) return (tiles_of(rows(0)) + slots - 1) / slots;
-  if (slots == B) return 1 << 24;
+  if (B == 1) return (tiles_of<TILE>(rows(0)) + slots - 1) / slots;
+  if (slots == B) return (1 << 30) / TILE;
   if (B > kTightBatch) {
     int total = 0;
     for (int b0 = 0; b0 < B; b0 += 64)
-      total += wave_sum_i(b0 + lane < B ? tiles_of(rows(b0 + lane)) : 0);
+      total += wave_sum_i(b0 + lane < B ? tiles_of<TILE>(rows(b0 + lane)) : 0);
     return (total + slots - B - 1) / (slots - B);
   }
-  const int mine = lane < B ? tiles_of(rows(lane)) : 0;
+  const int mine = lane < B ? tiles_of<TILE>(rows(lane)) : 0;
   int most = mine;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) most = max(most, __shfl_xor(most, off, 64));
@@ -65,17 +68,17 @@ struct Share {
 };
 // Finds the share of a slot; false: it has none.  The first workgroup leaves
 // every sequence's first slot and its slots in deal [B].
-template <typename Rows>
+template <int TILE = kTile, typename Rows>
 __device__ __forceinline__ bool share_of(const Rows& rows, int B, int slots, int2* deal, int slot,
                                          Share& s) {
   const int lane = threadIdx.x & 63;
-  const int per = slot_tiles(rows, B, slots);
+  const int per = slot_tiles<TILE>(rows, B, slots);
   const float inv = 1.f / (float)per;
   int first = 0, at = -1;  // of sequence at
   int base = 0;
   for (int b0 = 0; b0 < B; b0 += 64) {
     const int b = b0 + lane;
-    const int n = b < B ? slots_for(tiles_of(rows(b)), per, inv) : 0;
+    const int n = b < B ? slots_for(tiles_of<TILE>(rows(b)), per, inv) : 0;
     const int end = base + wave_scan(n);
     if (blockIdx.x == 0 && threadIdx.x < 64 && b < B) deal[b] = make_int2(end - n, n);
     const uint64_t who = __ballot(slot < end && slot >= end - n);
@@ -89,8 +92,8 @@ __device__ __forceinline__ bool share_of(const Rows& rows, int B, int slots, int
   if (at < 0) return false;
   s.b = __builtin_amdgcn_readfirstlane(at);
   const int n = rows(s.b);
-  s.k0 = __builtin_amdgcn_readfirstlane(min((slot - first) * per * kTile, n));
-  s.k1 = __builtin_amdgcn_readfirstlane(min(n - s.k0, per * kTile)) + s.k0;
+  s.k0 = __builtin_amdgcn_readfirstlane(min((slot - first) * per * TILE, n));
+  s.k1 = __builtin_amdgcn_readfirstlane(min(n - s.k0, per * TILE)) + s.k0;
   return true;
 }
 

@@ -178,14 +178,42 @@ __device__ __forceinline__ void patch_nan(const AttnArgs& a, const int32_t* tabl
 
 // ------------------------------------------------------- a few query rows --
 
+// a, b of the lanes c and c ^ 8 of 16: the lower eight get (a, a of the other), the
+// upper eight (b of the other, b).
+__device__ __forceinline__ uint32_t ror8(uint32_t old, uint32_t x, bool upper) {
+  return (uint32_t)(upper ? __builtin_amdgcn_update_dpp((int)old, (int)x, 0x128, 0xf, 0xc, false)
+                          : __builtin_amdgcn_update_dpp((int)old, (int)x, 0x128, 0xf, 0x3, false));
+}
+__device__ __forceinline__ void swap_halves(uint4& a, uint4& b) {
+  const uint4 t = a;
+  a = make_uint4(ror8(a.x, b.x, true), ror8(a.y, b.y, true), ror8(a.z, b.z, true), ror8(a.w, b.w, true));
+  b = make_uint4(ror8(b.x, t.x, false), ror8(b.y, t.y, false), ror8(b.z, t.z, false), ror8(b.w, t.w, false));
+}
+
+// 16 bytes that nobody else reads (NT), or that others find in L2.
+template <bool NT>
+__device__ __forceinline__ uint4 load16(const uint8_t* p) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  if constexpr (!NT) return *reinterpret_cast<const uint4*>(p);
+  const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+  return make_uint4(x[0], x[1], x[2], x[3]);
+}
+
 // Every wave holds all of the workgroup's 16 * NB rows and walks a run of the
 // slot's tiles; the four waves meet in LDS.
+// A load of a wave should take whole cache lines: half a line at a time, its other
+// half with the next load, costs a tenth of the stream.  So of a key of 128 bytes
+// eight lanes take one half and eight the other, two loads take twice as many
+// keys, and the lanes swap; the same for V in pages of 128 rows (VT = 2), a dim's
+// line of which is two tiles' keys.
 // DP: head_dim, rounded up to 64, 128 or 256 unless EXACT.
-template <int DP, bool EXACT, int NB, int PARTS>
+template <int DP, bool EXACT, int NB, int PARTS, int VT, bool NT>
 __global__ __launch_bounds__(256, DP * PARTS > 192 ? 1 : 2) void paged_stream_kernel(AttnArgs a) {
   typedef typename std::conditional<PARTS == 1, uint16_t, float>::type T;
   constexpr int KJ = DP / 64, DB = DP / 16;  // 16-byte pieces of a key a lane takes; 16-dim blocks
   constexpr int W = 4, kRows = 16 * NB, kPitch = DP + 4;
+  constexpr bool kLines = EXACT && DP == 128;
+  static_assert(VT == 1 || EXACT, "two tiles of V at once");
   __shared__ __attribute__((aligned(16))) float part[W * kRows * kPitch];
   __shared__ float msm[W][kRows], lsm[W][kRows];
 
@@ -199,7 +227,7 @@ __global__ __launch_bounds__(256, DP * PARTS > 192 ? 1 : 2) void paged_stream_ke
   const int rb = unit / pool.Hkv;
   const int D = EXACT ? DP : pool.D;
   Share s;
-  if (!share_of([&](int b) { return keys_of(a, b); }, a.p.B, a.slots, a.deal, slot, s)) return;
+  if (!share_of<64 * VT>([&](int b) { return keys_of(a, b); }, a.p.B, a.slots, a.deal, slot, s)) return;
 
   const int past = a.p.past[s.b];
   const int count = new_tokens(a.p.counts, a.p.N, s.b, past);
@@ -208,7 +236,7 @@ __global__ __launch_bounds__(256, DP * PARTS > 192 ? 1 : 2) void paged_stream_ke
   const int first = rb * kRows / a.group, last = min((rb * kRows + kRows - 1) / a.group, count - 1);
   const int k1 = min(s.k1, past + last + 1);  // (no token: last < first, and nothing is walked)
   const int all = last >= first && k1 > s.k0 ? (k1 - s.k0 + 63) / 64 : 0;
-  const int per = (all + W - 1) / W;
+  const int per = (all + W * VT - 1) / (W * VT) * VT;
   const int t0 = s.k0 / 64 + min(wave * per, all), t1 = s.k0 / 64 + min((wave + 1) * per, all);
   const int clear = past + first + 1;  // keys that all rows see
   bool strange = false;                // NaN among the values of tiles beyond
@@ -244,29 +272,50 @@ __global__ __launch_bounds__(256, DP * PARTS > 192 ? 1 : 2) void paged_stream_ke
     run.scales(a, hk);
   }
   const int64_t head_bytes = (int64_t)D << a.shift;
-  uint4 kr[4][KJ], vr[DB];
+  uint4 kr[4][KJ], vr[VT][DB];
   auto base = [&](const uint8_t* p, int page) {
     return p + ((int64_t)max(page, 0) * pool.Hkv + hk) * head_bytes;
   };
+  const int page_mask = (1 << a.shift) - 1;
   auto kload = [&](int t) {
-    const int x = 4 * (t - t0 & 15) + (c >> 2);
-    const int row = (64 * t + 16 * (c >> 2)) & ((1 << a.shift) - 1);
-    const uint8_t* p = base(pool.k, __shfl(run.page, x, 64)) + (row + (c & 3)) * D;
+    const int x = 4 * (t - t0 & 15);
+    if constexpr (kLines) {
 #pragma unroll
-    for (int mb = 0; mb < 4; ++mb)
+      for (int i = 0; i < 2; ++i) {
+        const int gk = 2 * i + (c >> 2 & 1);
+        const int row = 64 * t + 16 * gk & page_mask;
+        const uint8_t* p = base(pool.k, __shfl(run.page, x + gk, 64)) + (row + (c & 3)) * D + 64 * (c >> 3) + 16 * g;
 #pragma unroll
-      for (int j = 0; j < KJ; ++j) {
-        const int d = 64 * j + 16 * g;
-        kr[mb][j] = *reinterpret_cast<const uint4*>(p + 4 * mb * D + (EXACT || d < D ? d : 0));
+        for (int mb = 0; mb < 4; ++mb) kr[mb][i] = load16<NT>(p + 4 * mb * D);
       }
+    } else {
+      const int row = 64 * t + 16 * (c >> 2) & page_mask;
+      const uint8_t* p = base(pool.k, __shfl(run.page, x + (c >> 2), 64)) + (row + (c & 3)) * D;
+#pragma unroll
+      for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) {
+          const int d = 64 * j + 16 * g;
+          kr[mb][j] = load16<NT>(p + 4 * mb * D + (EXACT || d < D ? d : 0));
+        }
+    }
   };
   auto vload = [&](int t) {
-    const int x = 4 * (t - t0 & 15) + g;
-    const int row = (64 * t + 16 * g) & ((1 << a.shift) - 1);
-    const uint8_t* p = base(pool.v, __shfl(run.page, x, 64)) + ((int64_t)c << a.shift) + row;
+    const int x = 4 * (t - t0 & 15);
+    if constexpr (VT == 2) {
+      const uint8_t* p = base(pool.v, __builtin_amdgcn_readlane(run.page, x)) + 128 * (c & 7) + 64 * (c >> 3) + 16 * g;
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
-      vr[db] = *reinterpret_cast<const uint4*>(p + ((int64_t)(EXACT || 16 * db < D ? 16 * db : 0) << a.shift));
+      for (int db = 0; db < DB; ++db) {
+        vr[0][db] = load16<NT>(p + 128 * 16 * db);
+        vr[1][db] = load16<NT>(p + 128 * (16 * db + 8));
+      }
+    } else {
+      const int row = 64 * t + 16 * g & page_mask;
+      const uint8_t* p = base(pool.v, __shfl(run.page, x + g, 64)) + ((int64_t)c << a.shift) + row;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+        vr[0][db] = load16<NT>(p + ((int64_t)(EXACT || 16 * db < D ? 16 * db : 0) << a.shift));
+    }
   };
 
   f32x4 o[NB][DB];
@@ -285,11 +334,18 @@ __global__ __launch_bounds__(256, DP * PARTS > 192 ? 1 : 2) void paged_stream_ke
     vload(t0);
     run.look(a, table, t0 + 16, k1);
   }
-  for (int t = t0; t < t1; ++t) {
+  auto tile = [&](int t, auto sub) {
+    constexpr int V = decltype(sub)::value;  // of the tiles whose values are here
     const int x = 4 * (t - t0 & 15);
     const float ks = __shfl(run.ks, x + (c >> 2), 64);  // of the lane's K
     const float vs = __shfl(run.vs, x + g, 64);         // of its V
     const int page = __shfl(run.page, x + g, 64);
+    if constexpr (kLines)
+#pragma unroll
+      for (int mb = 0; mb < 4; ++mb) swap_halves(kr[mb][0], kr[mb][1]);
+    if constexpr (VT == 2 && V == 0)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) swap_halves(vr[0][db], vr[1][db]);
     f32x4 sc[NB][4];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
@@ -327,9 +383,9 @@ __global__ __launch_bounds__(256, DP * PARTS > 192 ? 1 : 2) void paged_stream_ke
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
         if (edge) {
-          strange |= clean_values(vr[db], left);
+          strange |= clean_values(vr[V][db], left);
         } else if (left <= 0) {
-          vr[db] = make_uint4(0u, 0u, 0u, 0u);
+          vr[V][db] = make_uint4(0u, 0u, 0u, 0u);
         }
       }
 #pragma unroll
@@ -374,14 +430,19 @@ __global__ __launch_bounds__(256, DP * PARTS > 192 ? 1 : 2) void paged_stream_ke
       for (int nb = 0; nb < NB; ++nb) split8<PARTS>(sc[nb][2 * k2], sc[nb][2 * k2 + 1], pb[nb]);
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
-        const bf16x8 v = bf16_of(k2 ? vr[db].z : vr[db].x, k2 ? vr[db].w : vr[db].y, vs);
+        const bf16x8 v = bf16_of(k2 ? vr[V][db].z : vr[V][db].x, k2 ? vr[V][db].w : vr[V][db].y, vs);
 #pragma unroll
         for (int p = PARTS - 1; p >= 0; --p)
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) o[nb][db] = mfma16x16x32(v, pb[nb][p], o[nb][db]);
       }
     }
-    if (more) vload(t + 1);
+  };
+  for (int t = t0; t < t1; t += VT) {
+    tile(t, std::integral_constant<int, 0>{});
+    if constexpr (VT == 2)
+      if (t + 1 < t1) tile(t + 1, std::integral_constant<int, 1>{});
+    if (t + VT < t1) vload(t + VT);
   }
 
   if (__any(strange))
@@ -813,16 +874,18 @@ constexpr int64_t kWantedTiled = 256;
 struct Plan {
   bool tiled;
   int rows;  // of a workgroup
+  int tile;  // keys by which a sequence is dealt out
   int units, slots;
 };
 
 Plan make_plan(const PagedProblem& p) {
   const int64_t R = (int64_t)p.N * (p.Hq / p.pool.Hkv);
-  const int64_t tiles = (int64_t)p.B * (((int64_t)p.width * p.pool.rows + kTile - 1) / kTile);
   Plan x;
   x.tiled = p.dtype == 1 && (p.pool.D == 64 || p.pool.D == 128) && R > 64;
   x.rows = x.tiled ? 256 : 16;
+  x.tile = !x.tiled && p.pool.rows == 128 && (p.pool.D == 64 || p.pool.D == 128) ? 128 : 64;
   x.units = (int)((R + x.rows - 1) / x.rows * p.pool.Hkv);
+  const int64_t tiles = (int64_t)p.B * (((int64_t)p.width * p.pool.rows + x.tile - 1) / x.tile);
   const int64_t slots =
       std::max<int64_t>(1, std::min<int64_t>((x.tiled ? kWantedTiled : kWanted) / x.units, tiles));
   if (slots == 1) x.slots = p.B;
@@ -862,17 +925,26 @@ hipError_t launch_paged_attn(const PagedProblem& p, const void* q, void* out, fl
   auto launch = [&](auto kernel, int threads = 256) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)(x.slots * x.units)), dim3(threads), 0, st, a);
   };
-  auto by_dim = [&](auto parts) {
+  const bool once = x.units == p.pool.Hkv;  // the cache is read once
+  auto by_dim = [&](auto parts, auto nt) {
     constexpr int P = decltype(parts)::value;
-    if (p.pool.D == 64) launch(paged_stream_kernel<64, true, 1, P>);
-    else if (p.pool.D == 128) launch(paged_stream_kernel<128, true, 1, P>);
-    else if (p.pool.D < 128) launch(paged_stream_kernel<128, false, 1, P>);
-    else launch(paged_stream_kernel<256, false, 1, P>);
+    constexpr bool NT = decltype(nt)::value;
+    const bool two = x.tile == 128;
+    if (p.pool.D == 64 && two) launch(paged_stream_kernel<64, true, 1, P, 2, NT>);
+    else if (p.pool.D == 64) launch(paged_stream_kernel<64, true, 1, P, 1, NT>);
+    else if (p.pool.D == 128 && two) launch(paged_stream_kernel<128, true, 1, P, 2, NT>);
+    else if (p.pool.D == 128) launch(paged_stream_kernel<128, true, 1, P, 1, NT>);
+    else if (p.pool.D < 128) launch(paged_stream_kernel<128, false, 1, P, 1, NT>);
+    else launch(paged_stream_kernel<256, false, 1, P, 1, NT>);
+  };
+  auto by_reads = [&](auto parts) {
+    if (once) by_dim(parts, std::true_type{});
+    else by_dim(parts, std::false_type{});
   };
   if (x.tiled && p.pool.D == 64) launch(paged_tile_kernel<64>, 512);
   else if (x.tiled) launch(paged_tile_kernel<128>, 512);
-  else if (p.dtype == 1) by_dim(std::integral_constant<int, 1>{});
-  else by_dim(std::integral_constant<int, 3>{});
+  else if (p.dtype == 1) by_reads(std::integral_constant<int, 1>{});
+  else by_reads(std::integral_constant<int, 3>{});
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.direct) return e;
   const int64_t rows = (int64_t)p.B * p.N * p.Hq;
