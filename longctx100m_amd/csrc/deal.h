@@ -97,4 +97,76 @@ __device__ __forceinline__ bool share_of(const Rows& rows, int B, int slots, int
   return true;
 }
 
+// The same with slots that do not end where a sequence does: the tiles of all
+// sequences one behind another, every slot the same number of them, `least` at
+// least.  A slot's run of one sequence's tiles is a segment, number slot + b (each
+// step of either starts one, so slots + B numbers suffice).
+//   for (Spans<TILE, Rows> s(...); s.next();) ... s.b, s.k0, s.k1, s.segment
+// visits a slot's segments, the whole workgroup together; a sequence without keys
+// has none.  The first workgroup leaves every sequence's first segment and its
+// segments in deal [B].  whole: slot b is sequence b, also one without keys.
+template <int TILE, typename Rows>
+struct Spans {
+  const Rows& rows;
+  int B, slot;
+  bool whole;
+  int2* deal;
+  int per, t0, t1;
+  int b0, base, mine, end;  // of the 64 sequences from b0 on, over the lanes
+  uint64_t left;            // those still to visit
+  int b, k0, k1, segment;
+
+  __device__ __forceinline__ static int tiles(int n) { return (n + TILE - 1) / TILE; }
+  __device__ __forceinline__ Spans(const Rows& rows_, int B_, int slots, bool whole_, int least, int2* deal_,
+                                   int slot_)
+      : rows(rows_), B(B_), slot(slot_), whole(whole_), deal(deal_) {
+    const int lane = threadIdx.x & 63;
+    b0 = -64;
+    base = 0;
+    left = 0;
+    per = t0 = t1 = 0;
+    if (whole) return;
+    int all = 0;
+    if (B == 1) all = tiles(rows(0));
+    else
+      for (int x = 0; x < B; x += 64) all += wave_sum_i(x + lane < B ? tiles(rows(x + lane)) : 0);
+    per = __builtin_amdgcn_readfirstlane(max((all + slots - 1) / slots, least));
+    t0 = slot * per;
+    t1 = min(t0 + per, all);
+  }
+  __device__ __forceinline__ bool next() {
+    if (whole) {
+      if (b0 >= 0) return false;
+      b0 = 0;
+      b = slot;
+      k0 = 0;
+      k1 = __builtin_amdgcn_readfirstlane(rows(b));
+      segment = b;
+      return true;
+    }
+    const int lane = threadIdx.x & 63;
+    while (left == 0) {
+      b0 += 64;
+      if (b0 >= B || (base >= t1 && blockIdx.x != 0)) return false;
+      mine = b0 + lane < B ? tiles(rows(b0 + lane)) : 0;
+      end = base + wave_scan(mine);
+      if (blockIdx.x == 0 && threadIdx.x < 64 && b0 + lane < B) {
+        const int first = (end - mine) / per, last = mine > 0 ? (end - 1) / per : first - 1;
+        deal[b0 + lane] = make_int2(first + b0 + lane, last - first + 1);
+      }
+      left = __ballot(mine > 0 && end > t0 && end - mine < t1);
+      base = __builtin_amdgcn_readlane(end, 63);
+    }
+    const int x = __ffsll((unsigned long long)left) - 1;
+    left &= left - 1;
+    b = b0 + x;
+    segment = slot + b;
+    const int stop = __builtin_amdgcn_readlane(end, x), start = stop - __builtin_amdgcn_readlane(mine, x);
+    const int n = __builtin_amdgcn_readfirstlane(rows(b));
+    k0 = max(t0 - start, 0) * TILE;
+    k1 = stop <= t1 ? n : (t1 - start) * TILE;
+    return true;
+  }
+};
+
 }  // namespace lc

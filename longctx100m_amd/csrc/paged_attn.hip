@@ -40,13 +40,14 @@ struct AttnArgs {
   const void* q;
   void* out;
   float *m, *l;
-  // Partials, slot s of query row (token, head) at row * slots + s: D values, and
+  // Partials, part s of query row (token, head) at row * parts + s: D values, and
   // (m, l), m in log2 units.
   float* po;
   float2* ps;
-  int2* deal;  // [B]: a sequence's first slot and its slots
+  int2* deal;  // [B]: a sequence's first part and its parts
   int group, R;
   int slots, units;  // units: workgroups of a slot
+  int parts;
   int shift;         // log2 of a page's rows
   bool direct;       // a slot is a whole sequence: results in place of partials
   float sl2;
@@ -59,8 +60,8 @@ __device__ __forceinline__ int keys_of(const AttnArgs& a, int b) {
   return n > 0 ? (int)min((int64_t)past + n, (int64_t)a.p.width << a.shift) : 0;
 }
 
-__device__ __forceinline__ int64_t partial_row(const AttnArgs& a, int r, int hk, int slot) {
-  return ((int64_t)(r / a.group) * a.p.Hq + hk * a.group + r % a.group) * a.slots + slot;
+__device__ __forceinline__ int64_t partial_row(const AttnArgs& a, int r, int hk, int part) {
+  return ((int64_t)(r / a.group) * a.p.Hq + hk * a.group + r % a.group) * a.parts + part;
 }
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -199,36 +200,35 @@ __device__ __forceinline__ uint4 load16(const uint8_t* p) {
   return make_uint4(x[0], x[1], x[2], x[3]);
 }
 
-// Every wave holds all of the workgroup's 16 * NB rows and walks a run of the
-// slot's tiles; the four waves meet in LDS.
+// Bound by the stream of the cache.  Every wave holds all of the workgroup's 16 * NB
+// rows and walks a run of the segment's tiles; the W waves meet in LDS.
 // A load of a wave should take whole cache lines: half a line at a time, its other
 // half with the next load, costs a tenth of the stream.  So of a key of 128 bytes
 // eight lanes take one half and eight the other, two loads take twice as many
 // keys, and the lanes swap; the same for V in pages of 128 rows (VT = 2), a dim's
 // line of which is two tiles' keys.
 // DP: head_dim, rounded up to 64, 128 or 256 unless EXACT.
-template <int DP, bool EXACT, int NB, int PARTS, int VT, bool NT>
-__global__ __launch_bounds__(256, DP * PARTS > 192 ? 1 : 2) void paged_stream_kernel(AttnArgs a) {
+template <int DP, bool EXACT, int NB, int PARTS, int VT, bool NT, int W>
+__global__ __launch_bounds__(64 * W, DP * PARTS > 192 || W > 4 ? 1 : 2) void paged_stream_kernel(AttnArgs a) {
   typedef typename std::conditional<PARTS == 1, uint16_t, float>::type T;
   constexpr int KJ = DP / 64, DB = DP / 16;  // 16-byte pieces of a key a lane takes; 16-dim blocks
-  constexpr int W = 4, kRows = 16 * NB, kPitch = DP + 4;
+  constexpr int kRows = 16 * NB, kPitch = DP + 4;
   constexpr bool kLines = EXACT && DP == 128;
   static_assert(VT == 1 || EXACT, "two tiles of V at once");
   __shared__ __attribute__((aligned(16))) float part[W * kRows * kPitch];
   __shared__ float msm[W][kRows], lsm[W][kRows];
 
-  const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int c = lane & 15, g = lane >> 4;
   const int slot = blockIdx.x / a.units;
   const int unit = blockIdx.x - slot * a.units;
   const Pool& pool = a.p.pool;
   const int hk = unit % pool.Hkv;
   const int rb = unit / pool.Hkv;
   const int D = EXACT ? DP : pool.D;
-  Share s;
-  if (!share_of<64 * VT>([&](int b) { return keys_of(a, b); }, a.p.B, a.slots, a.deal, slot, s)) return;
-
+  auto keys = [&](int b) { return keys_of(a, b); };
+  for (Spans<64 * VT, decltype(keys)> s(keys, a.p.B, a.slots, a.direct, W, a.deal, slot); s.next();) {
+  // (opaque: what follows from it is formed in each segment, not kept in registers)
+  const int tid = opaque(threadIdx.x), lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int past = a.p.past[s.b];
   const int count = new_tokens(a.p.counts, a.p.N, s.b, past);
   const int32_t* table = a.p.table + (int64_t)s.b * a.p.width;
@@ -472,7 +472,7 @@ __global__ __launch_bounds__(256, DP * PARTS > 192 ? 1 : 2) void paged_stream_ke
   }
   __syncthreads();
   const int chunks = D / 4;  // of a row
-  for (int it = threadIdx.x; it < kRows * chunks; it += 256) {
+  for (int it = tid; it < kRows * chunks; it += 64 * W) {
     const int rr = it / chunks, d = 4 * (it - rr * chunks);
     const int r = rb * kRows + rr;
     if (r >= a.R) break;
@@ -490,10 +490,12 @@ __global__ __launch_bounds__(256, DP * PARTS > 192 ? 1 : 2) void paged_stream_ke
       store_vec4(static_cast<T*>(a.out) + qi * D + d, there ? acc * inverse_sum(L) : f32x4{0.f, 0.f, 0.f, 0.f});
       if (d == 0) store_stats(a, s.b, hk, r, there ? M : -INFINITY, there ? L : 0.f);
     } else {
-      const int64_t pr = partial_row(a, r, hk, slot);
+      const int64_t pr = partial_row(a, r, hk, s.segment);
       *reinterpret_cast<f32x4*>(a.po + pr * D + d) = acc;
       if (d == 0) a.ps[pr] = make_float2(M, L);
     }
+  }
+  __syncthreads();  // the next segment's partials take their place
   }
 }
 
@@ -818,51 +820,75 @@ __global__ __launch_bounds__(512, 1) void paged_tile_kernel(AttnArgs a) {
 
 // ------------------------------------------------------------- the merge --
 
-// A wave per query row: lane 16 u + j holds 4-element chunks j, j + 16, .. of
-// the head dim for the u-th of every four splits.
-template <typename T, int NI>
+// WPR waves per query row, its parts dealt over them: lane 16 u + j holds 4-element
+// chunks j, j + 16, .. of the head dim for the u-th of every four parts.
+template <typename T, int NI, int WPR>
 __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a) {
+  constexpr int kRows = 4 / WPR;  // of a workgroup
+  __shared__ float top_s[4], l_s[4];
+  __shared__ f32x4 acc_s[4][16 * NI];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int j = lane & 15, u = lane >> 4;
-  const int64_t row = 4 * (int64_t)blockIdx.x + wave;
-  if (row >= (int64_t)a.p.B * a.p.N * a.p.Hq) return;
+  const int j = lane & 15, u = lane >> 4, w0 = wave % WPR;
+  const int64_t row = kRows * (int64_t)blockIdx.x + wave / WPR;
+  if (row >= (int64_t)a.p.B * a.p.N * a.p.Hq) return;  // (WPR = 4: nobody)
   const int h = (int)(row % a.p.Hq);
   const int64_t bi = row / a.p.Hq;
   const int b = (int)(bi / a.p.N), i = (int)(bi - (int64_t)b * a.p.N);
   const int D = a.p.pool.D, nch = D / 4;
   const bool there = i < new_tokens(a.p.counts, a.p.N, b, a.p.past[b]);
   const int2 deal = a.deal[b];
-  const int splits = there ? deal.y : 0;
-  const int64_t pr0 = ((int64_t)i * a.p.Hq + h) * a.slots + deal.x;
+  const int parts = there ? deal.y : 0;
+  const int64_t pr0 = ((int64_t)i * a.p.Hq + h) * a.parts + deal.x;
   float top = -INFINITY;
-  for (int s = lane; s < splits; s += 64) top = fmaxf(top, a.ps[pr0 + s].x);
+  for (int s = 64 * w0 + lane; s < parts; s += 64 * WPR) top = fmaxf(top, a.ps[pr0 + s].x);
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+  if constexpr (WPR > 1) {
+    if (lane == 0) top_s[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WPR; ++w) top = fmaxf(top, top_s[w]);
+  }
   const float muse = top == -INFINITY ? 0.f : top;
   f32x4 acc[NI];
 #pragma unroll
   for (int x = 0; x < NI; ++x) acc[x] = f32x4{0.f, 0.f, 0.f, 0.f};
   float l = 0.f;
 #pragma unroll 4
-  for (int s = u; s < splits; s += 4) {
+  for (int s = 4 * w0 + u; s < parts; s += 4 * WPR) {
     const int64_t pr = pr0 + s;
     const float2 st = a.ps[pr];
-    const float w = exp2f(st.x - muse);  // a split without keys: 0
+    const float w = exp2f(st.x - muse);  // a part without keys: 0
     l += w * st.y;
 #pragma unroll
     for (int x = 0; x < NI; ++x)
       acc[x] += load_w<float, 4>(a.po + pr * D, 4 * (j + 16 * x), D, true) * w;
   }
   l = group4_sum(l);
+#pragma unroll
+  for (int x = 0; x < NI; ++x)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[x][e] = group4_sum(acc[x][e]);
+  if constexpr (WPR > 1) {
+    if (u == 0)
+#pragma unroll
+      for (int x = 0; x < NI; ++x) acc_s[wave][j + 16 * x] = acc[x];
+    if (lane == 0) l_s[wave] = l;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int w = 1; w < WPR; ++w) {
+      l += l_s[w];
+#pragma unroll
+      for (int x = 0; x < NI; ++x) acc[x] += acc_s[w][j + 16 * x];
+    }
+  }
   const float inv = inverse_sum(l);
   T* out = static_cast<T*>(a.out) + row * D;
 #pragma unroll
-  for (int x = 0; x < NI; ++x) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[x][e] = group4_sum(acc[x][e]);
+  for (int x = 0; x < NI; ++x)
     if (u == 0 && j + 16 * x < nch) store_vec4<T>(out + 4 * (j + 16 * x), acc[x] * inv);
-  }
   if (lane == 0) store_stats(a, b, h / a.group, i * a.group + h % a.group, top, l);
 }
 
@@ -870,12 +896,17 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a) {
 
 constexpr int64_t kWanted = 512;  // workgroups of the streaming form for the chip
 constexpr int64_t kWantedTiled = 256;
+constexpr int64_t kShort = 16;  // tiles of a sequence that are not split over workgroups
+
+// Query rows from which a wave each is enough for the merge.
+constexpr int64_t kManyRows = 1024;
 
 struct Plan {
   bool tiled;
   int rows;  // of a workgroup
-  int tile;  // keys by which a sequence is dealt out
-  int units, slots;
+  int tile;  // keys by which sequences are dealt out
+  int waves;
+  int units, slots, parts;  // parts: 0, results without a merge
 };
 
 Plan make_plan(const PagedProblem& p) {
@@ -885,77 +916,103 @@ Plan make_plan(const PagedProblem& p) {
   x.rows = x.tiled ? 256 : 16;
   x.tile = !x.tiled && p.pool.rows == 128 && (p.pool.D == 64 || p.pool.D == 128) ? 128 : 64;
   x.units = (int)((R + x.rows - 1) / x.rows * p.pool.Hkv);
-  const int64_t tiles = (int64_t)p.B * (((int64_t)p.width * p.pool.rows + x.tile - 1) / x.tile);
-  const int64_t slots =
-      std::max<int64_t>(1, std::min<int64_t>((x.tiled ? kWantedTiled : kWanted) / x.units, tiles));
-  if (slots == 1) x.slots = p.B;
-  else x.slots = (int)(p.B > kTightBatch ? slots + p.B : std::max<int64_t>(slots, p.B > 1 ? p.B + slots / 2 : 1));
+  const int64_t each = ((int64_t)p.width * p.pool.rows + x.tile - 1) / x.tile;  // tiles of a sequence
+  const int64_t want = (x.tiled ? kWantedTiled : kWanted) / x.units;
+  x.waves = 8;
+  if (x.tiled) {
+    const int64_t slots = std::max<int64_t>(1, std::min<int64_t>(want, p.B * each));
+    x.slots = slots == 1           ? p.B
+              : p.B > kTightBatch ? (int)slots + p.B
+                                  : (int)std::max<int64_t>(slots, p.B > 1 ? p.B + slots / 2 : 1);
+    x.parts = x.slots == p.B ? 0 : x.slots;
+    return x;
+  }
+  if (each <= kShort || want <= 1) {
+    x.waves = want <= p.B || p.dtype == 0 || (p.pool.D != 64 && p.pool.D != 128) ? 4 : 8;
+    x.slots = p.B;
+    x.parts = 0;
+  } else {
+    x.waves = 4;
+    x.slots = (int)std::max<int64_t>(1, std::min<int64_t>(want, (p.B * each + x.waves - 1) / x.waves));
+    x.parts = x.slots + p.B;
+  }
   return x;
 }
 
 }  // namespace
 
 size_t paged_attn_bytes(const PagedProblem& p) {
-  const Plan x = make_plan(p);
-  if (x.slots == p.B) return (size_t)p.B * sizeof(int2);
-  return (size_t)x.slots * p.N * p.Hq * (p.pool.D + 2) * sizeof(float) + (size_t)p.B * sizeof(int2);
+  return (size_t)make_plan(p).parts * p.N * p.Hq * (p.pool.D + 2) * sizeof(float) + (size_t)p.B * sizeof(int2);
 }
 
 hipError_t launch_paged_attn(const PagedProblem& p, const void* q, void* out, float* m, float* l,
                              void* ws, hipStream_t st) {
   const Plan x = make_plan(p);
-  const int64_t prows = (int64_t)x.slots * p.N * p.Hq;
+  const int64_t prows = (int64_t)x.parts * p.N * p.Hq;
   AttnArgs a;
   a.p = p;
   a.q = q;
   a.out = out;
   a.m = m;
   a.l = l;
-  a.direct = x.slots == p.B;
-  const int64_t parts = a.direct ? 0 : prows;
+  a.direct = x.parts == 0;
+  a.parts = x.parts;
   a.po = static_cast<float*>(ws);
-  a.ps = reinterpret_cast<float2*>(a.po + parts * p.pool.D);
-  a.deal = reinterpret_cast<int2*>(a.ps + parts);
+  a.ps = reinterpret_cast<float2*>(a.po + prows * p.pool.D);
+  a.deal = reinterpret_cast<int2*>(a.ps + prows);
   a.group = p.Hq / p.pool.Hkv;
   a.R = p.N * a.group;
   a.slots = x.slots;
   a.units = x.units;
   a.shift = __builtin_ctz((unsigned)p.pool.rows);
   a.sl2 = (float)(1.4426950408889634 / sqrt((double)p.pool.D));
-  auto launch = [&](auto kernel, int threads = 256) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(x.slots * x.units)), dim3(threads), 0, st, a);
+  auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(x.slots * x.units)), dim3(64 * x.waves), 0, st, a);
   };
   const bool once = x.units == p.pool.Hkv;  // the cache is read once
   auto by_dim = [&](auto parts, auto nt) {
     constexpr int P = decltype(parts)::value;
     constexpr bool NT = decltype(nt)::value;
     const bool two = x.tile == 128;
-    if (p.pool.D == 64 && two) launch(paged_stream_kernel<64, true, 1, P, 2, NT>);
-    else if (p.pool.D == 64) launch(paged_stream_kernel<64, true, 1, P, 1, NT>);
-    else if (p.pool.D == 128 && two) launch(paged_stream_kernel<128, true, 1, P, 2, NT>);
-    else if (p.pool.D == 128) launch(paged_stream_kernel<128, true, 1, P, 1, NT>);
-    else if (p.pool.D < 128) launch(paged_stream_kernel<128, false, 1, P, 1, NT>);
-    else launch(paged_stream_kernel<256, false, 1, P, 1, NT>);
+    auto by_waves = [&](auto d, auto vt) {
+      constexpr int DP = decltype(d)::value, VT = decltype(vt)::value;
+      if constexpr (P == 1)
+        if (x.waves == 8) return launch(paged_stream_kernel<DP, true, 1, P, VT, NT, 8>);
+      launch(paged_stream_kernel<DP, true, 1, P, VT, NT, 4>);
+    };
+    auto by_pages = [&](auto d) {
+      if (two) by_waves(d, std::integral_constant<int, 2>{});
+      else by_waves(d, std::integral_constant<int, 1>{});
+    };
+    if (p.pool.D == 64) by_pages(std::integral_constant<int, 64>{});
+    else if (p.pool.D == 128) by_pages(std::integral_constant<int, 128>{});
+    else if (p.pool.D < 128) launch(paged_stream_kernel<128, false, 1, P, 1, NT, 4>);
+    else launch(paged_stream_kernel<256, false, 1, P, 1, NT, 4>);
   };
   auto by_reads = [&](auto parts) {
     if (once) by_dim(parts, std::true_type{});
     else by_dim(parts, std::false_type{});
   };
-  if (x.tiled && p.pool.D == 64) launch(paged_tile_kernel<64>, 512);
-  else if (x.tiled) launch(paged_tile_kernel<128>, 512);
+  if (x.tiled && p.pool.D == 64) launch(paged_tile_kernel<64>);
+  else if (x.tiled) launch(paged_tile_kernel<128>);
   else if (p.dtype == 1) by_reads(std::integral_constant<int, 1>{});
   else by_reads(std::integral_constant<int, 3>{});
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.direct) return e;
   const int64_t rows = (int64_t)p.B * p.N * p.Hq;
-  auto merge = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
+  auto merge = [&](auto kernel, int each) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + each - 1) / each)), dim3(256), 0, st, a);
+  };
+  auto merge_dim = [&](auto t, auto ni) {
+    using T = decltype(t);
+    constexpr int NI = decltype(ni)::value;
+    if (rows < kManyRows) merge(paged_merge_kernel<T, NI, 4>, 1);
+    else merge(paged_merge_kernel<T, NI, 1>, 4);
   };
   auto merge_type = [&](auto t) {
-    using T = decltype(t);
-    if (p.pool.D <= 64) merge(paged_merge_kernel<T, 1>);
-    else if (p.pool.D <= 128) merge(paged_merge_kernel<T, 2>);
-    else merge(paged_merge_kernel<T, 4>);
+    if (p.pool.D <= 64) merge_dim(t, std::integral_constant<int, 1>{});
+    else if (p.pool.D <= 128) merge_dim(t, std::integral_constant<int, 2>{});
+    else merge_dim(t, std::integral_constant<int, 4>{});
   };
   if (p.dtype == 1) merge_type(uint16_t{});
   else merge_type(float{});

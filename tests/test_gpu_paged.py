@@ -548,7 +548,7 @@ def test_refusals(gpu):
         with pytest.raises((ValueError, TypeError)):
             paged.attention(**dict(ok, **kw))
     with pytest.raises(_lib.LcError, match="workspace"):
-        paged.attention(**ok, workspace=gpu.zeros(8, device="cuda"))
+        paged.attention(**ok, workspace=gpu.zeros(1, dtype=gpu.uint8, device="cuda"))
     # nothing to do
     assert paged.append(p, t[:0], past[:0], k[:0], k[:0]) is None
     assert paged.append(p, t, past, k[:, :0], k[:, :0]) is None
