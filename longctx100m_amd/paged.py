@@ -75,34 +75,34 @@ class Pages:
             raise ValueError(f"a pool of shape {tuple(k.shape)}")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.count, self.kv_heads, self.rows, self.head_dim = n, h, rows, d
+        self._device = k.get_device() if k.is_cuda else -1
         self._ptrs = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
 
     def device(self) -> int:
-        if not self.k.is_cuda:
+        if self._device < 0:
             raise ValueError("tensors must live on the GPU (device pointers are passed to HIP)")
-        return self.k.get_device()
+        return self._device
 
 
-def _describe(pages: Pages, table: torch.Tensor, x: torch.Tensor, heads_q: int) -> _lib.Paged:
-    b, n = x.shape[:2]
+def _describe(pages: Pages, table: torch.Tensor, b: int, n: int, heads_q: int, dtype: int) -> _lib.Paged:
     if not isinstance(table, torch.Tensor) or table.dim() != 2:
         raise ValueError("table must be a [batch, pages of a sequence] tensor")
-    if max(b, n, heads_q, table.shape[1]) >= 2 ** 31:
+    width = table.shape[1]
+    if max(b, n, heads_q, width) >= 2 ** 31:
         raise ValueError(f"{n} tokens of {heads_q} heads in {b} sequences: a size is beyond 32 bits")
-    return _lib.Paged(b, n, heads_q, pages.kv_heads, pages.head_dim, _dtype_code(x), pages.count, pages.rows,
-                      table.shape[1], 0)
+    return _lib.Paged(b, n, heads_q, pages.kv_heads, pages.head_dim, dtype, pages.count, pages.rows, width, 0)
 
 
-def _lengths(table, past, counts, b: int, dev: int) -> Tuple[int, int, Optional[int]]:
-    return (_buf(table, (b, table.shape[1]), torch.int32, dev, "table"),
-            _buf(past, (b,), torch.int32, dev, "past"), _opt(counts, (b,), torch.int32, dev, "counts"))
+def _lengths(table, past, counts, desc: _lib.Paged, dev: int) -> Tuple[int, int, Optional[int]]:
+    b = (desc.batch,)
+    return (_buf(table, (desc.batch, desc.table_width), torch.int32, dev, "table"),
+            _buf(past, b, torch.int32, dev, "past"), _opt(counts, b, torch.int32, dev, "counts"))
 
 
-def _rows(t, like: torch.Tensor, heads: int, d: int, dev: int, name: str) -> _lib.Rows:
-    if not isinstance(t, torch.Tensor) or t.dim() != 4 or t.dtype is not like.dtype or \
-            t.get_device() != dev or t.shape != (*like.shape[:2], heads, d):
-        raise ValueError(f"{name} must be a [batch, tokens, {heads}, {d}] tensor of one type on cuda:{dev}")
-    return heads_of(t, name)
+def _rows(t, shape: Tuple[int, ...], dtype, dev: int, name: str) -> _lib.Rows:
+    if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype is not dtype or t.get_device() != dev:
+        raise ValueError(f"{name} must be a {dtype} tensor {shape} on cuda:{dev}")
+    return heads_of(t, shape, name)
 
 
 def append(pages: Pages, table: torch.Tensor, past: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
@@ -121,24 +121,28 @@ def append(pages: Pages, table: torch.Tensor, past: torch.Tensor, k: torch.Tenso
     dev = pages.device()
     if not isinstance(k, torch.Tensor) or k.dim() != 4:
         raise ValueError("k must be a [batch, tokens, heads, head_dim] tensor")
-    d, hkv = pages.head_dim, pages.kv_heads
-    ks, vs = _rows(k, k, hkv, d, dev, "k"), _rows(v, k, hkv, d, dev, "v")
-    hq, qs = 0, None
+    b, n = k.shape[:2]
+    dtype, d = k.dtype, pages.head_dim
+    shape = (b, n, pages.kv_heads, d)
+    ks, vs = _rows(k, shape, dtype, dev, "k"), _rows(v, shape, dtype, dev, "v")
+    hq = 0
+    qs = qp = qo = None
     if q is not None:
         if not isinstance(q, torch.Tensor) or q.dim() != 4:
             raise ValueError("q must be a [batch, tokens, heads, head_dim] tensor")
         hq = q.shape[2]
-        qs = _rows(q, k, hq, d, dev, "q")
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
-        _buf(q_out, q.shape, q.dtype, dev, "q_out")
+        shape = (b, n, hq, d)
+        qs = _rows(q, shape, dtype, dev, "q")
+        if q_out is None:
+            q_out = torch.empty(shape, dtype=dtype, device=q.device)
+        qp, qo = q.data_ptr(), _buf(q_out, shape, dtype, dev, "q_out")
     elif q_out is not None:
         raise ValueError("q_out comes with q")
-    desc = _describe(pages, table, k, hq)
-    if desc.batch == 0 or desc.tokens == 0:
+    desc = _describe(pages, table, b, n, hq, _dtype_code(k))
+    if b == 0 or n == 0:
         return q_out
     _call(dev, _lib.load().lc_paged_append, desc, rotary.on(dev) if rotary is not None else None,
-          *_lengths(table, past, counts, desc.batch, dev), q.data_ptr() if q is not None else None, qs,
-          q_out.data_ptr() if q is not None else None, k.data_ptr(), ks, v.data_ptr(), vs, *pages._ptrs)
+          *_lengths(table, past, counts, desc, dev), qp, qs, qo, k.data_ptr(), ks, v.data_ptr(), vs, *pages._ptrs)
     return q_out
 
 
@@ -152,7 +156,8 @@ def _queries(q, pages: Pages, dev: int) -> None:
 def attention_workspace_bytes(q: torch.Tensor, pages: Pages, table: torch.Tensor) -> int:
     """Workspace of :func:`attention` for queries, pools and tables of these shapes."""
     _queries(q, pages, pages.device())
-    return int(_lib.load().lc_paged_attn_workspace_bytes(_describe(pages, table, q, q.shape[2])))
+    b, n, hq, _ = q.shape
+    return int(_lib.load().lc_paged_attn_workspace_bytes(_describe(pages, table, b, n, hq, _dtype_code(q))))
 
 
 def attention(q: torch.Tensor, pages: Pages, table: torch.Tensor, past: torch.Tensor, *,
@@ -176,11 +181,11 @@ def attention(q: torch.Tensor, pages: Pages, table: torch.Tensor, past: torch.Te
     l = torch.empty(stats, dtype=torch.float32, device=dev) if l is None else l
     ptrs = (q.data_ptr(), *pages._ptrs, _buf(out, q.shape, q.dtype, dev, "out"),
             _buf(m, stats, torch.float32, dev, "m"), _buf(l, stats, torch.float32, dev, "l"))
-    desc = _describe(pages, table, q, hq)
+    desc = _describe(pages, table, b, n, hq, _dtype_code(q))
     if b == 0 or n == 0:
         return out, m, l
     lib = _lib.load()
     workspace = _workspace(workspace, lib.lc_paged_attn_workspace_bytes, desc, dev)
-    _call(dev, lib.lc_paged_attn, desc, *_lengths(table, past, counts, b, dev), *ptrs, workspace.data_ptr(),
+    _call(dev, lib.lc_paged_attn, desc, *_lengths(table, past, counts, desc, dev), *ptrs, workspace.data_ptr(),
           workspace.numel() * workspace.element_size())
     return out, m, l

@@ -149,47 +149,52 @@ class Rotary:
         return c
 
 
-def heads_of(t: torch.Tensor, name: str) -> _lib.Rows:
-    """Strides of a [batch, tokens, heads, head_dim] tensor for the C ABI."""
-    b, n, h, d = t.shape
-    sb, sn, sh, sd = t.stride()
-    if d > 1 and sd != 1:
-        raise ValueError(f"{name} must have contiguous head_dim")
+def heads_of(t: torch.Tensor, shape: Sequence[int], name: str) -> _lib.Rows:
+    """Strides of a tensor of this shape, [batch, tokens, heads, head_dim] or [tokens,
+    heads, head_dim], for the C ABI."""
     # The stride of a dimension of one is never used, and may be anything.
-    return _lib.Rows(sb if b > 1 else 0, sn if n > 1 else 0, sh if h > 1 else 0)
+    if len(shape) == 4:
+        b, n, h, d = shape
+        sb, sn, sh, sd = t.stride()
+        rows = _lib.Rows(sb if b > 1 else 0, sn if n > 1 else 0, sh if h > 1 else 0)
+    else:
+        n, h, d = shape
+        sn, sh, sd = t.stride()
+        rows = _lib.Rows(0, sn if n > 1 else 0, sh if h > 1 else 0)
+    if sd != 1 and d > 1:
+        raise ValueError(f"{name} must have contiguous head_dim")
+    return rows
 
 
 def _turn(x: torch.Tensor, positions: Union[torch.Tensor, int], rotary: Rotary, out: Optional[torch.Tensor],
           inverse: int) -> torch.Tensor:
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise ValueError("tensors must live on the GPU (device pointers are passed to HIP)")
-    if x.dim() not in (3, 4) or x.shape[-1] != rotary.head_dim:
-        raise ValueError(f"rows must be [(batch,) tokens, heads, {rotary.head_dim}], got {tuple(x.shape)}")
-    dev = x.get_device()
+    shape, dev = x.shape, x.get_device()
+    if len(shape) not in (3, 4) or shape[-1] != rotary.head_dim:
+        raise ValueError(f"rows must be [(batch,) tokens, heads, {rotary.head_dim}], got {tuple(shape)}")
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    elif not isinstance(out, torch.Tensor) or out.shape != x.shape or out.dtype is not x.dtype or \
+        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    elif not isinstance(out, torch.Tensor) or out.shape != shape or out.dtype is not x.dtype or \
             out.get_device() != dev:
         raise ValueError("out must have the shape, type and device of the rows")
-    shape = x.shape[:-2]
+    b, n, h = (1, shape[0], shape[1]) if len(shape) == 3 else shape[:3]
     if isinstance(positions, torch.Tensor):
-        if positions.dtype is not torch.int64 or positions.shape != shape or \
+        if positions.dtype is not torch.int64 or positions.shape != shape[:-2] or \
                 positions.get_device() != dev or not positions.is_contiguous():
-            raise ValueError(f"positions must be a contiguous int64 tensor {tuple(shape)} on cuda:{dev}, "
+            raise ValueError(f"positions must be a contiguous int64 tensor {tuple(shape[:-2])} on cuda:{dev}, "
                              "or the first one's number")
         at, pos0 = positions.data_ptr(), 0
     else:
         at, pos0 = None, int(positions)
         if not -2 ** 62 <= pos0 < 2 ** 62:
             raise ValueError(f"the first position is beyond 62 bits: {pos0}")
-    xs, os = (x, out) if x.dim() == 4 else (x.unsqueeze(0), out.unsqueeze(0))
-    b, n, h, _ = xs.shape
     if max(b, n, h) >= 2 ** 31:
-        raise ValueError(f"a size of {tuple(x.shape)} is beyond 32 bits")
+        raise ValueError(f"a size of {tuple(shape)} is beyond 32 bits")
     if h == 0:
         return out
     _call(dev, _lib.load().lc_rotary_apply, rotary.on(dev), _dtype_code(x), b, n, h, at, pos0, inverse,
-          x.data_ptr(), heads_of(xs, "x"), out.data_ptr(), heads_of(os, "out"))
+          x.data_ptr(), heads_of(x, shape, "x"), out.data_ptr(), heads_of(out, shape, "out"))
     return out
 
 
