@@ -12,7 +12,7 @@
 // Keys are [row][dim] in a page, values [dim][row]: the attention's second
 // product wants 16 consecutive keys of one dim in a lane, and gets them with
 // plain 16-byte loads.  A thread therefore takes 16 dims of one row of K, and 4
-// rows by 4 dims of V, so that it can write a dim's four codes as one word.
+// rows by 8 dims of V, so that it can write a dim's four codes as one word.
 #include "e4m3.h"
 #include "paged.h"
 #include "tile32.h"
@@ -66,7 +66,8 @@ __device__ __forceinline__ float group_max(float x, float* buf) {
 struct Block {
   int64_t token0;  // new token in the page's row 0 (negative: an earlier row)
   int lo, hi;      // new rows of the page
-  int64_t unit;    // page * Hkv + head
+  int head, page;  // (a page that is none is looked at after the new rows are on their way)
+  __device__ __forceinline__ int64_t unit(const Pool& p) const { return (int64_t)page * p.Hkv + head; }
 };
 
 // IT: 16 values a thread at a time, so many times (a page and head has rows * D).
@@ -74,9 +75,6 @@ template <typename T, int IT, bool kVec>
 __device__ __forceinline__ void append_keys(const AppendArgs& a, const Block& k, const T* src, int64_t pos0,
                                             float* buf) {
   const int D = a.p.pool.D, units = D / 16;
-  uint8_t* dst = a.p.pool.k + ((k.unit * D) << a.shift);
-  float* scale = a.p.pool.ks + k.unit;
-  const float was = k.lo > 0 ? *scale : __uint_as_float(kScaleMin);
   const int half = a.turns.turns ? a.turns.half : 0;
   const int u = threadIdx.x % units, r0 = threadIdx.x / units, step = 256 / units;
   const bool turned = 8 * u < half;
@@ -96,6 +94,10 @@ __device__ __forceinline__ void append_keys(const AppendArgs& a, const Block& k,
   if (turned)
 #pragma unroll
     for (int e = 0; e < 8; ++e) turns[e] = a.turns.turns[8 * u + e];
+  if (k.page < 0) return;  // the whole workgroup
+  uint8_t* dst = a.p.pool.k + ((k.unit(a.p.pool) * D) << a.shift);
+  float* scale = a.p.pool.ks + k.unit(a.p.pool);
+  const float was = k.lo > 0 ? *scale : __uint_as_float(kScaleMin);
   float top = 0.f;
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
@@ -144,12 +146,9 @@ __device__ __forceinline__ void append_keys(const AppendArgs& a, const Block& k,
 template <typename T, int IT, bool kVec>
 __device__ __forceinline__ void append_values(const AppendArgs& a, const Block& k, const T* src, float* buf) {
   const int D = a.p.pool.D;
-  uint8_t* dst = a.p.pool.v + ((k.unit * D) << a.shift);
-  float* scale = a.p.pool.vs + k.unit;
-  const float was = k.lo > 0 ? *scale : __uint_as_float(kScaleMin);
-  // Four rows from 4 rg, four dims from 4 dg: row groups across the lanes.
-  const int g0 = k.lo / 4, groups = (k.hi + 3) / 4 - g0, items = groups * (D / 4);
-  float x[IT][4][4];  // [row][dim]
+  // Four rows from 4 rg, eight dims from 8 dg: row groups across the lanes.
+  const int g0 = k.lo / 4, groups = (k.hi + 3) / 4 - g0, items = groups * (D / 8);
+  float x[IT][4][8];  // [row][dim]
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
     const int it = threadIdx.x + 256 * i;
@@ -158,14 +157,17 @@ __device__ __forceinline__ void append_values(const AppendArgs& a, const Block& 
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int row = 4 * rg + r;
-        f32x4 w = {0.f, 0.f, 0.f, 0.f};
-        if (row >= k.lo && row < k.hi)
-          w = load_w<T, 4>(src + (k.token0 + row) * a.vs.token + 4 * dg, 0, 4, kVec);
+        if (row >= k.lo && row < k.hi) load8<kVec>(x[i][r], src + (k.token0 + row) * a.vs.token + 8 * dg);
+        else
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[i][r][e] = w[e];
+          for (int e = 0; e < 8; ++e) x[i][r][e] = 0.f;
       }
     }
   }
+  if (k.page < 0) return;  // the whole workgroup
+  uint8_t* dst = a.p.pool.v + ((k.unit(a.p.pool) * D) << a.shift);
+  float* scale = a.p.pool.vs + k.unit(a.p.pool);
+  const float was = k.lo > 0 ? *scale : __uint_as_float(kScaleMin);
   float top = 0.f;
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
@@ -174,7 +176,7 @@ __device__ __forceinline__ void append_values(const AppendArgs& a, const Block& 
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top = fmaxf(top, finite_abs(x[i][r][e]));
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, finite_abs(x[i][r][e]));
   }
   top = group_max(top, buf);
   const float now = fmaxf(was, __uint_as_float(scale_bits(__float_as_uint(top))));
@@ -188,8 +190,8 @@ __device__ __forceinline__ void append_values(const AppendArgs& a, const Block& 
       const int dg = it / groups, rg = g0 + it - dg * groups;
       const int lo = max(k.lo - 4 * rg, 0), hi = min(k.hi - 4 * rg, 4);  // its new rows
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint32_t* at = reinterpret_cast<uint32_t*>(dst + (((int64_t)4 * dg + e) << a.shift) + 4 * rg);
+      for (int e = 0; e < 8; ++e) {
+        uint32_t* at = reinterpret_cast<uint32_t*>(dst + (((int64_t)8 * dg + e) << a.shift) + 4 * rg);
         float c[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) c[r] = finite_or_nan(x[i][r][e]) * inv;
@@ -220,8 +222,12 @@ template <typename T, int IT, bool kVec>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
   __shared__ float2 cs[kTurnTokens * kTurnPairs];
   __shared__ float buf[4];
-  if ((int)blockIdx.x < a.kv_blocks) {
-    int x = blockIdx.x;
+  // The queries first: their workgroups stream, those of the pages mostly wait and
+  // compute, and fill in behind (8,192 tokens of 32/8 heads of 128: 48 us, the pages
+  // first 52.5, both in turn 57.5).
+  const int q_blocks = gridDim.x - a.kv_blocks;
+  if ((int)blockIdx.x >= q_blocks) {
+    int x = blockIdx.x - q_blocks;
     const int what = x & 1;
     x >>= 1;
     const int h = x % a.p.pool.Hkv;
@@ -237,16 +243,15 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
     k.lo = (int)max((int64_t)0, past - row0);
     k.hi = (int)min((int64_t)1 << a.shift, past + (int64_t)n - row0);
     if (k.lo >= k.hi) return;
-    const int page = page_of(a.p.table + (int64_t)b * a.p.width, a.p.width, a.p.pool.pages, at);
-    if (page < 0) return;
-    k.unit = (int64_t)page * a.p.pool.Hkv + h;
+    k.head = h;
+    k.page = page_of(a.p.table + (int64_t)b * a.p.width, a.p.width, a.p.pool.pages, at);
     if (what == 0)
       append_keys<T, IT, kVec>(a, k, static_cast<const T*>(a.k) + b * a.ks.seq + h * a.ks.head, row0, buf);
     else
-      append_values<T, IT, kVec>(a, k, static_cast<const T*>(a.v) + b * a.vs.seq + h * a.vs.head, buf);
+      append_values<T, (IT + 1) / 2, kVec>(a, k, static_cast<const T*>(a.v) + b * a.vs.seq + h * a.vs.head, buf);
     return;
   }
-  const int64_t row0 = (int64_t)(blockIdx.x - a.kv_blocks) * a.group, rows = (int64_t)a.p.B * a.p.N;
+  const int64_t row0 = (int64_t)blockIdx.x * a.group, rows = (int64_t)a.p.B * a.p.N;
   const int n = (int)min((int64_t)a.group, rows - row0);
   turn_tokens<T, kVec>(
       cs, a.turns, n, a.p.Hq, a.p.pool.D, a.qs.head, a.p.pool.D, true, 1,
