@@ -43,7 +43,9 @@ hipError_t launch_paged_attn(const PagedProblem& p, const void* q, void* out, fl
 
 // New tokens of a sequence; 0 where there is no sequence.
 __device__ __forceinline__ int new_tokens(const int32_t* counts, int N, int b, int past) {
-  return past < 0 ? 0 : counts == nullptr ? N : max(0, min(counts[b], N));
+  int n = N;
+  if (counts != nullptr) n = max(0, min(counts[b], N));  // (read along with past, not after it)
+  return past < 0 ? 0 : n;
 }
 
 }  // namespace lc

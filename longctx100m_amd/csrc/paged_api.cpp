@@ -120,6 +120,8 @@ int check_paged(const lc_paged_t* c, bool queries) {
   if (queries && c->heads_q % c->heads_kv != 0)
     return set_error(LC_ERR_INVALID, "heads_q (%d) must be a multiple of heads_kv (%d)", c->heads_q,
                      c->heads_kv);
+  if (queries && c->heads_q / c->heads_kv > 1 << 16)
+    return set_error(LC_ERR_UNSUPPORTED, "more than 2^16 query heads share a KV head");
   if (int rc = check_dtype(c->dtype)) return rc;
   if (c->flags) return set_error(LC_ERR_INVALID, "unknown flag bits 0x%x", c->flags);
   if (c->head_dim % 16 != 0 || c->head_dim > 256)

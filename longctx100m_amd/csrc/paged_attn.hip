@@ -60,6 +60,22 @@ __device__ __forceinline__ int keys_of(const AttnArgs& a, int b) {
   return n > 0 ? (int)min((int64_t)past + n, (int64_t)a.p.width << a.shift) : 0;
 }
 
+// Tokens and heads of a block of query rows from r0 on: row r0 + x is token (r0 + x)
+// / group.  One division for the block, then (x < 2^17, group <= 2^16) a float
+// product that is off by less than half of 1 / group.
+struct RowMap {
+  int token0, rem, group;
+  float inv;
+  __device__ __forceinline__ RowMap(int r0, int group_) : group(group_) {
+    token0 = __builtin_amdgcn_readfirstlane(r0 / group);
+    rem = r0 - token0 * group;
+    inv = 1.f / (float)group;
+  }
+  __device__ __forceinline__ int step(int x) const { return (int)(((float)(rem + x) + 0.5f) * inv); }
+  __device__ __forceinline__ int token(int x) const { return token0 + step(x); }
+  __device__ __forceinline__ int head(int x) const { return rem + x - step(x) * group; }
+};
+
 __device__ __forceinline__ int64_t partial_row(const AttnArgs& a, int r, int hk, int part) {
   return ((int64_t)(r / a.group) * a.p.Hq + hk * a.group + r % a.group) * a.parts + part;
 }
@@ -124,10 +140,10 @@ __device__ __forceinline__ void store_vec4(T* p, const f32x4& r) {
 // 1 / l for a row's sum: 0 for a row that saw nothing, NaN for one that saw NaN.
 __device__ __forceinline__ float inverse_sum(float l) { return l > 0.f ? 1.f / l : l; }
 
-// The statistics of query row r (token r / group) of sequence b and KV head hk:
-// its maximum in log2 units, and its sum.
-__device__ __forceinline__ void store_stats(const AttnArgs& a, int b, int hk, int r, float top, float l) {
-  const int64_t si = ((int64_t)b * a.p.Hq + hk * a.group + r % a.group) * a.p.N + r / a.group;
+// The statistics of head h of token i of sequence b: its maximum in log2 units, and
+// its sum.
+__device__ __forceinline__ void store_stats(const AttnArgs& a, int b, int h, int i, float top, float l) {
+  const int64_t si = ((int64_t)b * a.p.Hq + h) * a.p.N + i;
   if (a.m) a.m[si] = top == -INFINITY ? top : top * kLn2;
   if (a.l) a.l[si] = l;
 }
@@ -233,44 +249,49 @@ __global__ __launch_bounds__(64 * W, DP * PARTS > 192 || W > 4 ? 1 : 2) void pag
   const int count = new_tokens(a.p.counts, a.p.N, s.b, past);
   const int32_t* table = a.p.table + (int64_t)s.b * a.p.width;
   // Tokens of this row block, and the rows that the last of them sees.
-  const int first = rb * kRows / a.group, last = min((rb * kRows + kRows - 1) / a.group, count - 1);
+  const RowMap map(rb * kRows, a.group);
+  const int first = map.token0, last = min(map.token(kRows - 1), count - 1);
   const int k1 = min(s.k1, past + last + 1);  // (no token: last < first, and nothing is walked)
   const int all = last >= first && k1 > s.k0 ? (k1 - s.k0 + 63) / 64 : 0;
   const int per = (all + W * VT - 1) / (W * VT) * VT;
   const int t0 = s.k0 / 64 + min(wave * per, all), t1 = s.k0 / 64 + min((wave + 1) * per, all);
   const int clear = past + first + 1;  // keys that all rows see
-  bool strange = false;                // NaN among the values of tiles beyond
+  bool strange = false;                // NaN among the values that some rows see only
+
+  PageRun run;
+  if (t0 < t1) run.look(a, table, t0, k1);
 
   // Rows of this lane: c of each 16; the keys they see.
   bf16x8 q[PARTS][NB][2 * KJ];
   int lim[NB];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    const int r = rb * kRows + 16 * nb + c, i = r / a.group;
-    const bool ok = r < a.R && i < count;
+    const int x = 16 * nb + c, i = map.token(x);
+    const bool ok = rb * kRows + x < a.R && i < count;
     lim[nb] = ok ? past + i + 1 : 0;
-    const int64_t qi = ok ? ((int64_t)s.b * a.p.N + i) * a.p.Hq + hk * a.group + r % a.group : 0;
+    const int64_t qi = ok ? ((int64_t)s.b * a.p.N + i) * a.p.Hq + hk * a.group + map.head(x) : 0;
     const T* qp = static_cast<const T*>(a.q) + qi * D;
 #pragma unroll
     for (int j = 0; j < 2 * KJ; ++j) {
       const int d = 64 * (j >> 1) + 16 * g + 8 * (j & 1);
-      f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
-      if (ok && (EXACT || d < D)) {
-        lo = load_vec<T, 4>(qp + d);
-        hi = load_vec<T, 4>(qp + d + 4);
-      }
-      bf16x8 x[PARTS];
-      split8<PARTS>(lo, hi, x);
+      const bool on = ok && (EXACT || d < D);
+      if constexpr (PARTS == 1) {
+        q[0][nb][j] = bf16x8{};
+        if (on) q[0][nb][j] = *reinterpret_cast<const bf16x8*>(qp + d);
+      } else {
+        f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+        if (on) {
+          lo = load_vec<T, 4>(qp + d);
+          hi = load_vec<T, 4>(qp + d + 4);
+        }
+        bf16x8 y[PARTS];
+        split8<PARTS>(lo, hi, y);
 #pragma unroll
-      for (int p = 0; p < PARTS; ++p) q[p][nb][j] = x[p];
+        for (int p = 0; p < PARTS; ++p) q[p][nb][j] = y[p];
+      }
     }
   }
-
-  PageRun run;
-  if (t0 < t1) {
-    run.look(a, table, t0, k1);
-    run.scales(a, hk);
-  }
+  if (t0 < t1) run.scales(a, hk);
   const int64_t head_bytes = (int64_t)D << a.shift;
   uint4 kr[4][KJ], vr[VT][DB];
   auto base = [&](const uint8_t* p, int page) {
@@ -380,13 +401,14 @@ __global__ __launch_bounds__(64 * W, DP * PARTS > 192 || W > 4 ? 1 : 2) void pag
     const bool edge = 64 * (t + 1) > clear;
     if (edge || __any(page < 0)) {
       const int left = page < 0 ? 0 : k1 - (64 * t + 16 * g);  // values that some row sees
+      if (edge && last > first) {
 #pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        if (edge) {
-          strange |= clean_values(vr[V][db], left);
-        } else if (left <= 0) {
-          vr[V][db] = make_uint4(0u, 0u, 0u, 0u);
-        }
+        for (int db = 0; db < DB; ++db) strange |= clean_values(vr[V][db], left);
+      } else {  // all rows see the same
+        const uint32_t m[4] = {low_bytes(left), low_bytes(left - 4), low_bytes(left - 8), low_bytes(left - 12)};
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+          vr[V][db] = make_uint4(vr[V][db].x & m[0], vr[V][db].y & m[1], vr[V][db].z & m[2], vr[V][db].w & m[3]);
       }
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
@@ -476,8 +498,7 @@ __global__ __launch_bounds__(64 * W, DP * PARTS > 192 || W > 4 ? 1 : 2) void pag
   const int chunks = D / 4;  // of a row
   for (int it = tid; it < kRows * chunks; it += 64 * W) {
     const int rr = it / chunks, d = 4 * (it - rr * chunks);
-    const int r = rb * kRows + rr;
-    if (r >= a.R) break;
+    if (rb * kRows + rr >= a.R) break;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     float L = 0.f, M = -INFINITY;
 #pragma unroll
@@ -486,13 +507,14 @@ __global__ __launch_bounds__(64 * W, DP * PARTS > 192 || W > 4 ? 1 : 2) void pag
       L += lsm[w][rr];
       M = fmaxf(M, msm[w][rr]);
     }
+    const int i = map.token(rr), h = hk * a.group + map.head(rr);
     if (a.direct) {
-      const int64_t qi = ((int64_t)s.b * a.p.N + r / a.group) * a.p.Hq + hk * a.group + r % a.group;
-      const bool there = r / a.group < count;
-      store_vec4(static_cast<T*>(a.out) + qi * D + d, there ? acc * inverse_sum(L) : f32x4{0.f, 0.f, 0.f, 0.f});
-      if (d == 0) store_stats(a, s.b, hk, r, there ? M : -INFINITY, there ? L : 0.f);
+      const bool there = i < count;
+      store_vec4(static_cast<T*>(a.out) + (((int64_t)s.b * a.p.N + i) * a.p.Hq + h) * D + d,
+                 there ? acc * inverse_sum(L) : f32x4{0.f, 0.f, 0.f, 0.f});
+      if (d == 0) store_stats(a, s.b, h, i, there ? M : -INFINITY, there ? L : 0.f);
     } else {
-      const int64_t pr = partial_row(a, r, hk, s.segment);
+      const int64_t pr = ((int64_t)i * a.p.Hq + h) * a.parts + s.segment;
       *reinterpret_cast<f32x4*>(a.po + pr * D + d) = acc;
       if (d == 0) a.ps[pr] = make_float2(M, L);
     }
@@ -816,7 +838,7 @@ __global__ __launch_bounds__(512, 1) void paged_tile_kernel(AttnArgs a) {
       else *reinterpret_cast<f32x4*>(a.po + pr * D + at) = x;
     }
   if (hh == 0) {
-    if (a.direct) store_stats(a, s.b, hk, r, ok ? mrun : -INFINITY, ok ? l : 0.f);
+    if (a.direct) store_stats(a, s.b, hk * a.group + r % a.group, i, ok ? mrun : -INFINITY, ok ? l : 0.f);
     else a.ps[pr] = make_float2(mrun, l);
   }
 }
@@ -892,7 +914,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a) {
 #pragma unroll
   for (int x = 0; x < NI; ++x)
     if (u == 0 && j + 16 * x < nch) store_vec4<T>(out + 4 * (j + 16 * x), acc[x] * inv);
-  if (lane == 0) store_stats(a, b, h / a.group, i * a.group + h % a.group, top, l);
+  if (lane == 0) store_stats(a, b, h, i, top, l);
 }
 
 // ------------------------------------------------------------------- host --
