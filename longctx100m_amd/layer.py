@@ -24,7 +24,9 @@ import torch
 
 from . import _lib
 from . import cache as kv
+from . import paged
 from . import ring_attention as ra
+from . import rotary as rot
 from .ring_attention import _dtype_code, _stream
 
 
@@ -616,6 +618,133 @@ class BoundedCache:
             kv.evict(k, v, w, lens, budget, sinks=sinks, recent=recent, positions=p, kept=kept,
                      ends=ends, weights_out=w, positions_out=p, workspace=ws)
         self.past = self.kept = budget
+
+
+# ------------------------------------------- many sequences, paged 8-bit caches --
+
+def layer_extend_paged(x: torch.Tensor, w: Dict[str, torch.Tensor], cfg: ModelConfig,
+                       rotary: rot.Rotary, pages: paged.Pages, table: torch.Tensor,
+                       past: torch.Tensor, counts: Optional[torch.Tensor] = None,
+                       residual: Optional[torch.Tensor] = None,
+                       workspace: Optional[torch.Tensor] = None):
+    """One decoder layer for N new tokens of each of B sequences (x [B * N, hidden],
+    a sequence's tokens together): their K and V are appended to the sequences'
+    pages and each token attends to its sequence up to itself.  ``table`` [B, W],
+    ``past`` [B] and ``counts`` [B] as in ``paged``; rows of tokens from counts on are
+    padding.  Returns (x_after_attention, mlp_out) as layer_decode."""
+    b = table.shape[0]
+    n = x.shape[0] // b
+    d, hq, hkv = cfg.head_dim, cfg.num_heads, cfg.num_key_value_heads
+    if x.shape[0] != b * n:
+        raise ValueError(f"{x.shape[0]} rows are no {b} sequences of as many tokens")
+    if residual is not None:
+        xin = torch.empty_like(x)
+        h = rmsnorm(x, w["norm1"], cfg.rms_norm_eps, residual=residual, residual_out=xin)
+    else:
+        xin = x
+        h = rmsnorm(x, w["norm1"], cfg.rms_norm_eps)
+    q, k, v = linear(h, w["wqkv"]).view(b, n, hq + 2 * hkv, d).split((hq, hkv, hkv), 2)
+    q = paged.append(pages, table, past, k, v, counts=counts, rotary=rotary, q=q)
+    attn, _, _ = paged.attention(q, pages, table, past, counts=counts, workspace=workspace)
+    ao = linear(attn.view(b * n, hq * d), w["wo"])
+    x2 = torch.empty_like(x)
+    h2 = rmsnorm(xin, w["norm2"], cfg.rms_norm_eps, residual=ao, residual_out=x2)
+    gu = linear(h2, w["wgu"])
+    inter = cfg.intermediate_size
+    a = swiglu(gu[:, :inter], gu[:, inter:])
+    return x2, linear(a, w["wd"])
+
+
+class PagedCache:
+    """The caches of a model's layers for many sequences, which take pages of a
+    common pool as they grow, in 8 bits (``paged``):
+
+        c = PagedCache(cfg, pages=4096, sequences=32, device="cuda")
+        a, b = c.open(), c.open()
+        logits = c.extend([a, b], [prompt_a, prompt_b], weights)  # [2, vocab]
+        logits = c.extend([a, b], [next_a, next_b], weights)      # one token each, or drafts
+        c.close(a)                                                # its pages are free again
+
+    ``rows[slot]`` tokens of a sequence are held.  ``rotary`` is the model's rotation,
+    without one that of the config's rope_theta and rope_scaling with the
+    reference's frequencies.  Calls run on one stream: a page that a closed
+    sequence leaves is written again without a wait."""
+
+    def __init__(self, cfg: ModelConfig, pages: int, sequences: int, device, *, page_rows: int = 64,
+                 rotary: Optional[rot.Rotary] = None):
+        if pages <= 0 or sequences <= 0:
+            raise ValueError("a cache has pages and sequences")
+        self.cfg, self.page_rows = cfg, page_rows
+        self.pools = [paged.Pages(pages, page_rows, cfg.num_key_value_heads, cfg.head_dim, device)
+                      for _ in range(cfg.num_layers)]
+        self.rotary = rotary if rotary is not None else rot.Rotary.of(
+            rope_params(cfg.head_dim, cfg.rope_theta, cfg.rope_scaling), device)
+        self.rows = [0] * sequences
+        self._device = device
+        self._pages: List[Optional[List[int]]] = [None] * sequences  # None: the slot is free
+        self._free = list(range(pages - 1, -1, -1))
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def open(self) -> int:
+        """A slot for a new sequence."""
+        for slot, held in enumerate(self._pages):
+            if held is None:
+                self._pages[slot], self.rows[slot] = [], 0
+                return slot
+        raise ValueError(f"all {len(self._pages)} sequences are open")
+
+    def _held(self, slot: int) -> List[int]:
+        if not 0 <= slot < len(self._pages) or self._pages[slot] is None:
+            raise ValueError(f"no sequence is open in slot {slot}")
+        return self._pages[slot]
+
+    def close(self, slot: int) -> None:
+        """Ends a sequence; its pages go back to the pool."""
+        self._free += reversed(self._held(slot))
+        self._pages[slot], self.rows[slot] = None, 0
+
+    def extend(self, slots: Sequence[int], ids: Sequence[torch.Tensor], weights: Dict,
+               workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Appends the tokens ids[i] (1-D, any number but none) to the sequence in
+        slots[i], each at its next positions; the logits [len(slots), vocab] of each
+        one's last.  A call that fails leaves slots, rows and free pages as they were."""
+        slots, counts = list(slots), [t.numel() for t in ids]
+        if not slots or len(slots) != len(counts) or len(set(slots)) < len(slots):
+            raise ValueError("extend takes sequences, each once, and tokens for each")
+        if min(counts) == 0 or any(t.dim() != 1 for t in ids):
+            raise ValueError("a sequence is extended by a 1-D tensor of tokens, one at least")
+        held = [self._held(slot) for slot in slots]
+        past = [self.rows[slot] for slot in slots]
+        need = [-(-(p + c) // self.page_rows) - len(h) for p, c, h in zip(past, counts, held)]
+        if sum(need) > len(self._free):
+            raise ValueError(f"{sum(need)} pages are needed, {len(self._free)} are free")
+        taken = self._free[len(self._free) - sum(need):][::-1]
+        tables, at = [], 0
+        for h, k in zip(held, need):
+            tables.append(h + taken[at:at + k])
+            at += k
+        width = max(len(t) for t in tables)
+        i32 = dict(dtype=torch.int32, device=self._device)
+        table = torch.tensor([t + [-1] * (width - len(t)) for t in tables], **i32)
+        tpast, tcounts = torch.tensor(past, **i32), torch.tensor(counts, **i32)
+        n = max(counts)
+        padded = torch.nn.utils.rnn.pad_sequence(list(ids), batch_first=True)
+        x = torch.nn.functional.embedding(padded.reshape(-1), weights["embed"])
+        res = None
+        for lw, pool in zip(weights["layers"], self.pools):
+            x, res = layer_extend_paged(x, lw, self.cfg, self.rotary, pool, table, tpast,
+                                        tcounts if min(counts) < n else None, residual=res,
+                                        workspace=workspace)
+        last = torch.arange(len(slots), device=self._device) * n + tcounts.long() - 1
+        h = rmsnorm(x[last], weights["final_norm"], self.cfg.rms_norm_eps, residual=res[last])
+        logits = linear(h, weights["lm_head"])
+        del self._free[len(self._free) - sum(need):]  # every layer has its rows
+        for slot, t, p, c in zip(slots, tables, past, counts):
+            self._pages[slot], self.rows[slot] = t, p + c
+        return logits
 
 
 def init_model_weights(cfg: ModelConfig, gen: torch.Generator, device, dtype=torch.bfloat16,

@@ -1,0 +1,111 @@
+"""What layer.PagedCache decides on the host: slots, pages, tables, and what a
+refused or failing call leaves behind.  The layers are replaced by a recorder, so
+this runs without a GPU."""
+
+import pytest
+import torch
+
+from longctx100m_amd import layer as ly
+from longctx100m_amd import rotary as rot
+
+CFG = ly.ModelConfig(hidden_size=64, num_heads=4, num_key_value_heads=2, intermediate_size=64, num_layers=2,
+                     vocab_size=50)
+
+
+@pytest.fixture
+def cache(monkeypatch):
+    calls = []
+
+    def layer(x, w, cfg, rotary, pages, table, past, counts, residual=None, workspace=None):
+        if w.get("fail"):
+            raise RuntimeError("a layer failed")
+        calls.append((x.shape[0], table.tolist(), past.tolist(), None if counts is None else counts.tolist()))
+        return x + 1, x * 2
+
+    monkeypatch.setattr(ly, "layer_extend_paged", layer)
+    monkeypatch.setattr(ly, "rmsnorm", lambda x, w, eps, residual=None: x + residual)
+    c = ly.PagedCache(CFG, pages=6, sequences=3, device="cpu", page_rows=16)
+    weights = {"embed": torch.randn(50, 64), "lm_head": torch.randn(50, 64), "final_norm": torch.ones(64),
+               "layers": [{}, {}]}
+    return c, weights, calls
+
+
+def ids(n):
+    return torch.arange(n) % 50
+
+
+def test_pages_follow_the_rows(cache):
+    c, w, calls = cache
+    a, b = c.open(), c.open()
+    assert (a, b) == (0, 1) and c.free_pages == 6
+    out = c.extend([a, b], [ids(16), ids(3)], w)
+    assert out.shape == (2, 50) and c.rows[:2] == [16, 3] and c.free_pages == 4
+    assert len(calls) == 2  # layers
+    rows, table, past, counts = calls[0]
+    assert rows == 32 and past == [0, 0] and counts == [16, 3]
+    assert len({x for t in table for x in t}) == 2 and len(table[0]) == 1
+    c.extend([b, a], [ids(1), ids(1)], w)  # a's next page
+    rows, table, past, counts = calls[-1]
+    assert past == [3, 16] and counts is None and table[0][1] == -1
+    assert table[1][0] == calls[0][1][0][0] and table[0][0] == calls[0][1][1][0]
+    assert c.rows[:2] == [17, 4] and c.free_pages == 3
+    # the logits are those of the last tokens: each layer adds one, the last residual twice x
+    x = w["embed"][ids(1)]
+    assert torch.allclose(c.extend([b], [ids(1)], w), (x + 2 + 2 * (x + 1)) @ w["lm_head"].t(), atol=1e-5)
+
+
+def test_last_tokens_of_a_padded_batch(cache):
+    c, w, _ = cache
+    a, b = c.open(), c.open()
+    out = c.extend([a, b], [ids(5) + 7, ids(2) + 20], w)
+    x = w["embed"][[11, 21]]
+    assert torch.allclose(out, (x + 2 + 2 * (x + 1)) @ w["lm_head"].t(), atol=1e-5)
+
+
+def test_closed_sequences_give_their_pages_back(cache):
+    c, w, _ = cache
+    a = c.open()
+    c.extend([a], [ids(90)], w)
+    assert c.free_pages == 0
+    with pytest.raises(ValueError, match="pages are needed"):
+        c.extend([a], [ids(7)], w)
+    assert c.rows[a] == 90
+    c.extend([a], [ids(6)], w)  # the last page's rows
+    c.close(a)
+    assert c.free_pages == 6 and c.rows[a] == 0
+    for bad in (a, 1, 3, -1):
+        with pytest.raises(ValueError, match="no sequence"):
+            c.close(bad)
+    assert [c.open() for _ in range(3)] == [0, 1, 2]
+    with pytest.raises(ValueError, match="all 3"):
+        c.open()
+
+
+def test_refused_and_failing_calls_leave_everything(cache):
+    c, w, calls = cache
+    a, b = c.open(), c.open()
+    c.extend([a], [ids(20)], w)
+    before = (list(c.rows), list(c._free), [None if p is None else list(p) for p in c._pages], len(calls))
+    for slots, toks in (([], []), ([a, a], [ids(1), ids(1)]), ([a], [ids(1), ids(1)]), ([a], [ids(0)]),
+                        ([a], [ids(4).view(2, 2)]), ([2], [ids(1)]), ([a, b], [ids(1), ids(80)])):
+        with pytest.raises(ValueError):
+            c.extend(slots, toks, w)
+    bad = dict(w, layers=[{}, {"fail": True}])
+    with pytest.raises(RuntimeError, match="a layer failed"):
+        c.extend([a, b], [ids(20), ids(5)], bad)
+    after = (list(c.rows), list(c._free), [None if p is None else list(p) for p in c._pages])
+    assert after == before[:3]
+    c.extend([b, a], [ids(1), ids(1)], w)
+    assert c.rows[:2] == [21, 1]
+    held = [x for p in c._pages if p for x in p] + c._free
+    assert sorted(held) == list(range(6))
+
+
+def test_sizes(monkeypatch):
+    for kw in (dict(pages=0, sequences=1), dict(pages=1, sequences=0), dict(pages=-1, sequences=1)):
+        with pytest.raises(ValueError):
+            ly.PagedCache(CFG, device="cpu", **kw)
+    r = rot.Rotary(16, 100.0, device="cpu")
+    c = ly.PagedCache(CFG, 2, 1, "cpu", rotary=r)
+    assert c.rotary is r and len(c.pools) == 2 and c.pools[0].rows == 64
+    assert ly.PagedCache(CFG, 2, 1, "cpu").rotary.inv_freq[0] == 1.0
