@@ -50,12 +50,17 @@ struct AttnArgs {
   int parts;
   int shift;         // log2 of a page's rows
   bool direct;       // a slot is a whole sequence: results in place of partials
+  bool early;        // and its table one run of pages, read beside its length
   float sl2;
 };
 
+// The rows before a sequence's new tokens, negative: none.  (A table has 2^30 rows at
+// most, so more are as many.)
+__device__ __forceinline__ int past_of(const int32_t* past, int b) { return min(past[b], 1 << 30); }
+
 // Keys of a sequence: its past and its new tokens, as far as the page table goes.
 __device__ __forceinline__ int keys_of(const AttnArgs& a, int b) {
-  const int past = a.p.past[b];
+  const int past = past_of(a.p.past, b);
   const int n = new_tokens(a.p.counts, a.p.N, b, past);
   return n > 0 ? (int)min((int64_t)past + n, (int64_t)a.p.width << a.shift) : 0;
 }
@@ -169,6 +174,10 @@ struct PageRun {
       nvs = a.p.pool.vs[u];
     }
   }
+  // Of a run that was looked up without an end: what lies at or behind it.
+  __device__ __forceinline__ void cut(int end) {
+    if (16 * (int)(threadIdx.x & 63) >= end) next = -1;
+  }
   __device__ __forceinline__ void turn() {
     page = next;
     ks = nks;
@@ -216,19 +225,22 @@ __device__ __forceinline__ uint4 load16(const uint8_t* p) {
   return make_uint4(x[0], x[1], x[2], x[3]);
 }
 
-// Bound by the stream of the cache.  Every wave holds all of the workgroup's 16 * NB
-// rows and walks a run of the segment's tiles; the W waves meet in LDS.
+// Bound by the stream of the cache.  Every wave holds all of the workgroup's 16 rows
+// and walks a run of the segment's tiles; the W waves meet in LDS.  (More rows are
+// blocks of 16, whose second finds in L2 what the first has read: with 32 rows a
+// wave 64 rows over 16,000 keys take 31 us for 28, over 131,072 106 for 115, and 64
+// of them do not fit the registers.)
 // A load of a wave should take whole cache lines: half a line at a time, its other
 // half with the next load, costs a tenth of the stream.  So of a key of 128 bytes
 // eight lanes take one half and eight the other, two loads take twice as many
 // keys, and the lanes swap; the same for V in pages of 128 rows (VT = 2), a dim's
 // line of which is two tiles' keys.
 // DP: head_dim, rounded up to 64, 128 or 256 unless EXACT.
-template <int DP, bool EXACT, int NB, int PARTS, int VT, bool NT, int W>
+template <int DP, bool EXACT, int PARTS, int VT, bool NT, int W>
 __global__ __launch_bounds__(64 * W, DP * PARTS > 192 || W > 4 ? 1 : 2) void paged_stream_kernel(AttnArgs a) {
   typedef typename std::conditional<PARTS == 1, uint16_t, float>::type T;
   constexpr int KJ = DP / 64, DB = DP / 16;  // 16-byte pieces of a key a lane takes; 16-dim blocks
-  constexpr int kRows = 16 * NB, kPitch = DP + 4;
+  constexpr int kRows = 16, kPitch = DP + 4;
   constexpr bool kLines = EXACT && DP == 128;
   static_assert(VT == 1 || EXACT, "two tiles of V at once");
   __shared__ __attribute__((aligned(16))) float part[W * kRows * kPitch];
@@ -241,285 +253,262 @@ __global__ __launch_bounds__(64 * W, DP * PARTS > 192 || W > 4 ? 1 : 2) void pag
   const int hk = unit % pool.Hkv;
   const int rb = unit / pool.Hkv;
   const int D = EXACT ? DP : pool.D;
+  PageRun run;
+  if (a.early) run.look(a, a.p.table + (int64_t)slot * a.p.width, 0, 1 << 30);
   auto keys = [&](int b) { return keys_of(a, b); };
   for (Spans<64 * VT, decltype(keys)> s(keys, a.p.B, a.slots, a.direct, W, a.deal, slot); s.next();) {
-  // (opaque: what follows from it is formed in each segment, not kept in registers)
-  const int tid = opaque(threadIdx.x), lane = tid & 63, c = lane & 15, g = lane >> 4;
-  const int past = a.p.past[s.b];
-  const int count = new_tokens(a.p.counts, a.p.N, s.b, past);
-  const int32_t* table = a.p.table + (int64_t)s.b * a.p.width;
-  // Tokens of this row block, and the rows that the last of them sees.
-  const RowMap map(rb * kRows, a.group);
-  const int first = map.token0, last = min(map.token(kRows - 1), count - 1);
-  const int k1 = min(s.k1, past + last + 1);  // (no token: last < first, and nothing is walked)
-  const int all = last >= first && k1 > s.k0 ? (k1 - s.k0 + 63) / 64 : 0;
-  const int per = (all + W * VT - 1) / (W * VT) * VT;
-  const int t0 = s.k0 / 64 + min(wave * per, all), t1 = s.k0 / 64 + min((wave + 1) * per, all);
-  const int clear = past + first + 1;  // keys that all rows see
-  bool strange = false;                // NaN among the values that some rows see only
+    // (opaque: what follows from it is formed in each segment, not kept in registers)
+    const int tid = opaque(threadIdx.x), lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int past = past_of(a.p.past, s.b);
+    const int count = new_tokens(a.p.counts, a.p.N, s.b, past);
+    const int32_t* table = a.p.table + (int64_t)s.b * a.p.width;
+    // Tokens of this row block, and the rows that the last of them sees.
+    const RowMap map(rb * kRows, a.group);
+    const int first = map.token0, last = min(map.token(kRows - 1), count - 1);
+    const int k1 = min(s.k1, past + last + 1);  // (no token: last < first, and nothing is walked)
+    const int all = last >= first && k1 > s.k0 ? (k1 - s.k0 + 63) / 64 : 0;
+    const int per = (all + W * VT - 1) / (W * VT) * VT;
+    const int t0 = s.k0 / 64 + min(wave * per, all), t1 = s.k0 / 64 + min((wave + 1) * per, all);
+    const int tb = a.early ? 0 : t0;     // the first tile of the page run
+    const int clear = past + first + 1;  // keys that all rows see
+    bool strange = false;                // NaN among the values that some rows see only
+    if (a.early) run.cut(k1);
+    else if (t0 < t1) run.look(a, table, t0, k1);
 
-  PageRun run;
-  if (t0 < t1) run.look(a, table, t0, k1);
+    // The lane's row: c; the keys it sees.
+    const int qtok = map.token(c);
+    const bool ok = rb * kRows + c < a.R && qtok < count;
+    const int lim = ok ? past + qtok + 1 : 0;
+    bf16x8 q[PARTS][2 * KJ];
+    {
+      const int64_t qi = ok ? ((int64_t)s.b * a.p.N + qtok) * a.p.Hq + hk * a.group + map.head(c) : 0;
+      const T* qp = static_cast<const T*>(a.q) + qi * D;
+#pragma unroll
+      for (int j = 0; j < 2 * KJ; ++j) {
+        const int d = 64 * (j >> 1) + 16 * g + 8 * (j & 1);
+        const bool on = ok && (EXACT || d < D);
+        if constexpr (PARTS == 1) {
+          q[0][j] = bf16x8{};
+          if (on) q[0][j] = *reinterpret_cast<const bf16x8*>(qp + d);
+        } else {
+          f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+          if (on) {
+            lo = load_vec<T, 4>(qp + d);
+            hi = load_vec<T, 4>(qp + d + 4);
+          }
+          bf16x8 y[PARTS];
+          split8<PARTS>(lo, hi, y);
+#pragma unroll
+          for (int p = 0; p < PARTS; ++p) q[p][j] = y[p];
+        }
+      }
+    }
+    if (t0 < t1) run.scales(a, hk);
 
-  // Rows of this lane: c of each 16; the keys they see.
-  bf16x8 q[PARTS][NB][2 * KJ];
-  int lim[NB];
+    const int64_t head_bytes = (int64_t)D << a.shift;
+    const int page_mask = (1 << a.shift) - 1;
+    uint4 kr[4][KJ], vr[VT][DB];
+    auto base = [&](const uint8_t* p, int page) {
+      return p + ((int64_t)max(page, 0) * pool.Hkv + hk) * head_bytes;
+    };
+    auto kload = [&](int t) {
+      const int x = 4 * (t - tb & 15);
+      if constexpr (kLines) {
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    const int x = 16 * nb + c, i = map.token(x);
-    const bool ok = rb * kRows + x < a.R && i < count;
-    lim[nb] = ok ? past + i + 1 : 0;
-    const int64_t qi = ok ? ((int64_t)s.b * a.p.N + i) * a.p.Hq + hk * a.group + map.head(x) : 0;
-    const T* qp = static_cast<const T*>(a.q) + qi * D;
+        for (int i = 0; i < 2; ++i) {
+          const int gk = 2 * i + (c >> 2 & 1);
+          const int row = 64 * t + 16 * gk & page_mask;
+          const uint8_t* p =
+              base(pool.k, __shfl(run.page, x + gk, 64)) + (row + (c & 3)) * D + 64 * (c >> 3) + 16 * g;
 #pragma unroll
-    for (int j = 0; j < 2 * KJ; ++j) {
-      const int d = 64 * (j >> 1) + 16 * g + 8 * (j & 1);
-      const bool on = ok && (EXACT || d < D);
-      if constexpr (PARTS == 1) {
-        q[0][nb][j] = bf16x8{};
-        if (on) q[0][nb][j] = *reinterpret_cast<const bf16x8*>(qp + d);
+          for (int mb = 0; mb < 4; ++mb) kr[mb][i] = load16<NT>(p + 4 * mb * D);
+        }
       } else {
-        f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
-        if (on) {
-          lo = load_vec<T, 4>(qp + d);
-          hi = load_vec<T, 4>(qp + d + 4);
-        }
-        bf16x8 y[PARTS];
-        split8<PARTS>(lo, hi, y);
+        const int row = 64 * t + 16 * (c >> 2) & page_mask;
+        const uint8_t* p = base(pool.k, __shfl(run.page, x + (c >> 2), 64)) + (row + (c & 3)) * D;
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p) q[p][nb][j] = y[p];
-      }
-    }
-  }
-  if (t0 < t1) run.scales(a, hk);
-  const int64_t head_bytes = (int64_t)D << a.shift;
-  uint4 kr[4][KJ], vr[VT][DB];
-  auto base = [&](const uint8_t* p, int page) {
-    return p + ((int64_t)max(page, 0) * pool.Hkv + hk) * head_bytes;
-  };
-  const int page_mask = (1 << a.shift) - 1;
-  auto kload = [&](int t) {
-    const int x = 4 * (t - t0 & 15);
-    if constexpr (kLines) {
+        for (int mb = 0; mb < 4; ++mb)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int gk = 2 * i + (c >> 2 & 1);
-        const int row = 64 * t + 16 * gk & page_mask;
-        const uint8_t* p = base(pool.k, __shfl(run.page, x + gk, 64)) + (row + (c & 3)) * D + 64 * (c >> 3) + 16 * g;
-#pragma unroll
-        for (int mb = 0; mb < 4; ++mb) kr[mb][i] = load16<NT>(p + 4 * mb * D);
-      }
-    } else {
-      const int row = 64 * t + 16 * (c >> 2) & page_mask;
-      const uint8_t* p = base(pool.k, __shfl(run.page, x + (c >> 2), 64)) + (row + (c & 3)) * D;
-#pragma unroll
-      for (int mb = 0; mb < 4; ++mb)
-#pragma unroll
-        for (int j = 0; j < KJ; ++j) {
-          const int d = 64 * j + 16 * g;
-          kr[mb][j] = load16<NT>(p + 4 * mb * D + (EXACT || d < D ? d : 0));
-        }
-    }
-  };
-  auto vload = [&](int t) {
-    const int x = 4 * (t - t0 & 15);
-    if constexpr (VT == 2) {
-      const uint8_t* p = base(pool.v, __builtin_amdgcn_readlane(run.page, x)) + 128 * (c & 7) + 64 * (c >> 3) + 16 * g;
-#pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        vr[0][db] = load16<NT>(p + 128 * 16 * db);
-        vr[1][db] = load16<NT>(p + 128 * (16 * db + 8));
-      }
-    } else {
-      const int row = 64 * t + 16 * g & page_mask;
-      const uint8_t* p = base(pool.v, __shfl(run.page, x + g, 64)) + ((int64_t)c << a.shift) + row;
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-        vr[0][db] = load16<NT>(p + ((int64_t)(EXACT || 16 * db < D ? 16 * db : 0) << a.shift));
-    }
-  };
-
-  f32x4 o[NB][DB];
-  float mrow[NB], lsum[NB];  // running maximum (log2 units), lane-partial sum of p
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-    for (int db = 0; db < DB; ++db) o[nb][db] = f32x4{0.f, 0.f, 0.f, 0.f};
-    mrow[nb] = -INFINITY;
-    lsum[nb] = 0.f;
-  }
-
-  if (t0 < t1) {
-    run.turn();
-    kload(t0);
-    vload(t0);
-    run.look(a, table, t0 + 16, k1);
-  }
-  auto tile = [&](int t, auto sub) {
-    constexpr int V = decltype(sub)::value;  // of the tiles whose values are here
-    const int x = 4 * (t - t0 & 15);
-    const float ks = __shfl(run.ks, x + (c >> 2), 64);  // of the lane's K
-    const float vs = __shfl(run.vs, x + g, 64);         // of its V
-    const int page = __shfl(run.page, x + g, 64);
-    if constexpr (kLines)
-#pragma unroll
-      for (int mb = 0; mb < 4; ++mb) swap_halves(kr[mb][0], kr[mb][1]);
-    if constexpr (VT == 2 && V == 0)
-#pragma unroll
-      for (int db = 0; db < DB; ++db) swap_halves(vr[0][db], vr[1][db]);
-    f32x4 sc[NB][4];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int mb = 0; mb < 4; ++mb) sc[nb][mb] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < KJ; ++j)
-#pragma unroll
-      for (int mb = 0; mb < 4; ++mb) {
-        const bf16x8 k0 = bf16_of(kr[mb][j].x, kr[mb][j].y, ks), k1 = bf16_of(kr[mb][j].z, kr[mb][j].w, ks);
-#pragma unroll
-        for (int p = PARTS - 1; p >= 0; --p)
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            sc[nb][mb] = mfma16x16x32(k0, q[p][nb][2 * j], sc[nb][mb]);
-            sc[nb][mb] = mfma16x16x32(k1, q[p][nb][2 * j + 1], sc[nb][mb]);
+          for (int j = 0; j < KJ; ++j) {
+            const int d = 64 * j + 16 * g;
+            kr[mb][j] = load16<NT>(p + 4 * mb * D + (EXACT || d < D ? d : 0));
           }
       }
-    const bool more = t + 1 < t1;
-    if (more) {
-      const int step = t + 1 - t0 & 15;
-      if (step == 0) {
-        run.turn();
-        run.look(a, table, t + 17, k1);
-      } else if (step == 8) {
-        run.scales(a, hk);
-      }
-      kload(t + 1);
-    }
-
-    // A tile that not every row sees wholly, or with a page that there is not.
-    const bool edge = 64 * (t + 1) > clear;
-    if (edge || __any(page < 0)) {
-      const int left = page < 0 ? 0 : k1 - (64 * t + 16 * g);  // values that some row sees
-      if (edge && last > first) {
+    };
+    auto vload = [&](int t) {
+      const int x = 4 * (t - tb & 15);
+      if constexpr (VT == 2) {
+        const uint8_t* p =
+            base(pool.v, __builtin_amdgcn_readlane(run.page, x)) + 128 * (c & 7) + 64 * (c >> 3) + 16 * g;
 #pragma unroll
-        for (int db = 0; db < DB; ++db) strange |= clean_values(vr[V][db], left);
-      } else {  // all rows see the same
-        const uint32_t m[4] = {low_bytes(left), low_bytes(left - 4), low_bytes(left - 8), low_bytes(left - 12)};
+        for (int db = 0; db < DB; ++db) {
+          vr[0][db] = load16<NT>(p + 128 * 16 * db);
+          vr[1][db] = load16<NT>(p + 128 * (16 * db + 8));
+        }
+      } else {
+        const int row = 64 * t + 16 * g & page_mask;
+        const uint8_t* p = base(pool.v, __shfl(run.page, x + g, 64)) + ((int64_t)c << a.shift) + row;
 #pragma unroll
         for (int db = 0; db < DB; ++db)
-          vr[V][db] = make_uint4(vr[V][db].x & m[0], vr[V][db].y & m[1], vr[V][db].z & m[2], vr[V][db].w & m[3]);
+          vr[0][db] = load16<NT>(p + ((int64_t)(EXACT || 16 * db < D ? 16 * db : 0) << a.shift));
       }
+    };
+
+    f32x4 o[DB];
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const int see = page < 0 ? 0 : lim[nb] - (64 * t + 16 * g);
+    for (int db = 0; db < DB; ++db) o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float mrow = -INFINITY, lsum = 0.f;  // running maximum (log2 units), lane-partial sum of p
+
+    if (t0 < t1) {
+      run.turn();
+      kload(t0);
+      vload(t0);
+      if (!a.early) run.look(a, table, t0 + 16, k1);
+    }
+    auto tile = [&](int t, auto sub) {
+      constexpr int V = decltype(sub)::value;  // of the tiles whose values are here
+      const int x = 4 * (t - tb & 15);
+      const float ks = __shfl(run.ks, x + (c >> 2), 64);  // of the lane's K
+      const float vs = __shfl(run.vs, x + g, 64);         // of its V
+      const int page = __shfl(run.page, x + g, 64);
+      if constexpr (kLines)
+#pragma unroll
+        for (int mb = 0; mb < 4; ++mb) swap_halves(kr[mb][0], kr[mb][1]);
+      if constexpr (VT == 2 && V == 0)
+#pragma unroll
+        for (int db = 0; db < DB; ++db) swap_halves(vr[0][db], vr[1][db]);
+      f32x4 sc[4];
+#pragma unroll
+      for (int mb = 0; mb < 4; ++mb) sc[mb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < KJ; ++j)
+#pragma unroll
+        for (int mb = 0; mb < 4; ++mb) {
+          const bf16x8 lo = bf16_of(kr[mb][j].x, kr[mb][j].y, ks), hi = bf16_of(kr[mb][j].z, kr[mb][j].w, ks);
+#pragma unroll
+          for (int p = PARTS - 1; p >= 0; --p) {
+            sc[mb] = mfma16x16x32(lo, q[p][2 * j], sc[mb]);
+            sc[mb] = mfma16x16x32(hi, q[p][2 * j + 1], sc[mb]);
+          }
+        }
+      if (t + 1 < t1) {
+        const int step = t + 1 - tb & 15;
+        if (step == 0) {
+          run.turn();
+          run.look(a, table, t + 17, k1);
+        } else if (step == 8 && !a.early) {
+          run.scales(a, hk);
+        }
+        kload(t + 1);
+      }
+
+      // A tile that not every row sees wholly, or with a page that there is not.
+      const bool edge = 64 * (t + 1) > clear;
+      if (edge || __any(page < 0)) {
+        const int left = page < 0 ? 0 : k1 - (64 * t + 16 * g);  // values that some row sees
+        if (edge && last > first) {
+#pragma unroll
+          for (int db = 0; db < DB; ++db) strange |= clean_values(vr[V][db], left);
+        } else {  // all rows see the same
+          const uint32_t m[4] = {low_bytes(left), low_bytes(left - 4), low_bytes(left - 8), low_bytes(left - 12)};
+#pragma unroll
+          for (int db = 0; db < DB; ++db)
+            vr[V][db] = make_uint4(vr[V][db].x & m[0], vr[V][db].y & m[1], vr[V][db].z & m[2], vr[V][db].w & m[3]);
+        }
+        const int see = page < 0 ? 0 : lim - (64 * t + 16 * g);
 #pragma unroll
         for (int mb = 0; mb < 4; ++mb)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (4 * mb + i >= see) sc[nb][mb][i] = -INFINITY;
+            if (4 * mb + i >= see) sc[mb][i] = -INFINITY;
       }
-    }
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
+
       float mx = -INFINITY;
 #pragma unroll
       for (int mb = 0; mb < 4; ++mb)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[nb][mb][i]);
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[mb][i]);
       mx = group4_max(mx) * a.sl2;
-      if (mx > mrow[nb]) {
-        const float up = fast_exp2(mrow[nb] - mx);  // mrow = -inf: 0
-        lsum[nb] *= up;
+      if (mx > mrow) {
+        const float up = fast_exp2(mrow - mx);  // mrow = -inf: 0
+        lsum *= up;
 #pragma unroll
-        for (int db = 0; db < DB; ++db) o[nb][db] *= up;
-        mrow[nb] = mx;
+        for (int db = 0; db < DB; ++db) o[db] *= up;
+        mrow = mx;
       }
-      const float muse = mrow[nb] == -INFINITY ? 0.f : mrow[nb];
+      const float muse = mrow == -INFINITY ? 0.f : mrow;
       float sum = 0.f;  // (a tile's by itself: over 18,000 keys 3e-7 from 64 bits, 1e-6 in one chain)
 #pragma unroll
       for (int mb = 0; mb < 4; ++mb)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float p = fast_exp2(fmaf(sc[nb][mb][i], a.sl2, -muse));
+          const float p = fast_exp2(fmaf(sc[mb][i], a.sl2, -muse));
           sum += p;
-          sc[nb][mb][i] = p;
+          sc[mb][i] = p;
         }
-      lsum[nb] += sum;
-    }
+      lsum += sum;
 #pragma unroll
-    for (int k2 = 0; k2 < 2; ++k2) {
-      bf16x8 pb[NB][PARTS];
+      for (int k2 = 0; k2 < 2; ++k2) {
+        bf16x8 pb[PARTS];
+        split8<PARTS>(sc[2 * k2], sc[2 * k2 + 1], pb);
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) split8<PARTS>(sc[nb][2 * k2], sc[nb][2 * k2 + 1], pb[nb]);
+        for (int db = 0; db < DB; ++db) {
+          const bf16x8 v = bf16_of(k2 ? vr[V][db].z : vr[V][db].x, k2 ? vr[V][db].w : vr[V][db].y, vs);
 #pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        const bf16x8 v = bf16_of(k2 ? vr[V][db].z : vr[V][db].x, k2 ? vr[V][db].w : vr[V][db].y, vs);
-#pragma unroll
-        for (int p = PARTS - 1; p >= 0; --p)
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) o[nb][db] = mfma16x16x32(v, pb[nb][p], o[nb][db]);
+          for (int p = PARTS - 1; p >= 0; --p) o[db] = mfma16x16x32(v, pb[p], o[db]);
+        }
       }
+    };
+    for (int t = t0; t < t1; t += VT) {
+      tile(t, std::integral_constant<int, 0>{});
+      if constexpr (VT == 2)
+        if (t + 1 < t1) tile(t + 1, std::integral_constant<int, 1>{});
+      if (t + VT < t1) vload(t + VT);
     }
-  };
-  for (int t = t0; t < t1; t += VT) {
-    tile(t, std::integral_constant<int, 0>{});
-    if constexpr (VT == 2)
-      if (t + 1 < t1) tile(t + 1, std::integral_constant<int, 1>{});
-    if (t + VT < t1) vload(t + VT);
-  }
-
-  if (__any(strange))
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+    if (__any(strange))
       patch_nan<4 * DB>(
-          a, table, hk, max(64 * t0, clear & ~63), min(64 * t1, lim[nb]),
-          [&](int n) { return 16 * (n >> 2) + 4 * g + (n & 3); }, [&](int n) { o[nb][n >> 2][n & 3] = NAN; });
+          a, table, hk, max(64 * t0, clear & ~63), min(64 * t1, lim),
+          [&](int n) { return 16 * (n >> 2) + 4 * g + (n & 3); }, [&](int n) { o[n >> 2][n & 3] = NAN; });
 
-  // The waves' partials, brought to each row's maximum, meet in LDS.
+    // The waves' partials, brought to each row's maximum, meet in LDS.
+    if (g == 0) msm[wave][c] = mrow;
+    __syncthreads();
+    float top = -INFINITY;
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb)
-    if (g == 0) msm[wave][16 * nb + c] = mrow[nb];
-  __syncthreads();
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    float M = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < W; ++w) M = fmaxf(M, msm[w][16 * nb + c]);
-    const float f = mrow[nb] == -INFINITY ? 0.f : fast_exp2(mrow[nb] - M);
-    const float lt = group4_sum(lsum[nb]) * f;
-    if (g == 0) lsm[wave][16 * nb + c] = lt;
+    for (int w = 0; w < W; ++w) top = fmaxf(top, msm[w][c]);
+    const float f = mrow == -INFINITY ? 0.f : fast_exp2(mrow - top);
+    lsum = group4_sum(lsum) * f;
+    if (g == 0) lsm[wave][c] = lsum;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
-      *reinterpret_cast<f32x4*>(part + (wave * kRows + 16 * nb + c) * kPitch + 16 * db + 4 * g) =
-          mrow[nb] == -INFINITY ? f32x4{0.f, 0.f, 0.f, 0.f} : o[nb][db] * f;
-  }
-  __syncthreads();
-  const int chunks = D / 4;  // of a row
-  for (int it = tid; it < kRows * chunks; it += 64 * W) {
-    const int rr = it / chunks, d = 4 * (it - rr * chunks);
-    if (rb * kRows + rr >= a.R) break;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    float L = 0.f, M = -INFINITY;
+      *reinterpret_cast<f32x4*>(part + (wave * kRows + c) * kPitch + 16 * db + 4 * g) =
+          mrow == -INFINITY ? f32x4{0.f, 0.f, 0.f, 0.f} : o[db] * f;
+    __syncthreads();
+    const int chunks = D / 4;  // of a row
+    for (int it = tid; it < kRows * chunks; it += 64 * W) {
+      const int rr = it / chunks, d = 4 * (it - rr * chunks);
+      if (rb * kRows + rr >= a.R) break;
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      float L = 0.f, M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-      acc += *reinterpret_cast<const f32x4*>(part + (w * kRows + rr) * kPitch + d);
-      L += lsm[w][rr];
-      M = fmaxf(M, msm[w][rr]);
+      for (int w = 0; w < W; ++w) {
+        acc += *reinterpret_cast<const f32x4*>(part + (w * kRows + rr) * kPitch + d);
+        L += lsm[w][rr];
+        M = fmaxf(M, msm[w][rr]);
+      }
+      const int i = map.token(rr), h = hk * a.group + map.head(rr);
+      if (a.direct) {
+        const bool there = i < count;
+        store_vec4(static_cast<T*>(a.out) + (((int64_t)s.b * a.p.N + i) * a.p.Hq + h) * D + d,
+                   there ? acc * inverse_sum(L) : f32x4{0.f, 0.f, 0.f, 0.f});
+        if (d == 0) store_stats(a, s.b, h, i, there ? M : -INFINITY, there ? L : 0.f);
+      } else {
+        const int64_t pr = ((int64_t)i * a.p.Hq + h) * a.parts + s.segment;
+        *reinterpret_cast<f32x4*>(a.po + pr * D + d) = acc;
+        if (d == 0) a.ps[pr] = make_float2(M, L);
+      }
     }
-    const int i = map.token(rr), h = hk * a.group + map.head(rr);
-    if (a.direct) {
-      const bool there = i < count;
-      store_vec4(static_cast<T*>(a.out) + (((int64_t)s.b * a.p.N + i) * a.p.Hq + h) * D + d,
-                 there ? acc * inverse_sum(L) : f32x4{0.f, 0.f, 0.f, 0.f});
-      if (d == 0) store_stats(a, s.b, h, i, there ? M : -INFINITY, there ? L : 0.f);
-    } else {
-      const int64_t pr = ((int64_t)i * a.p.Hq + h) * a.parts + s.segment;
-      *reinterpret_cast<f32x4*>(a.po + pr * D + d) = acc;
-      if (d == 0) a.ps[pr] = make_float2(M, L);
-    }
-  }
-  __syncthreads();  // the next segment's partials take their place
+    __syncthreads();  // the next segment's partials take their place
   }
 }
 
@@ -558,7 +547,7 @@ __global__ __launch_bounds__(512, 1) void paged_tile_kernel(AttnArgs a) {
   Share s;
   if (!share_of([&](int b) { return keys_of(a, b); }, a.p.B, a.slots, a.deal, slot, s)) return;
 
-  const int past = a.p.past[s.b];
+  const int past = past_of(a.p.past, s.b);
   const int count = new_tokens(a.p.counts, a.p.N, s.b, past);
   const int32_t* table = a.p.table + (int64_t)s.b * a.p.width;
   constexpr int kRows = 32 * RW;
@@ -981,6 +970,7 @@ hipError_t launch_paged_attn(const PagedProblem& p, const void* q, void* out, fl
   a.m = m;
   a.l = l;
   a.direct = x.parts == 0;
+  a.early = a.direct && !x.tiled && (int64_t)p.width * p.pool.rows <= 1024;
   a.parts = x.parts;
   a.po = static_cast<float*>(ws);
   a.ps = reinterpret_cast<float2*>(a.po + prows * p.pool.D);
@@ -1002,8 +992,8 @@ hipError_t launch_paged_attn(const PagedProblem& p, const void* q, void* out, fl
     auto by_waves = [&](auto d, auto vt) {
       constexpr int DP = decltype(d)::value, VT = decltype(vt)::value;
       if constexpr (P == 1)
-        if (x.waves == 8) return launch(paged_stream_kernel<DP, true, 1, P, VT, NT, 8>);
-      launch(paged_stream_kernel<DP, true, 1, P, VT, NT, 4>);
+        if (x.waves == 8) return launch(paged_stream_kernel<DP, true, P, VT, NT, 8>);
+      launch(paged_stream_kernel<DP, true, P, VT, NT, 4>);
     };
     auto by_pages = [&](auto d) {
       if (two) by_waves(d, std::integral_constant<int, 2>{});
@@ -1011,8 +1001,8 @@ hipError_t launch_paged_attn(const PagedProblem& p, const void* q, void* out, fl
     };
     if (p.pool.D == 64) by_pages(std::integral_constant<int, 64>{});
     else if (p.pool.D == 128) by_pages(std::integral_constant<int, 128>{});
-    else if (p.pool.D < 128) launch(paged_stream_kernel<128, false, 1, P, 1, NT, 4>);
-    else launch(paged_stream_kernel<256, false, 1, P, 1, NT, 4>);
+    else if (p.pool.D < 128) launch(paged_stream_kernel<128, false, P, 1, NT, 4>);
+    else launch(paged_stream_kernel<256, false, P, 1, NT, 4>);
   };
   auto by_reads = [&](auto parts) {
     if (once) by_dim(parts, std::true_type{});

@@ -410,6 +410,19 @@ def test_bad_pages_are_not_seen(gpu, n, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,dtype", [(1, "bf16"), (3, "fp32"), (40, "bf16")])
+def test_lengths_beyond_the_table(gpu, n, dtype):
+    """A past of up to 2^31 - 1 rows sees what the table has."""
+    rng = np.random.default_rng(19)
+    pool = _pool(rng, 8, 16, 2, 64)
+    table = np.array([[3, 5, 1, 7], [2, 0, 6, 4]])
+    q, _ = _rows(gpu, rng, 2, n, 4, 64, dtype)
+    want = op.attention(q, pool, table, [64, 64], [n] * 2)
+    for past in ([2 ** 31 - 1, 2 ** 30], [64, 2 ** 30 + 5]):
+        _check_attention(_attend(gpu, q, _to_pages(gpu, pool), table, past, None, dtype), want, q, pool, dtype)
+
+
+@pytest.mark.gpu
 def test_shared_pages(gpu):
     """Two sequences with the same prefix see the same pages."""
     rng = np.random.default_rng(13)
