@@ -325,7 +325,19 @@ ATTEND = [
     (4, 1, 256, "fp32", 16, [129, 64], 11, None, 0),
     (2, 2, 256, "bf16", 64, [313], 40, None, 0),
     (4, 2, 192, "bf16", 128, [90], 20, None, 0),
-] + [(4, 2, 64, "bf16", 16, [(37 * i) % 91 - 1 for i in range(70)], 2, [i % 3 for i in range(70)], 0)]
+    # long ones: more than a run of 16 tiles a wave, several workgroups a sequence
+    (4, 2, 128, "bf16", 128, [5000, 70, 2300], 2, None, 0),
+    (4, 2, 64, "bf16", 128, [9100], 3, None, 0),
+    (2, 1, 128, "fp32", 128, [3000], 2, None, 0),
+    (8, 2, 128, "bf16", 16, [4200, 1], 1, None, 3),
+    (4, 2, 64, "bf16", 32, [3000, 2999, 64], 1, None, 0),
+    (2, 1, 64, "bf16", 64, [70000], 1, None, 0),
+    (2, 1, 128, "bf16", 64, [70000], 2, None, 0),
+    (8, 2, 128, "bf16", 64, [5000, 300], 70, [70, 33], 0),
+    (2, 1, 64, "bf16", 128, [4000], 90, None, 0),
+] + [(4, 2, 64, "bf16", 16, [(37 * i) % 91 - 1 for i in range(70)], 2, [i % 3 for i in range(70)], 0),
+     (2, 1, 64, "bf16", 128, [(379 * i) % 2500 for i in range(67)], 1, None, 0),
+     (2, 1, 128, "bf16", 64, [(379 * i) % 900 for i in range(70)], 40, None, 0)]
 
 
 @pytest.mark.gpu
