@@ -912,6 +912,18 @@ constexpr int64_t kWanted = 512;  // workgroups of the streaming form for the ch
 constexpr int64_t kWantedTiled = 256;
 constexpr int64_t kShort = 16;  // tiles of a sequence that are not split over workgroups
 
+// Many rows go by tiles that a workgroup shares once all blocks of 16 rows together
+// would read more than this, at the tables' width; up to there, and up to kFewRows
+// rows a KV head, each block reads the cache by itself, later ones from L2 (32/8 heads;
+// blocks of 16 against tiles, us).  Of 128: 24 tokens over 2,000 keys (25 MB) 18.4
+// and 21.4, 64 over 500 (18 MB) 12.7 and 20.6, 64 over 4,000 (133 MB) 27.3 and 31.9, 32
+// over 16,000 (263 MB) 38.5 and 31.8, 256 over 8,000 (1.1 GB) 98 and 63; eight
+// sequences' 64 over 500 (148 MB) 27 and 36, 32 over 2,000 (266 MB) 41 and 33.  Of 64: 64
+// tokens over 8,000 (132 MB) 22 and 26, 128 over 16,000 (529 MB) 52 and 44.  8 tokens over
+// 131,072 keys (537 MB) 78 and 87.  Around the limit either is up to a sixth behind.
+constexpr int64_t kBlockBytes = 160 << 20;
+constexpr int64_t kFewRows = 48;
+
 // Query rows from which a wave each is enough for the merge.
 constexpr int64_t kManyRows = 1024;
 
@@ -926,7 +938,8 @@ struct Plan {
 Plan make_plan(const PagedProblem& p) {
   const int64_t R = (int64_t)p.N * (p.Hq / p.pool.Hkv);
   Plan x;
-  x.tiled = p.dtype == 1 && (p.pool.D == 64 || p.pool.D == 128) && R > 64;
+  const int64_t reads = (R + 15) / 16 * p.B * p.width * p.pool.rows * p.pool.Hkv * p.pool.D * 2;
+  x.tiled = p.dtype == 1 && (p.pool.D == 64 || p.pool.D == 128) && R > kFewRows && reads > kBlockBytes;
   x.rows = x.tiled ? 256 : 16;
   x.tile = !x.tiled && p.pool.rows == 128 && (p.pool.D == 64 || p.pool.D == 128) ? 128 : 64;
   x.units = (int)((R + x.rows - 1) / x.rows * p.pool.Hkv);

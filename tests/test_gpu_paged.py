@@ -302,6 +302,15 @@ def _attend(gpu, q, p, table, past, counts, dtype, ws=True):
                            m=nan(b, hq, n), l=nan(b, hq, n), workspace=work)
 
 
+def _wide(table, q, pool):
+    """The same table with entries of no page behind, so many that rows of a bf16 cache
+    go by shared tiles instead of blocks of 16 (csrc/paged_attn.hip, make_plan)."""
+    (b, n, hq, d), (_, hkv, rows, _) = q.shape, pool["k"].shape
+    blocks = -(-n * hq // hkv // 16)
+    width = (160 << 20) // (blocks * b * rows * hkv * d * 2) + 1
+    return np.pad(table, ((0, 0), (0, max(0, width - table.shape[1]))), constant_values=-7)
+
+
 # hq, hkv, d, dtype, rows of a page, past, tokens, counts, table wider by
 ATTEND = [
     (8, 2, 64, "bf16", 16, [5], 1, None, 0),
@@ -358,13 +367,17 @@ def test_attention(gpu, case):
     again = _attend(gpu, q, p, table, past, counts, dtype, ws=False)
     for x, y in zip(got, again):
         assert gpu.equal(x, y)
+    if n * hq // hkv > 48 and dtype == "bf16":
+        got = _attend(gpu, q, p, _wide(table, q, pool), past, counts, dtype)
+        _check_attention(got, want, q, pool, dtype)
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("wide", [False, True], ids=["", "wide"])
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("n", [1, 6, 40, 130])
-def test_rows_that_are_not_seen_do_not_matter(gpu, n, d, dtype):
+def test_rows_that_are_not_seen_do_not_matter(gpu, n, d, dtype, wide):
     """NaN codes and scales in pages and rows behind a token, also the next tokens'
     own, reach nobody; a seen one reaches its column alone."""
     rng = np.random.default_rng(5)
@@ -372,6 +385,8 @@ def test_rows_that_are_not_seen_do_not_matter(gpu, n, d, dtype):
     table, pages = _table(rng, past, n, rows)
     pool = _pool(rng, pages, rows, hkv, d)
     q, _ = _rows(gpu, rng, 3, n, hq, d, dtype, 1.5)
+    if wide:
+        table = _wide(table, q, pool)
     want = op.attention(q, pool, table, past, counts)
     seen = np.zeros((pages, rows), bool)
     for b in range(3):
@@ -401,9 +416,10 @@ def test_rows_that_are_not_seen_do_not_matter(gpu, n, d, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("wide", [False, True], ids=["", "wide"])
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 @pytest.mark.parametrize("n", [1, 20, 70])
-def test_bad_pages_are_not_seen(gpu, n, dtype):
+def test_bad_pages_are_not_seen(gpu, n, dtype, wide):
     rng = np.random.default_rng(12)
     hq, hkv, d, rows = 8, 2, 128, 16
     past = [200, 90, 150]
@@ -414,22 +430,26 @@ def test_bad_pages_are_not_seen(gpu, n, dtype):
     pool = _pool(rng, pages, rows, hkv, d)
     q, _ = _rows(gpu, rng, 3, n, hq, d, dtype)
     want = op.attention(q, pool, table, past, [n] * 3)
-    _check_attention(_attend(gpu, q, _to_pages(gpu, pool), table, past, None, dtype), want, q, pool, dtype)
+    widen = (lambda t: _wide(t, q, pool)) if wide else (lambda t: t)
+    _check_attention(_attend(gpu, q, _to_pages(gpu, pool), widen(table), past, None, dtype), want, q, pool, dtype)
     # a table that ends before the tokens
-    short = table[:, :9]
+    short = widen(table[:, :9])
     want = op.attention(q, pool, short, past, [n] * 3)
     _check_attention(_attend(gpu, q, _to_pages(gpu, pool), short, past, None, dtype), want, q, pool, dtype)
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("n,dtype", [(1, "bf16"), (3, "fp32"), (40, "bf16")])
+@pytest.mark.parametrize("n,dtype", [(1, "bf16"), (3, "fp32"), (40, "bf16"), (40, "wide")])
 def test_lengths_beyond_the_table(gpu, n, dtype):
     """A past of up to 2^31 - 1 rows sees what the table has."""
     rng = np.random.default_rng(19)
     pool = _pool(rng, 8, 16, 2, 64)
     table = np.array([[3, 5, 1, 7], [2, 0, 6, 4]])
+    dtype, wide = ("bf16", True) if dtype == "wide" else (dtype, False)
     q, _ = _rows(gpu, rng, 2, n, 4, 64, dtype)
     want = op.attention(q, pool, table, [64, 64], [n] * 2)
+    if wide:  # (more query heads' rows than kFewRows)
+        table = _wide(table, q, pool)
     for past in ([2 ** 31 - 1, 2 ** 30], [64, 2 ** 30 + 5]):
         _check_attention(_attend(gpu, q, _to_pages(gpu, pool), table, past, None, dtype), want, q, pool, dtype)
 
