@@ -36,7 +36,7 @@ struct Rows {
   const lc_rows_t* s;
   size_t elem;
 
-  // Elements from the first to behind the last; strides are >= 0 and bounded.
+  // Elements from the first to behind the last: 2^40 at most (check).
   int64_t extent() const {
     return (batch - 1) * s->seq_stride + (tokens - 1) * s->token_stride + (heads - 1) * s->head_stride + D;
   }
@@ -52,6 +52,9 @@ struct Rows {
     for (int64_t x : st)
       if (x < 0 || x > (int64_t)1 << 40)
         return set_error(LC_ERR_INVALID, "strides of %s must lie in 0 .. 2^40", name);
+    const __int128 last = (__int128)(batch - 1) * st[0] + (__int128)(tokens - 1) * st[1] +
+                          (__int128)(heads - 1) * st[2] + D;
+    if (last > (__int128)1 << 40) return set_error(LC_ERR_INVALID, "%s spans more than 2^40 elements", name);
     return LC_OK;
   }
   // No two rows may share memory.

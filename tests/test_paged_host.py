@@ -321,3 +321,21 @@ def test_rotary_apply_is_checked():
         assert call(**kw) == U, kw
     assert call(batch=0, x=None, out=None) == _lib.LC_OK
     assert call(tokens=0) == _lib.LC_OK
+
+
+def test_extents_beyond_64_bits_are_refused():
+    """Strides within their bounds whose products with the sizes are not."""
+    lib = _lib.load()
+    far = _lib.Rows(1 << 40, 1 << 40, 64)
+    near = _lib.Rows(64, 64, 64)
+    rot = _lib.Rotary(64, 64, 0, 1.0, 1 << 30)
+    n = 1 << 23  # n 2^40 is 2^63
+    for x, out in ((far, near), (near, far)):
+        for batch, tokens in ((n + 1, 1), (1, n + 1), (2, 1)):
+            assert lib.lc_rotary_apply(rot, 1, batch, tokens, 1, None, 0, 0, 1 << 50, x, 1 << 52, out, None) == I
+    d = _desc(tokens=n + 1, batch=1, heads_q=1, heads_kv=1)
+    apart = [i << 24 for i in range(1, 8)]
+    for k, v in ((far, near), (near, far)):
+        rc = lib.lc_paged_append(d, None, *apart[:2], None, None, None, None, 1 << 50, k, 1 << 52, v, 1 << 54, 1 << 55,
+                                 1 << 56, 1 << 57, None)
+        assert rc == I
