@@ -345,7 +345,10 @@ int lc_cache_commit(const lc_cache_t* cache, int32_t layers, void* const* ks, vo
  * a page that an append writes to must be one sequence's alone.
  * past[b] (int32, device) rows stand before the new tokens; < 0: no sequence.
  * counts[b] (int32, device; NULL: tokens) of the call's tokens are there, the
- * others are padding; it is clipped to [0, tokens].  New token i is row past + i. */
+ * others are padding; it is clipped to [0, tokens].  New token i is row past + i.
+ * Limits: table_width * page_rows 2^30, and 2^36 times batch; batch * heads_kv 2^20;
+ * tokens 2^24; batch * tokens * heads_q 2^25 (heads_kv, where no queries are given);
+ * heads_q / heads_kv 2^16. */
 typedef struct lc_paged {
   int32_t batch;
   int32_t tokens;   /* new tokens of a sequence, at most */

@@ -131,7 +131,9 @@ int check_paged(const lc_paged_t* c, bool queries) {
     return set_error(LC_ERR_UNSUPPORTED, "the paged cache needs head_dim %% 16 == 0 and <= 256");
   if (c->page_rows != 16 && c->page_rows != 32 && c->page_rows != 64 && c->page_rows != 128)
     return set_error(LC_ERR_UNSUPPORTED, "a page has 16, 32, 64 or 128 rows");
+  // (All sequences' 64-key tiles are counted in 31 bits, shared pages in each.)
   if ((int64_t)c->table_width * c->page_rows > 1 << 30 || (int64_t)c->batch * c->heads_kv > 1 << 20 ||
+      (int64_t)c->table_width * c->page_rows * c->batch > (int64_t)1 << 36 ||
       c->tokens > 1 << 24 || (int64_t)c->batch * c->tokens * (queries ? c->heads_q : c->heads_kv) > 1 << 25)
     return set_error(LC_ERR_UNSUPPORTED, "the cache or its tokens exceed the kernels' grids");
   return LC_OK;

@@ -339,3 +339,13 @@ def test_extents_beyond_64_bits_are_refused():
         rc = lib.lc_paged_append(d, None, *apart[:2], None, None, None, None, 1 << 50, k, 1 << 52, v, 1 << 54, 1 << 55,
                                  1 << 56, 1 << 57, None)
         assert rc == I
+
+
+def test_tiles_of_all_sequences_are_counted_in_31_bits():
+    """Sequences that share pages may have more rows together than the pool."""
+    lib = _lib.load()
+    a = 1 << 20  # never dereferenced
+    for d in (_desc(batch=65, table_width=1 << 26), _desc(batch=1 << 10, table_width=(1 << 22) + 1)):
+        assert lib.lc_paged_attn_workspace_bytes(d) == 0
+        assert lib.lc_paged_attn(d, *[a] * 12, 1 << 30, None) == U
+    assert lib.lc_paged_attn_workspace_bytes(_desc(batch=64, table_width=1 << 26)) > 0
