@@ -633,26 +633,27 @@ def layer_extend_paged(x: torch.Tensor, w: Dict[str, torch.Tensor], cfg: ModelCo
     ``past`` [B] and ``counts`` [B] as in ``paged``; rows of tokens from counts on are
     padding.  Returns (x_after_attention, mlp_out) as layer_decode."""
     b = table.shape[0]
-    n = x.shape[0] // b
+    n = x.shape[0] // max(b, 1)
     d, hq, hkv = cfg.head_dim, cfg.num_heads, cfg.num_key_value_heads
-    if x.shape[0] != b * n:
+    if n == 0 or x.shape[0] != b * n:
         raise ValueError(f"{x.shape[0]} rows are no {b} sequences of as many tokens")
-    if residual is not None:
-        xin = torch.empty_like(x)
-        h = rmsnorm(x, w["norm1"], cfg.rms_norm_eps, residual=residual, residual_out=xin)
-    else:
-        xin = x
-        h = rmsnorm(x, w["norm1"], cfg.rms_norm_eps)
-    q, k, v = linear(h, w["wqkv"]).view(b, n, hq + 2 * hkv, d).split((hq, hkv, hkv), 2)
-    q = paged.append(pages, table, past, k, v, counts=counts, rotary=rotary, q=q)
-    attn, _, _ = paged.attention(q, pages, table, past, counts=counts, workspace=workspace)
-    ao = linear(attn.view(b * n, hq * d), w["wo"])
-    x2 = torch.empty_like(x)
-    h2 = rmsnorm(xin, w["norm2"], cfg.rms_norm_eps, residual=ao, residual_out=x2)
-    gu = linear(h2, w["wgu"])
-    inter = cfg.intermediate_size
-    a = swiglu(gu[:, :inter], gu[:, inter:])
-    return x2, linear(a, w["wd"])
+    with torch.cuda.device_of(x):  # the other operators here launch on the current device
+        if residual is not None:
+            xin = torch.empty_like(x)
+            h = rmsnorm(x, w["norm1"], cfg.rms_norm_eps, residual=residual, residual_out=xin)
+        else:
+            xin = x
+            h = rmsnorm(x, w["norm1"], cfg.rms_norm_eps)
+        q, k, v = linear(h, w["wqkv"]).view(b, n, hq + 2 * hkv, d).split((hq, hkv, hkv), 2)
+        q = paged.append(pages, table, past, k, v, counts=counts, rotary=rotary, q=q)
+        attn, _, _ = paged.attention(q, pages, table, past, counts=counts, workspace=workspace)
+        ao = linear(attn.view(b * n, hq * d), w["wo"])
+        x2 = torch.empty_like(x)
+        h2 = rmsnorm(xin, w["norm2"], cfg.rms_norm_eps, residual=ao, residual_out=x2)
+        gu = linear(h2, w["wgu"])
+        inter = cfg.intermediate_size
+        a = swiglu(gu[:, :inter], gu[:, inter:])
+        return x2, linear(a, w["wd"])
 
 
 class PagedCache:
@@ -680,7 +681,7 @@ class PagedCache:
         self.rotary = rotary if rotary is not None else rot.Rotary.of(
             rope_params(cfg.head_dim, cfg.rope_theta, cfg.rope_scaling), device)
         self.rows = [0] * sequences
-        self._device = device
+        self._device = torch.empty(0, device=device).device  # (with its number: the current one may change)
         self._pages: List[Optional[List[int]]] = [None] * sequences  # None: the slot is free
         self._free = list(range(pages - 1, -1, -1))
 
@@ -733,14 +734,15 @@ class PagedCache:
         n = max(counts)
         padded = torch.nn.utils.rnn.pad_sequence(list(ids), batch_first=True)
         x = torch.nn.functional.embedding(padded.reshape(-1), weights["embed"])
-        res = None
-        for lw, pool in zip(weights["layers"], self.pools):
-            x, res = layer_extend_paged(x, lw, self.cfg, self.rotary, pool, table, tpast,
-                                        tcounts if min(counts) < n else None, residual=res,
-                                        workspace=workspace)
-        last = torch.arange(len(slots), device=self._device) * n + tcounts.long() - 1
-        h = rmsnorm(x[last], weights["final_norm"], self.cfg.rms_norm_eps, residual=res[last])
-        logits = linear(h, weights["lm_head"])
+        with torch.cuda.device_of(x):
+            res = None
+            for lw, pool in zip(weights["layers"], self.pools):
+                x, res = layer_extend_paged(x, lw, self.cfg, self.rotary, pool, table, tpast,
+                                            tcounts if min(counts) < n else None, residual=res,
+                                            workspace=workspace)
+            last = torch.arange(len(slots), device=self._device) * n + tcounts.long() - 1
+            h = rmsnorm(x[last], weights["final_norm"], self.cfg.rms_norm_eps, residual=res[last])
+            logits = linear(h, weights["lm_head"])
         del self._free[len(self._free) - sum(need):]  # every layer has its rows
         for slot, t, p, c in zip(slots, tables, past, counts):
             self._pages[slot], self.rows[slot] = t, p + c

@@ -109,3 +109,37 @@ def test_sizes(monkeypatch):
     c = ly.PagedCache(CFG, 2, 1, "cpu", rotary=r)
     assert c.rotary is r and len(c.pools) == 2 and c.pools[0].rows == 64
     assert ly.PagedCache(CFG, 2, 1, "cpu").rotary.inv_freq[0] == 1.0
+
+
+def test_runs_on_its_own_device(cache, monkeypatch):
+    """Layers and the final norm run with the tensors' device current, and tables are
+    made where the cache was, not where the current device is by then."""
+    from contextlib import contextmanager
+
+    c, w, calls = cache
+    inside = []
+
+    @contextmanager
+    def device_of(t):
+        inside.append(t.device)
+        yield
+        inside.pop()
+
+    monkeypatch.setattr(torch.cuda, "device_of", device_of)
+    for name in ("layer_extend_paged", "rmsnorm"):
+        was = getattr(ly, name)
+
+        def checked(*args, was=was, **kw):
+            assert inside == [torch.device("cpu")]
+            return was(*args, **kw)
+
+        monkeypatch.setattr(ly, name, checked)
+    c.extend([c.open()], [ids(3)], w)
+    assert len(calls) == 2 and not inside
+    assert isinstance(c._device, torch.device)
+
+
+def test_a_layer_needs_tokens_of_every_sequence():
+    for rows, b in ((5, 2), (0, 2), (3, 0)):
+        with pytest.raises(ValueError, match="sequences"):
+            ly.layer_extend_paged(torch.zeros(rows, 64), {}, CFG, None, None, torch.zeros(b, 1), None)
