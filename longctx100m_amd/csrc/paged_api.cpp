@@ -41,9 +41,10 @@ struct Rows {
     return (batch - 1) * s->seq_stride + (tokens - 1) * s->token_stride + (heads - 1) * s->head_stride + D;
   }
   Range bytes(const void* p) const { return range(p, (size_t)extent() * elem); }
-  bool vec(const void* p) const {
-    const int64_t e = 16 / (int64_t)elem;
-    return aligned(p, 16) && (batch == 1 || s->seq_stride % e == 0) &&
+  // Whether every row is so aligned.
+  bool vec(const void* p, int bytes = 16) const {
+    const int64_t e = bytes / (int64_t)elem;
+    return aligned(p, bytes) && (batch == 1 || s->seq_stride % e == 0) &&
            (tokens == 1 || s->token_stride % e == 0) && (heads == 1 || s->head_stride % e == 0);
   }
   int check(const char* name) const {
@@ -246,7 +247,9 @@ int lc_rotary_apply(const lc_rotary_t* rotary, int32_t dtype, int64_t batch, int
   p.out = out;
   p.xs = head_rows(x_rows);
   p.os = head_rows(out_rows);
-  p.vec = xr.vec(x) && orr.vec(out);
+  p.align = (int)e;
+  for (int bytes : {8, 16})
+    if (xr.vec(x, bytes) && orr.vec(out, bytes)) p.align = bytes;
   p.copy = !in_place;
   hipError_t err = lc::launch_rotary(p, static_cast<hipStream_t>(stream));
   return err == hipSuccess ? LC_OK : hip_error(err, "lc_rotary_apply launch");

@@ -90,8 +90,8 @@ __device__ __forceinline__ void append_keys(const AppendArgs& a, const Block& k,
     const int row = k.lo + r0 + i * step;
     if (r0 < step && row < k.hi) {
       const T* p = src + (k.token0 + row) * a.ks.token;
-      load8<kVec>(x[i], p + da);
-      load8<kVec>(y[i], p + db);
+      load_n<kVec>(x[i], p + da);
+      load_n<kVec>(y[i], p + db);
     }
   }
   uint64_t turns[8];
@@ -111,7 +111,7 @@ __device__ __forceinline__ void append_keys(const AppendArgs& a, const Block& k,
         float2 cs[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) cs[e] = turn_cos_sin((uint64_t)(pos0 + row) * turns[e], a.turns.factor);
-        turn8(x[i], y[i], cs, a.turns.interleaved);
+        turn_n(x[i], y[i], cs, a.turns.interleaved);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) top = fmaxf(top, fmaxf(finite_abs(x[i][e]), finite_abs(y[i][e])));
@@ -161,7 +161,7 @@ __device__ __forceinline__ void append_values(const AppendArgs& a, const Block& 
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int row = 4 * rg + r;
-        if (row >= k.lo && row < k.hi) load8<kVec>(x[i][r], src + (k.token0 + row) * a.vs.token + 8 * dg);
+        if (row >= k.lo && row < k.hi) load_n<kVec>(x[i][r], src + (k.token0 + row) * a.vs.token + 8 * dg);
         else
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[i][r][e] = 0.f;
@@ -257,7 +257,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
   }
   const uint32_t row0 = blockIdx.x * (uint32_t)a.group, rows = (uint32_t)a.p.B * a.p.N;  // below 2^25
   const int n = (int)min((uint32_t)a.group, rows - row0);
-  turn_tokens<T, kVec>(
+  turn_tokens<T, 8, kVec>(
       cs, a.turns, n, a.p.Hq, a.p.pool.D, a.qs.head, a.p.pool.D, true, 1,
       [&](int t) {
         const uint32_t row = row0 + t, b = row / (uint32_t)a.p.N;

@@ -46,65 +46,73 @@ __device__ __forceinline__ float2 turn_cos_sin(uint64_t phase, float factor) {
   return make_float2((quarter + 1) & 2 ? -u * factor : u * factor, quarter & 2 ? -v * factor : v * factor);
 }
 
-// Eight consecutive elements as fp32, by 16-byte accesses (kVec) or one by one.
-template <bool kVec>
-__device__ __forceinline__ void load8(float (&x)[8], const float* p) {
+// N consecutive elements as fp32, by 16-byte accesses (kVec; four bf16: 8-byte
+// ones) or one by one.
+template <bool kVec, int N>
+__device__ __forceinline__ void load_n(float (&x)[N], const float* p) {
   if constexpr (kVec) {
-    const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+    static_assert(N % 4 == 0, "whole vectors");
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = a[e], x[4 + e] = b[e];
+    for (int i = 0; i < N / 4; ++i) {
+      const f32x4 a = reinterpret_cast<const f32x4*>(p)[i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * i + e] = a[e];
+    }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = p[e];
+    for (int e = 0; e < N; ++e) x[e] = p[e];
   }
 }
-template <bool kVec>
-__device__ __forceinline__ void load8(float (&x)[8], const uint16_t* p) {
+template <bool kVec, int N>
+__device__ __forceinline__ void load_n(float (&x)[N], const uint16_t* p) {
   if constexpr (kVec) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    static_assert(N == 8 || N == 4, "one vector");
+    typedef uint32_t words __attribute__((ext_vector_type(N / 2)));
+    const words w = *reinterpret_cast<const words*>(p);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < N / 2; ++e) {
       x[2 * e] = __uint_as_float(w[e] << 16);
       x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = bf16_to_f32(p[e]);
+    for (int e = 0; e < N; ++e) x[e] = bf16_to_f32(p[e]);
   }
 }
-template <bool kVec>
-__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
+template <bool kVec, int N>
+__device__ __forceinline__ void store_n(float* p, const float (&x)[N]) {
   if constexpr (kVec) {
-    reinterpret_cast<f32x4*>(p)[0] = f32x4{x[0], x[1], x[2], x[3]};
-    reinterpret_cast<f32x4*>(p)[1] = f32x4{x[4], x[5], x[6], x[7]};
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i)
+      reinterpret_cast<f32x4*>(p)[i] = f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) p[e] = x[e];
+    for (int e = 0; e < N; ++e) p[e] = x[e];
   }
 }
-template <bool kVec>
-__device__ __forceinline__ void store8(uint16_t* p, const float (&x)[8]) {
+template <bool kVec, int N>
+__device__ __forceinline__ void store_n(uint16_t* p, const float (&x)[N]) {
   if constexpr (kVec) {
-    uint32_t w[4];
+    typedef uint32_t words __attribute__((ext_vector_type(N / 2)));
+    words w;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int e = 0; e < N / 2; ++e)
       w[e] = (uint32_t)f32_to_bf16(x[2 * e]) | ((uint32_t)f32_to_bf16(x[2 * e + 1]) << 16);
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<words*>(p) = w;
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) p[e] = f32_to_bf16(x[e]);
+    for (int e = 0; e < N; ++e) p[e] = f32_to_bf16(x[e]);
   }
 }
 
-// Turns eight pairs.  Half layout: a holds the first elements, b the second
-// ones; interleaved: a and b are 16 consecutive elements.  cs: (cos, sin) of
-// the pairs.
-__device__ __forceinline__ void turn8(float (&a)[8], float (&b)[8], const float2* cs, int interleaved) {
-  if (interleaved) {
+// Turns N pairs.  Half layout: a holds the first elements, b the second ones;
+// interleaved: a and b are 2 N consecutive elements.  cs: (cos, sin) of the pairs.
+template <int N>
+__device__ __forceinline__ void turn_n(float (&a)[N], float (&b)[N], const float2* cs, int interleaved) {
+  if (N > 1 && interleaved) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 p = cs[e], q = cs[4 + e];
+    for (int e = 0; e < N / 2; ++e) {
+      const float2 p = cs[e], q = cs[N / 2 + e];
       const float x = a[2 * e], y = a[2 * e + 1], z = b[2 * e], w = b[2 * e + 1];
       a[2 * e] = x * p.x - y * p.y;
       a[2 * e + 1] = y * p.x + x * p.y;
@@ -113,7 +121,7 @@ __device__ __forceinline__ void turn8(float (&a)[8], float (&b)[8], const float2
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < N; ++e) {
       const float2 p = cs[e];
       const float x = a[e], y = b[e];
       a[e] = x * p.x - y * p.y;
@@ -132,30 +140,32 @@ struct HeadRows {
 constexpr int kTurnTokens = 4;
 constexpr int kTurnPairs = 128;  // at most in a head
 
-// Units of eight pairs (16 elements) of `tokens` rows, token t of the workgroup
-// at x(t) / out(t) and position pos(t), or absent (there(t) false); dims past the
-// pairs are copied, where copy says so.  Requires half % 8 == 0 and D % 16 == 0.
-template <typename T, bool kVec, typename In, typename Out, typename Pos, typename There>
+// Units of N pairs (2 N elements) of `tokens` rows, token t of the workgroup at
+// x(t) / out(t) and position pos(t), or absent (there(t) false); dims past the pairs
+// are copied, where copy says so.  Requires half % N == 0, and D % 2 N == 0 unless N
+// is one.
+template <typename T, int N, bool kVec, typename In, typename Out, typename Pos, typename There>
 __device__ __forceinline__ void turn_tokens(float2* cs, const Turns& r, int tokens, int heads, int D,
                                             int64_t in_head, int64_t out_head, bool copy,
                                             uint64_t sign, const In& in, const Out& out,
                                             const Pos& pos, const There& there) {
   const int tid = threadIdx.x;
-  const int units = (copy ? D : 2 * r.half) / 16;  // of a head
+  const int units = ((copy ? D : 2 * r.half) + 2 * N - 1) / (2 * N);  // of a head
   const int step = 256 / units;                    // heads that the workgroup takes at once
   const int u = tid % units, h0 = tid / units;
-  const bool turned = 8 * u < r.half;
-  // Where the unit's two groups of eight begin.
-  const int da = turned && !r.interleaved ? 8 * u : 16 * u;
-  const int db = turned && !r.interleaved ? 8 * u + r.half : 16 * u + 8;
+  const bool turned = N * u < r.half;
+  // Where the unit's two groups of N begin.
+  const int da = turned && !r.interleaved ? N * u : 2 * N * u;
+  const int db = turned && !r.interleaved ? N * u + r.half : 2 * N * u + N;
+  const bool both = N > 1 || db < D;  // (a head of odd size ends in half a unit)
   const int rows = tokens * heads;
   const bool mine = h0 < step;
-  float a[8], b[8], an[8], bn[8];
-  auto load = [&](int t, int h, float (&x)[8], float (&y)[8]) {
+  float a[N], b[N], an[N], bn[N];
+  auto load = [&](int t, int h, float (&x)[N], float (&y)[N]) {
     if (!there(t)) return;
     const T* p = in(t) + h * in_head;
-    load8<kVec>(x, p + da);
-    load8<kVec>(y, p + db);
+    load_n<kVec>(x, p + da);
+    if (both) load_n<kVec>(y, p + db);
   };
   int t = h0 / heads, h = h0 - t * heads;
   if (mine && h0 < rows) load(t, h, a, b);  // on its way while the angles are formed
@@ -170,13 +180,13 @@ __device__ __forceinline__ void turn_tokens(float2* cs, const Turns& r, int toke
     while (hn >= heads) hn -= heads, ++tn;
     if (row + step < rows) load(tn, hn, an, bn);
     if (there(t)) {
-      if (turned) turn8(a, b, cs + t * r.half + 8 * u, r.interleaved);
+      if (turned) turn_n(a, b, cs + t * r.half + N * u, r.interleaved);
       T* p = out(t) + h * out_head;
-      store8<kVec>(p + da, a);
-      store8<kVec>(p + db, b);
+      store_n<kVec>(p + da, a);
+      if (both) store_n<kVec>(p + db, b);
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) a[e] = an[e], b[e] = bn[e];
+    for (int e = 0; e < N; ++e) a[e] = an[e], b[e] = bn[e];
     t = tn;
     h = hn;
   }
@@ -193,7 +203,7 @@ struct RotaryProblem {
   const void* x;
   void* out;
   HeadRows xs, os;
-  bool vec;   // every row is 16-byte aligned
+  int align;  // of every row, in bytes: 16, 8, or an element's
   bool copy;  // dims that do not turn have to be copied
 };
 hipError_t launch_rotary(const RotaryProblem& p, hipStream_t s);

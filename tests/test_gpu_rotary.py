@@ -200,3 +200,36 @@ def test_streams_and_graphs(gpu):
         g.replay()
         gpu.cuda.synchronize()
         assert gpu.equal(out, rotary.rotate(x, at, r))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("interleaved", [False, True], ids=["half", "interleaved"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("d,rd", [(80, 40), (40, 24), (128, 100), (90, 90), (33, 32), (65, 6), (255, 254), (2, 2), (3, 2)])
+@pytest.mark.parametrize("heads", [1, 7, 300])
+def test_pairs_that_are_no_vectors(gpu, heads, d, rd, dtype, interleaved):
+    """Four pairs at a time, or one; heads of odd size; more heads than a workgroup takes
+    at once; rows of 8-byte alignment."""
+    rng = np.random.default_rng(d + heads)
+    tokens = 1030 if heads == 7 else 3
+    x, tx = _data(gpu, rng, (tokens, heads, d), dtype)
+    r = rotary.Rotary(d, 500000.0, rotary_dim=rd, interleaved=interleaved)
+    positions = rng.integers(-2 ** 30, 2 ** 30, tokens).tolist()
+    tp = gpu.tensor(positions, dtype=gpu.int64).cuda()
+    at = [0, tokens // 2, tokens - 1]
+    some = [positions[i] for i in at]
+    for turn, backward in ((rotary.rotate, False), (rotary.rotate_backward, True)):
+        want = op.rotate(x[at], some, r.inv_freq, r.factor, interleaved, backward)
+        out = gpu.full_like(tx, float("nan"))
+        turn(tx, tp, r, out=out)
+        assert (np.abs(out.float().cpu().numpy()[at] - want) <= _tolerance(x[at], want, r, some, dtype)).all()
+        assert gpu.equal(out[..., rd:], tx[..., rd:]) and not out.isnan().any()
+        same = tx.clone()
+        assert gpu.equal(turn(same, tp, r, out=same), out)
+        # the same rows 8 bytes on, with 8 bytes between the heads
+        pad = 8 // tx.element_size()
+        room = gpu.full((tokens * heads * (d + pad) + pad,), float("nan"), dtype=tx.dtype, device="cuda")
+        view = room[pad:].view(tokens, heads, d + pad)[..., :d]
+        view.copy_(tx)
+        assert gpu.equal(turn(view, tp, r, out=view), out)
+        assert int(room.isnan().sum()) == pad * (tokens * heads + 1)
