@@ -6,4 +6,4 @@ the reference's ring-attention functions on torch GPU tensors; ``build``
 compiles the library.
 """
 
-__all__ = ["ring_attention", "cache", "build"]
+__all__ = ["ring_attention", "cache", "paged", "rotary", "build"]

@@ -240,7 +240,7 @@ __device__ __forceinline__ uint4 load16(const uint8_t* p) {
 // is two tiles' keys.
 // DP: head_dim, rounded up to 64, 128 or 256 unless EXACT.
 template <int DP, bool EXACT, int PARTS, int VT, bool NT, int W>
-__global__ __launch_bounds__(64 * W, DP * PARTS > 192 || W > 4 ? 1 : 2) void paged_stream_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * W, DP == 256 || W > 4 ? 1 : 2) void paged_stream_kernel(AttnArgs a) {
   typedef typename std::conditional<PARTS == 1, uint16_t, float>::type T;
   constexpr int KJ = DP / 64, DB = DP / 16;  // 16-byte pieces of a key a lane takes; 16-dim blocks
   constexpr int kRows = 16, kPitch = DP + 4;
@@ -248,6 +248,9 @@ __global__ __launch_bounds__(64 * W, DP * PARTS > 192 || W > 4 ? 1 : 2) void pag
   static_assert(VT == 1 || EXACT, "two tiles of V at once");
   __shared__ __attribute__((aligned(16))) float part[W * kRows * kPitch];
   __shared__ float msm[W][kRows], lsm[W][kRows];
+  // Queries of many registers stay in LDS, one copy for all waves.
+  constexpr bool kShared = DP * PARTS > 192 && PARTS > 1;
+  __shared__ __attribute__((aligned(16))) bf16x8 qs[kShared ? PARTS * 2 * KJ * 64 : 1];
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int slot = blockIdx.x / a.units;
@@ -282,29 +285,35 @@ __global__ __launch_bounds__(64 * W, DP * PARTS > 192 || W > 4 ? 1 : 2) void pag
     const int qtok = map.token(c);
     const bool ok = rb * kRows + c < a.R && qtok < count;
     const int lim = ok ? past + qtok + 1 : 0;
-    bf16x8 q[PARTS][2 * KJ];
-    {
-      const int64_t qi = ok ? ((int64_t)s.b * a.p.N + qtok) * a.p.Hq + hk * a.group + map.head(c) : 0;
-      const T* qp = static_cast<const T*>(a.q) + qi * D;
-#pragma unroll
-      for (int j = 0; j < 2 * KJ; ++j) {
-        const int d = 64 * (j >> 1) + 16 * g + 8 * (j & 1);
-        const bool on = ok && (EXACT || d < D);
-        if constexpr (PARTS == 1) {
-          q[0][j] = bf16x8{};
-          if (on) q[0][j] = *reinterpret_cast<const bf16x8*>(qp + d);
-        } else {
-          f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
-          if (on) {
-            lo = load_vec<T, 4>(qp + d);
-            hi = load_vec<T, 4>(qp + d + 4);
-          }
-          bf16x8 y[PARTS];
-          split8<PARTS>(lo, hi, y);
-#pragma unroll
-          for (int p = 0; p < PARTS; ++p) q[p][j] = y[p];
+    const int64_t qi = ok ? ((int64_t)s.b * a.p.N + qtok) * a.p.Hq + hk * a.group + map.head(c) : 0;
+    const T* qp = static_cast<const T*>(a.q) + qi * D;
+    auto qload = [&](int j, bf16x8 (&x)[PARTS]) {
+      const int d = 64 * (j >> 1) + 16 * g + 8 * (j & 1);
+      const bool on = ok && (EXACT || d < D);
+      if constexpr (PARTS == 1) {
+        x[0] = bf16x8{};
+        if (on) x[0] = *reinterpret_cast<const bf16x8*>(qp + d);
+      } else {
+        f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+        if (on) {
+          lo = load_vec<T, 4>(qp + d);
+          hi = load_vec<T, 4>(qp + d + 4);
         }
+        split8<PARTS>(lo, hi, x);
       }
+    };
+    bf16x8 q[kShared ? 1 : 2 * KJ][PARTS];
+    if constexpr (kShared) {
+      for (int j = wave; j < 2 * KJ; j += W) {
+        bf16x8 x[PARTS];
+        qload(j, x);
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) qs[(j * PARTS + p) * 64 + lane] = x[p];
+      }
+      __syncthreads();
+    } else {
+#pragma unroll
+      for (int j = 0; j < 2 * KJ; ++j) qload(j, q[j]);
     }
     if (t0 < t1) run.scales(a, hk);
 
@@ -384,16 +393,24 @@ __global__ __launch_bounds__(64 * W, DP * PARTS > 192 || W > 4 ? 1 : 2) void pag
 #pragma unroll
       for (int mb = 0; mb < 4; ++mb) sc[mb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < KJ; ++j)
+      for (int j = 0; j < KJ; ++j) {
+        bf16x8 ql[PARTS], qh[PARTS];
+        const int at = kShared ? opaque(lane) : 0;  // (read here in every tile)
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+          ql[p] = kShared ? qs[(2 * j * PARTS + p) * 64 + at] : q[kShared ? 0 : 2 * j][p];
+          qh[p] = kShared ? qs[((2 * j + 1) * PARTS + p) * 64 + at] : q[kShared ? 0 : 2 * j + 1][p];
+        }
 #pragma unroll
         for (int mb = 0; mb < 4; ++mb) {
           const bf16x8 lo = bf16_of(kr[mb][j].x, kr[mb][j].y, ks), hi = bf16_of(kr[mb][j].z, kr[mb][j].w, ks);
 #pragma unroll
           for (int p = PARTS - 1; p >= 0; --p) {
-            sc[mb] = mfma16x16x32(lo, q[p][2 * j], sc[mb]);
-            sc[mb] = mfma16x16x32(hi, q[p][2 * j + 1], sc[mb]);
+            sc[mb] = mfma16x16x32(lo, ql[p], sc[mb]);
+            sc[mb] = mfma16x16x32(hi, qh[p], sc[mb]);
           }
         }
+      }
       if (t + 1 < t1) {
         const int step = t + 1 - tb & 15;
         if (step == 0) {

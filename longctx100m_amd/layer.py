@@ -663,7 +663,7 @@ class PagedCache:
         c = PagedCache(cfg, pages=4096, sequences=32, device="cuda")
         a, b = c.open(), c.open()
         logits = c.extend([a, b], [prompt_a, prompt_b], weights)  # [2, vocab]
-        logits = c.extend([a, b], [next_a, next_b], weights)      # one token each, or drafts
+        logits = c.extend([a, b], [next_a, next_b], weights)      # one token each, or more
         c.close(a)                                                # its pages are free again
 
     ``rows[slot]`` tokens of a sequence are held.  ``rotary`` is the model's rotation,
