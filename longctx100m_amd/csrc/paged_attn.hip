@@ -248,7 +248,9 @@ __global__ __launch_bounds__(64 * W, DP == 256 || W > 4 ? 1 : 2) void paged_stre
   static_assert(VT == 1 || EXACT, "two tiles of V at once");
   __shared__ __attribute__((aligned(16))) float part[W * kRows * kPitch];
   __shared__ float msm[W][kRows], lsm[W][kRows];
-  // Queries of many registers stay in LDS, one copy for all waves.
+  // The parts of fp32 queries of 128 dims and more stay in LDS, a copy for all waves:
+  // 48 registers fewer, with which two waves fit a SIMD (512 tokens of 32/8 heads of
+  // 128 over 4,000 rows 125 us, 170 with the parts in registers; 64 over 16,001 69, 91).
   constexpr bool kShared = DP * PARTS > 192 && PARTS > 1;
   __shared__ __attribute__((aligned(16))) bf16x8 qs[kShared ? PARTS * 2 * KJ * 64 : 1];
 
