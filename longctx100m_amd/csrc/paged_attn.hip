@@ -537,7 +537,7 @@ __global__ __launch_bounds__(64 * W, DP == 256 || W > 4 ? 1 : 2) void paged_stre
 // ------------------------------------------------------ many query rows --
 
 // Bound by the products and the softmax beside them: 2,048 tokens of 32/8 heads of
-// 128 behind 16,001 take 580 us, 985 TFLOP/s; a large library product reaches
+// 128 behind 16,001 take 565 us, 1,010 TFLOP/s; a large library product reaches
 // 1,172, and keeping the tile in 8 bits in LDS would have each wave convert all of
 // it.  Eight waves of 32 rows share 64-key tiles of K and V^T, which the threads
 // read from the pages as codes, 16 bytes at a time, one tile ahead, and write to
@@ -549,7 +549,10 @@ __global__ __launch_bounds__(64 * W, DP == 256 || W > 4 ? 1 : 2) void paged_stre
 // the order 0-3, 8-11, 4-7, 12-15, so that the eight of a lane half are one 16-byte
 // read, and P^T needs no shuffle.  Chunks of 16 bytes of an LDS row of 128 bytes are
 // XOR-swizzled by (row / 2) % 8, for reads without bank conflicts (tile128.h has
-// the lane groups of a ds_read_b128).
+// the lane groups of a ds_read_b128).  A wave issues a VALU instruction in 8 cycles at
+// best, two on a SIMD one in 4, and 128-dim rows leave registers for two: the products
+// are 46% of the cycles, and neither earlier reads of LDS, nor half of the waves a phase
+// behind, nor O's products beside the next tile's S changed more than 1%.
 template <int D>
 __global__ __launch_bounds__(512, 1) void paged_tile_kernel(AttnArgs a) {
   constexpr int BN = 64, RW = 8, KT = D / 16, DB = D / 32;  // products of S over the dims; 32-dim blocks
@@ -597,8 +600,12 @@ __global__ __launch_bounds__(512, 1) void paged_tile_kernel(AttnArgs a) {
   const int krow = tid / (D / 16), kch = tid % (D / 16);
   const int vdim = (D == 128 ? tid : tid - kStageK) >> 2, vg = tid & 3;
   const int kg = __builtin_amdgcn_readfirstlane(krow >> 4) & 3;  // (uniform in the wave)
-  const int64_t head_bytes = (int64_t)D << a.shift;
+  const int64_t head_bytes = (int64_t)D << a.shift, page_bytes = pool.Hkv * head_bytes;
+  const uint8_t* const kpages = pool.k + hk * head_bytes;
+  const uint8_t* const vpages = pool.v + hk * head_bytes;
   const int page_mask = (1 << a.shift) - 1;
+  const uint32_t kat = (krow & 15) * D + 16 * kch;                // in a page, from its group's first row
+  const uint32_t vat = (vdim << a.shift) + (16 * vg & page_mask);  // from its tile's first row
   const int kdst = krow * 2 * D + 16 * ((2 * kch) ^ (D == 128 ? t128::swz(krow) : (krow >> 1) & 7));
   const int vdst = vdim * 128 + 16 * ((2 * vg) ^ ((vdim >> 1) & 7));
   PageRun run;
@@ -613,10 +620,8 @@ __global__ __launch_bounds__(512, 1) void paged_tile_kernel(AttnArgs a) {
     const int x = 4 * (j & 15) + kg;
     const int page = max(__builtin_amdgcn_readlane(ahead ? run.next : run.page, x), 0);
     kscale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ahead ? run.nks : run.ks), x));
-    if (do_k) {
-      const int row = (BN * (t0 + j) + 16 * kg & page_mask) + (krow & 15);
-      kw = *reinterpret_cast<const uint4*>(pool.k + ((int64_t)page * pool.Hkv + hk) * head_bytes + row * D + 16 * kch);
-    }
+    const int row = BN * (t0 + j) + 16 * kg & page_mask;
+    if (do_k) kw = *reinterpret_cast<const uint4*>(kpages + page * page_bytes + row * D + kat);
   };
   auto vload = [&](int j) {
     gone = gone_next;
@@ -626,13 +631,19 @@ __global__ __launch_bounds__(512, 1) void paged_tile_kernel(AttnArgs a) {
       run.look(a, table, t0 + j + 16, k1);
     }
     const int x = 4 * (j & 15);
-    gone_next = (uint32_t)(__ballot(run.page < 0) >> x) & 15u;
-    vscale = __shfl(run.vs, x + vg, 64);
-    const int page = max(__shfl(run.page, x + vg, 64), 0);
-    if (do_v) {
-      const int row = BN * (t0 + j) + 16 * vg & page_mask;
-      vw = *reinterpret_cast<const uint4*>(pool.v + ((int64_t)page * pool.Hkv + hk) * head_bytes +
-                                           ((int64_t)vdim << a.shift) + row);
+    const int row = BN * (t0 + j) & page_mask;
+    // One page: its address and scale are the workgroup's (2% of the time of 2,048
+    // tokens).
+    if (page_mask >= BN - 1) {
+      const int page = __builtin_amdgcn_readlane(run.page, x);
+      gone_next = page < 0 ? 15 : 0;
+      vscale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(run.vs), x));
+      if (do_v) vw = *reinterpret_cast<const uint4*>(vpages + max(page, 0) * page_bytes + row + vat);
+    } else {
+      gone_next = (uint32_t)(__ballot(run.page < 0) >> x) & 15u;
+      vscale = __shfl(run.vs, x + vg, 64);
+      const int page = max(__shfl(run.page, x + vg, 64), 0);
+      if (do_v) vw = *reinterpret_cast<const uint4*>(vpages + page * page_bytes + row + vat);
     }
   };
   auto kwrite = [&](int j, auto parity) {  // parity: j % 2
@@ -644,12 +655,13 @@ __global__ __launch_bounds__(512, 1) void paged_tile_kernel(AttnArgs a) {
   auto vwrite = [&](int j, auto parity) {
     constexpr int P = decltype(parity)::value;
     if (j >= ntiles) return;
+    const bool edge = BN * (t0 + j) + BN > all_clear;
+    if (edge || gone_next != 0) {
+      const bool none = gone_next >> vg & 1;
+      if (edge && do_v) strange |= clean_values(vw, none ? 0 : k1 - (BN * (t0 + j) + 16 * vg));
+      else if (none) vw = make_uint4(0u, 0u, 0u, 0u);
+    }
     if (!do_v) return;
-    const bool none = gone_next >> vg & 1;
-    if (BN * (t0 + j) + BN > all_clear)
-      strange |= clean_values(vw, none ? 0 : k1 - (BN * (t0 + j) + 16 * vg));
-    else if (none)
-      vw = make_uint4(0u, 0u, 0u, 0u);
     *reinterpret_cast<bf16x8*>(vbuf + P * kTileB + vdst) = bf16_of(vw.x, vw.z, vscale);
     *reinterpret_cast<bf16x8*>(vbuf + P * kTileB + (vdst ^ 16)) = bf16_of(vw.y, vw.w, vscale);
   };
@@ -716,7 +728,18 @@ __global__ __launch_bounds__(512, 1) void paged_tile_kernel(AttnArgs a) {
       A[0] = kread(kt, 0);
       A[1] = kread(kt, 1);
     }
-    float pmax = -INFINITY, muse = 0.f, sum = 0.f;  // (sum: as in the streaming form)
+    float pmax = -INFINITY, muse = 0.f, sum[2] = {0.f, 0.f};  // (sum: as in the streaming form)
+    auto argument = [&](int e) { sc[e >> 4][e & 15] = fmaf(sc[e >> 4][e & 15], a.sl2, -muse); };
+    auto exponential = [&](int e) { sc[e >> 4][e & 15] = fast_exp2(sc[e >> 4][e & 15]); };
+    auto add = [&](int e) { sum[e & 1] += sc[e >> 4][e & 15]; };
+    auto pack = [&](int mb) {  // the B operands of keys 32 mb .. 32 mb + 31
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int e = 8 * u;
+        pb[2 * mb + u] = pack_bf16x8(f32x4{sc[mb][e], sc[mb][e + 1], sc[mb][e + 2], sc[mb][e + 3]},
+                                     f32x4{sc[mb][e + 4], sc[mb][e + 5], sc[mb][e + 6], sc[mb][e + 7]});
+      }
+    };
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int st = 0; st < S; ++st) {
@@ -746,29 +769,24 @@ __global__ __launch_bounds__(512, 1) void paged_tile_kernel(AttnArgs a) {
         }
         muse = mrun == -INFINITY ? 0.f : mrun;
       }
-      if (st >= 8) {  // probabilities, 4 per step
+      // Probabilities, 4 per step, each in three steps, argument, exponential and sum, so
+      // that nothing waits for the instruction before it.
+      if (st >= 7)
 #pragma unroll
-        for (int e = 4 * (st - 8); e < 4 * (st - 8) + 4; ++e) {
-          const int mb = e >> 4, v = e & 15;
-          const float p = fast_exp2(fmaf(sc[mb][v], a.sl2, -muse));
-          sum += p;
-          sc[mb][v] = p;
+        for (int k = 0; k < 4; ++k) {
+          if (st >= 8) exponential(4 * (st - 8) + k);
+          if (st < 15) argument(4 * (st - 7) + k);
+          if (st >= 9) add(4 * (st - 9) + k);
         }
-        if (st == 15) lsum += sum;
-      }
-      if (st == 11 || st == 15) {  // B operands of keys 32 mb .. 32 mb + 31
-        const int mb = (st - 11) >> 2;
-#pragma unroll
-        for (int u2 = 0; u2 < 2; ++u2) {
-          const int e0 = 8 * u2;
-          pb[2 * mb + u2] = pack_bf16x8(f32x4{sc[mb][e0], sc[mb][e0 + 1], sc[mb][e0 + 2], sc[mb][e0 + 3]},
-                                        f32x4{sc[mb][e0 + 4], sc[mb][e0 + 5], sc[mb][e0 + 6], sc[mb][e0 + 7]});
-        }
-      }
+      if (st == 12) pack(0);
       if (st == 14) B[0] = vread(vt, 0);
       if (st == 15) B[1] = vread(vt, 1);
       __builtin_amdgcn_sched_barrier(0);
     }
+#pragma unroll
+    for (int k = 28; k < 32; ++k) add(k);
+    pack(1);
+    lsum += sum[0] + sum[1];
 #pragma unroll
     for (int n = 0; n < 4 * DB; ++n) {
       o[n % DB] = mfma32x32x16(B[n & 1], pb[n / DB], o[n % DB]);
