@@ -537,7 +537,7 @@ __global__ __launch_bounds__(64 * W, DP == 256 || W > 4 ? 1 : 2) void paged_stre
 // ------------------------------------------------------ many query rows --
 
 // Bound by the products and the softmax beside them: 2,048 tokens of 32/8 heads of
-// 128 behind 16,001 take 565 us, 1,010 TFLOP/s; a large library product reaches
+// 128 behind 16,001 take 566 us, 1,007 TFLOP/s; a large library product reaches
 // 1,172, and keeping the tile in 8 bits in LDS would have each wave convert all of
 // it.  Eight waves of 32 rows share 64-key tiles of K and V^T, which the threads
 // read from the pages as codes, 16 bytes at a time, one tile ahead, and write to
