@@ -551,7 +551,7 @@ __global__ __launch_bounds__(64 * W, DP == 256 || W > 4 ? 1 : 2) void paged_stre
 // XOR-swizzled by (row / 2) % 8, for reads without bank conflicts (tile128.h has
 // the lane groups of a ds_read_b128).  A wave issues a VALU instruction in 8 cycles at
 // best, two on a SIMD one in 4, and 128-dim rows leave registers for two: the products
-// are 46% of the cycles, and neither earlier reads of LDS, nor half of the waves a phase
+// are 48% of the cycles, and neither earlier reads of LDS, nor half of the waves a phase
 // behind, nor O's products beside the next tile's S changed more than 1%.
 template <int D>
 __global__ __launch_bounds__(512, 1) void paged_tile_kernel(AttnArgs a) {

@@ -709,3 +709,46 @@ def test_the_workspace_holds_what_the_query_says(monkeypatch):
     c = _lib.Paged(1, 1, 32, 8, 128, 1, 4096, 64, 4096, 0)
     need = lib.lc_paged_attn_workspace_bytes(ctypes.byref(c))
     assert 0 < need < 1 << 26
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wide", [False, True], ids=["", "wide"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [64, 128])
+@pytest.mark.parametrize("n", [1, 50, 140])
+def test_pages_of_whole_tiles(gpu, n, rows, d, wide):
+    """Pages that hold one or two 64-key tiles: missing ones in the middle and at the
+    end, NaN and NaN scales wherever nobody looks, a NaN that some tokens see."""
+    rng = np.random.default_rng(n + rows)
+    hq, hkv, past, counts = 8, 2, [5 * rows + 3, 0, 2 * rows - 1], [n, max(n - 3, 1), n]
+    table, pages = _table(rng, past, n, rows)
+    table[0, 1], table[0, 4], table[2, 0] = -1, pages + 5, -3
+    pool = _pool(rng, pages, rows, hkv, d)
+    q, _ = _rows(gpu, rng, 3, n, hq, d, "bf16", 1.5)
+    if wide:
+        table = _wide(table, q, pool)
+    want = op.attention(q, pool, table, past, counts)
+    seen = np.zeros((pages, rows), bool)
+    for b in range(3):
+        for r in range(past[b] + counts[b]):
+            if 0 <= table[b][r // rows] < pages:
+                seen[table[b][r // rows], r % rows] = True
+    clean = {x: y.copy() for x, y in pool.items()}
+    pool["k"].transpose(0, 2, 1, 3)[~seen] = np.nan
+    pool["v"].transpose(0, 3, 1, 2)[~seen] = np.nan
+    for name in ("k_scale", "v_scale"):
+        pool[name][~seen.any(1)] = np.nan
+    _check_attention(_attend(gpu, q, _to_pages(gpu, pool), table, past, counts, "bf16"), want, q, clean, "bf16")
+    # one token in the middle of the new ones, and one that all see
+    for row, first in ((past[0] + n // 2, n // 2), (2 * rows + 5, 0)):
+        at = table[0][row // rows], 1, 3, row % rows
+        was, pool["v"][at] = pool["v"][at], np.nan
+        got = _attend(gpu, q, _to_pages(gpu, pool), table, past, counts, "bf16")
+        only = np.zeros(got[0].shape, bool)
+        only[0, first:, hq // 2:, 3] = True
+        assert np.array_equal(got[0].isnan().cpu().numpy(), only)
+        pool["v"][at] = was
+    # a table that ends inside the new tokens' rows, or before them
+    short = table[:, :max(2, (past[0] + n // 2) // rows)]
+    want = op.attention(q, clean, short, past, counts)
+    _check_attention(_attend(gpu, q, _to_pages(gpu, pool), short, past, counts, "bf16"), want, q, clean, "bf16")
