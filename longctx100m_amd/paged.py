@@ -40,7 +40,8 @@ PAGE_ROWS = (16, 32, 64, 128)
 class Pages:
     """The pool of a layer: ``k`` [pages, Hkv, rows, D] and ``v`` [pages, Hkv, D, rows]
     in float8_e4m3fn, ``k_scale`` and ``v_scale`` [pages, Hkv] fp32.  A row's K is its
-    codes times its page's scale."""
+    codes times its page's scale.  The attributes cannot be set: another pool is another
+    ``Pages``."""
 
     def __init__(self, pages: int, rows: int, kv_heads: int, head_dim: int, device="cuda"):
         def codes(*shape):
@@ -73,15 +74,20 @@ class Pages:
             raise ValueError(f"a page has {PAGE_ROWS} rows, got {rows}")
         if max(n, h, d) >= 2 ** 31 or min(n, h, d) == 0:
             raise ValueError(f"a pool of shape {tuple(k.shape)}")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.count, self.kv_heads, self.rows, self.head_dim = n, h, rows, d
-        self._device = k.get_device() if k.is_cuda else -1
-        self._ptrs = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
+        self.__dict__.update(k=k, v=v, k_scale=k_scale, v_scale=v_scale, count=n, kv_heads=h, rows=rows, head_dim=d)
+
+    def __setattr__(self, name, value):  # the checks above hold for these tensors
+        raise AttributeError(f"{name} of a pool cannot be set: Pages.of makes a pool of other tensors")
+
+    # Asked of the tensors at every call: a copied or unpickled pool has its own.
+    @property
+    def _ptrs(self) -> Tuple[int, int, int, int]:
+        return self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr()
 
     def device(self) -> int:
-        if self._device < 0:
+        if not self.k.is_cuda:
             raise ValueError("tensors must live on the GPU (device pointers are passed to HIP)")
-        return self._device
+        return self.k.get_device()
 
 
 def _describe(pages: Pages, table: torch.Tensor, b: int, n: int, heads_q: int, dtype: int) -> _lib.Paged:

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from longctx100m_amd import layer as ly
+from longctx100m_amd import paged
 from longctx100m_amd import rotary as rot
 
 CFG = ly.ModelConfig(hidden_size=64, num_heads=4, num_key_value_heads=2, intermediate_size=64, num_layers=2,
@@ -143,3 +144,25 @@ def test_a_layer_needs_tokens_of_every_sequence():
     for rows, b in ((5, 2), (0, 2), (3, 0)):
         with pytest.raises(ValueError, match="sequences"):
             ly.layer_extend_paged(torch.zeros(rows, 64), {}, CFG, None, None, torch.zeros(b, 1), None)
+
+
+def test_a_pool_has_its_own_addresses():
+    """Copies of a pool are pools of their own tensors, and a pool's tensors and sizes,
+    which the kernels' addresses and bounds come from, cannot be replaced."""
+    import copy
+    import io
+
+    p = paged.Pages(3, 16, 2, 64, device="cpu")
+    file = io.BytesIO()
+    torch.save(p, file)
+    file.seek(0)
+    for q in (copy.deepcopy(p), torch.load(file, weights_only=False)):
+        assert q._ptrs == tuple(t.data_ptr() for t in (q.k, q.v, q.k_scale, q.v_scale))
+        assert not set(q._ptrs) & set(p._ptrs)
+        assert (q.count, q.kv_heads, q.rows, q.head_dim) == (3, 2, 16, 64)
+    assert copy.copy(p)._ptrs == p._ptrs
+    for name in ("k", "v", "k_scale", "v_scale", "rows", "count", "kv_heads", "head_dim"):
+        with pytest.raises(AttributeError, match="Pages.of"):
+            setattr(p, name, getattr(p, name))
+    p.k.set_(torch.zeros(3, 2, 16, 64, dtype=torch.uint8).view(torch.float8_e4m3fn))
+    assert p._ptrs[0] == p.k.data_ptr()
