@@ -20,7 +20,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from typing import Dict, List, Optional, Sequence, Tuple, Union
+from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -93,35 +93,36 @@ class Rotary:
     """A model's rotation: ``Rotary(head_dim, theta)`` with ``rotary_dim`` (all of the
     head), ``interleaved`` pairs and ``scaling`` as :func:`frequencies` takes it, or
     with ``inv_freq`` (and ``factor``) given instead.  Keeps the frequencies on
-    ``device``."""
+    ``device``.  The attributes cannot be set: another rotation is another ``Rotary``."""
 
     def __init__(self, head_dim: int, theta: float = 10000.0, *, rotary_dim: Optional[int] = None,
                  interleaved: bool = False, scaling: Optional[dict] = None,
                  inv_freq: Optional[Sequence[float]] = None, factor: Optional[float] = None, device="cuda"):
-        self.head_dim = int(head_dim)
+        head_dim = int(head_dim)
         if inv_freq is not None:
             if scaling is not None:
                 raise ValueError("inv_freq comes in place of scaling")
-            self.inv_freq = [float(x) for x in inv_freq]
-            own = 1.0
-            if rotary_dim is not None and rotary_dim != 2 * len(self.inv_freq):
+            inv_freq, own = [float(x) for x in inv_freq], 1.0
+            if rotary_dim is not None and rotary_dim != 2 * len(inv_freq):
                 raise ValueError("inv_freq needs rotary_dim / 2 values")
-            rotary_dim = 2 * len(self.inv_freq)
+            rotary_dim = 2 * len(inv_freq)
         else:
-            rotary_dim = self.head_dim if rotary_dim is None else int(rotary_dim)
-            self.inv_freq, own = frequencies(rotary_dim, float(theta), scaling)
-        self.rotary_dim, self.interleaved = rotary_dim, bool(interleaved)
-        self.factor = own if factor is None else float(factor)
-        if not 0 < self.head_dim <= 256 or not 0 < rotary_dim <= self.head_dim:
+            rotary_dim = head_dim if rotary_dim is None else int(rotary_dim)
+            inv_freq, own = frequencies(rotary_dim, float(theta), scaling)
+        if not 0 < head_dim <= 256 or not 0 < rotary_dim <= head_dim:
             raise ValueError(f"rotary_dim ({rotary_dim}) must be positive and at most head_dim "
-                             f"({self.head_dim}), and that at most 256")
+                             f"({head_dim}), and that at most 256")
         n = rotary_dim // 2
         turns = (ctypes.c_uint64 * n)()
-        _lib.check(_lib.load().lc_rotary_turns(n, (ctypes.c_double * n)(*self.inv_freq), turns))
+        _lib.check(_lib.load().lc_rotary_turns(n, (ctypes.c_double * n)(*inv_freq), turns))
         # (two's complement: torch has no arithmetic on uint64, nor needs any here)
         host = torch.tensor([x - (x >> 63 << 64) for x in turns], dtype=torch.int64)
-        self.turns = host.to(device)
-        self._c: Dict[int, _lib.Rotary] = {}
+        self.__dict__.update(head_dim=head_dim, rotary_dim=rotary_dim, interleaved=bool(interleaved),
+                             inv_freq=inv_freq, factor=own if factor is None else float(factor),
+                             turns=host.to(device))
+
+    def __setattr__(self, name, value):  # turns follow from the rest
+        raise AttributeError(f"{name} of a rotation cannot be set: make another Rotary")
 
     @classmethod
     def of(cls, rope: _lib.Rope, device="cuda") -> "Rotary":
@@ -140,13 +141,9 @@ class Rotary:
 
     def on(self, device: int) -> _lib.Rotary:
         """The rotation as the C ABI takes it, for tensors of that GPU."""
-        c = self._c.get(device)
-        if c is None:
-            if not self.turns.is_cuda or self.turns.get_device() != device:
-                raise ValueError(f"the rotary frequencies live on {self.turns.device}, not on cuda:{device}")
-            c = self._c[device] = _lib.Rotary(self.head_dim, self.rotary_dim, int(self.interleaved), self.factor,
-                                              self.turns.data_ptr())
-        return c
+        if self.turns.get_device() != device:
+            raise ValueError(f"the rotary frequencies live on {self.turns.device}, not on cuda:{device}")
+        return _lib.Rotary(self.head_dim, self.rotary_dim, self.interleaved, self.factor, self.turns.data_ptr())
 
 
 def heads_of(t: torch.Tensor, shape: Sequence[int], name: str) -> _lib.Rows:

@@ -166,3 +166,24 @@ def test_a_pool_has_its_own_addresses():
             setattr(p, name, getattr(p, name))
     p.k.set_(torch.zeros(3, 2, 16, 64, dtype=torch.uint8).view(torch.float8_e4m3fn))
     assert p._ptrs[0] == p.k.data_ptr()
+
+
+def test_a_rotation_stays_as_it_is_made(monkeypatch):
+    """What the C ABI is given follows from the attributes, of which none can be set,
+    and a copy of a rotation that was used has frequencies of its own."""
+    import copy
+
+    r = rot.Rotary(64, 10000.0, rotary_dim=32, interleaved=True, factor=0.5, device="cpu")
+    for name, value in (("factor", 2.0), ("turns", r.turns.clone()), ("interleaved", False), ("rotary_dim", 64),
+                        ("head_dim", 128), ("inv_freq", [1.0] * 16)):
+        with pytest.raises(AttributeError, match="another Rotary"):
+            setattr(r, name, value)
+    with pytest.raises(ValueError, match="live on cpu"):
+        r.on(0)
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True)
+    for x in (r, copy.deepcopy(r), copy.copy(r)):
+        c = x.on(0)
+        assert (c.head_dim, c.rotary_dim, c.interleaved, c.factor) == (64, 32, 1, 0.5)
+        assert c.turns == x.turns.data_ptr()
+    assert copy.deepcopy(r).on(0).turns != r.on(0).turns
