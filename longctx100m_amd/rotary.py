@@ -10,7 +10,7 @@ a radian at 10^7.  Here
   * pairs lie half the rotated part apart, or side by side (``interleaved``);
   * the first ``rotary_dim`` dims of a head turn, the others stay;
   * angles are 64-bit fractions of a turn: right to 2^-38 of a turn at 10^8;
-  * the backward pass is there.
+  * the backward pass is there, and autograd takes it.
 
 A :class:`Rotary` holds what a model's rotation is; kernels run on the current
 stream of the tensors' device and nothing synchronises.
@@ -195,15 +195,44 @@ def _turn(x: torch.Tensor, positions: Union[torch.Tensor, int], rotary: Rotary, 
     return out
 
 
+class _Rotate(torch.autograd.Function):
+    """The rotation, or its transpose (inverse = 1), each of which is the other's gradient."""
+
+    @staticmethod
+    def forward(ctx, x, positions, rotary, inverse):
+        at = isinstance(positions, torch.Tensor)
+        ctx.save_for_backward(*[positions] if at else [])
+        ctx.args = None if at else positions, rotary, inverse
+        return _turn(x, positions, rotary, None, inverse)
+
+    @staticmethod
+    def backward(ctx, grad):
+        first, rotary, inverse = ctx.args
+        positions = ctx.saved_tensors[0] if first is None else first
+        if grad.stride(-1) != 1:  # (of a sum: one element for all)
+            grad = grad.contiguous()
+        return _Rotate.apply(grad, positions, rotary, 1 - inverse), None, None, None
+
+
+def _differentiable(x, positions, rotary, out, inverse: int) -> torch.Tensor:
+    if not (isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled()):
+        return _turn(x, positions, rotary, out, inverse)
+    if out is not None:
+        raise ValueError("rows that need a gradient are not rotated into out: leave it away, or use torch.no_grad()")
+    return _Rotate.apply(x, positions, rotary, inverse)
+
+
 def rotate(x: torch.Tensor, positions: Union[torch.Tensor, int], rotary: Rotary, *,
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Turns the rows x [(batch,) tokens, heads, head_dim] (bf16 or fp32, any strides
     with contiguous head_dim) to ``positions``: int64 [(batch,) tokens] on the GPU,
-    or the number of each sequence's first one.  ``out`` may be x."""
-    return _turn(x, positions, rotary, out, 0)
+    or the number of each sequence's first one.  ``out`` may be x.  Differentiable in x
+    where no ``out`` is given."""
+    return _differentiable(x, positions, rotary, out, 0)
 
 
 def rotate_backward(grad: torch.Tensor, positions: Union[torch.Tensor, int], rotary: Rotary, *,
                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """The gradient of :func:`rotate`'s x from that of its result."""
-    return _turn(grad, positions, rotary, out, 1)
+    """The gradient of :func:`rotate`'s x from that of its result (which autograd calls by
+    itself)."""
+    return _differentiable(grad, positions, rotary, out, 1)

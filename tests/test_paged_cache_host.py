@@ -187,3 +187,40 @@ def test_a_rotation_stays_as_it_is_made(monkeypatch):
         assert (c.head_dim, c.rotary_dim, c.interleaved, c.factor) == (64, 32, 1, 0.5)
         assert c.turns == x.turns.data_ptr()
     assert copy.deepcopy(r).on(0).turns != r.on(0).turns
+
+
+def test_rotate_is_differentiable(monkeypatch):
+    """Autograd reaches x through rotate and rotate_backward, by the kernel of the other,
+    twice if asked; a result in ``out`` has no graph, so it is refused where a gradient is
+    wanted."""
+    calls = []
+
+    def turn(x, positions, rotary, out, inverse):  # what the kernel does: (half layout, whole head)
+        assert x.stride(-1) == 1
+        at = positions if isinstance(positions, torch.Tensor) else positions + torch.arange(x.shape[0])
+        angle = at.double()[:, None, None] * torch.tensor(rotary.inv_freq, dtype=torch.float64) * (-1) ** inverse
+        a, b = x.detach().chunk(2, -1)
+        calls.append(inverse)
+        return torch.cat((a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin()), -1) * rotary.factor
+
+    monkeypatch.setattr(rot, "_turn", turn)
+    r = rot.Rotary(8, 100.0, factor=1.5, device="cpu")
+    gen = torch.Generator().manual_seed(0)
+    x = torch.randn(5, 3, 8, dtype=torch.float64, generator=gen, requires_grad=True)
+    for at in (torch.tensor([4, 0, 100, -3, 7]), 9):
+        for f in (rot.rotate, rot.rotate_backward):
+            assert torch.autograd.gradcheck(lambda y: f(y, at, r), (x,))
+            assert torch.autograd.gradgradcheck(lambda y: f(y, at, r), (x,))
+            calls.clear()
+            (g,) = torch.autograd.grad(f(x, at, r).sum(), x)  # the gradient of a sum: strides of zero
+            assert torch.equal(g, turn(torch.ones_like(x), at, r, None, int(f is rot.rotate)))
+            with pytest.raises(ValueError, match="no_grad"):
+                f(x, at, r, out=torch.empty_like(x))
+            with torch.no_grad():
+                assert not f(x, at, r, out=torch.empty_like(x)).requires_grad
+            assert not f(x.detach(), at, r, out=torch.empty_like(x)).requires_grad
+    at = torch.tensor([4, 0, 100, -3, 7])
+    y = rot.rotate(x, at, r).sum()
+    at += 1  # the backward pass would take other angles
+    with pytest.raises(RuntimeError, match="modified"):
+        y.backward()
