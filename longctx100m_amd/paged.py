@@ -37,10 +37,21 @@ from .rotary import Rotary, heads_of
 PAGE_ROWS = (16, 32, 64, 128)
 
 
+def _check_scales(scale: torch.Tensor, name: str) -> None:
+    bits = scale.view(torch.int32)
+    bad = ((bits & 0x7fffff) != 0) | (bits < 0) | (bits > 247 << 23)  # (2^120: of the largest finite values)
+    bad = (bad & (scale == scale)).nonzero()
+    if bad.numel():
+        page, head = bad[0].tolist()
+        raise ValueError(f"{name}[{page}, {head}] = {float(scale[page, head])} is no power of two from 2^-126 to 2^120 "
+                         "(nor 0 or NaN, of a page that is not in use)")
+
+
 class Pages:
     """The pool of a layer: ``k`` [pages, Hkv, rows, D] and ``v`` [pages, Hkv, D, rows]
     in float8_e4m3fn, ``k_scale`` and ``v_scale`` [pages, Hkv] fp32.  A row's K is its
-    codes times its page's scale.  The attributes cannot be set: another pool is another
+    codes times its page's scale, which is a power of two (csrc/e4m3.h has why); those of
+    pages not in use may be 0 or NaN.  The attributes cannot be set: another pool is another
     ``Pages``."""
 
     def __init__(self, pages: int, rows: int, kv_heads: int, head_dim: int, device="cuda"):
@@ -52,9 +63,14 @@ class Pages:
 
     @classmethod
     def of(cls, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> "Pages":
-        """A pool in tensors that are there already."""
+        """A pool in tensors that are there already.  Scales of another kind, such as amax /
+        448, are refused: the kernels take their exponents alone.  (This waits for the GPU,
+        and is left out while a graph is captured.)"""
         p = cls.__new__(cls)
         p._set(k, v, k_scale, v_scale)
+        if not (k.is_cuda and torch.cuda.is_current_stream_capturing()):
+            _check_scales(k_scale, "k_scale")
+            _check_scales(v_scale, "v_scale")
         return p
 
     def _set(self, k, v, k_scale, v_scale):

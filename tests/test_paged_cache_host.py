@@ -224,3 +224,19 @@ def test_rotate_is_differentiable(monkeypatch):
     at += 1  # the backward pass would take other angles
     with pytest.raises(RuntimeError, match="modified"):
         y.backward()
+
+
+def test_scales_are_powers_of_two():
+    """A pool of scales that are none would be read wrongly without a word."""
+    def pool(name, value):
+        p = paged.Pages(3, 16, 2, 64, device="cpu")
+        scales = {"k_scale": p.k_scale.clone(), "v_scale": p.v_scale.clone()}
+        scales[name][2, 1] = value
+        return paged.Pages.of(p.k, p.v, **scales)
+
+    for name in ("k_scale", "v_scale"):
+        for good in (0.0, 1.0, 2.0 ** -126, 2.0 ** 120, 0.25, float("nan")):
+            pool(name, good)
+        for bad in (3.1 / 448, 3.0, 1.0 + 2.0 ** -23, 2.0 ** 121, 2.0 ** -127, 1e-45, -1.0, float("inf"), -0.25):
+            with pytest.raises(ValueError, match=rf"{name}\[2, 1\].*power of two"):
+                pool(name, bad)
