@@ -666,7 +666,8 @@ class PagedCache:
         logits = c.extend([a, b], [next_a, next_b], weights)      # one token each, or more
         c.close(a)                                                # its pages are free again
 
-    ``rows[slot]`` tokens of a sequence are held.  ``rotary`` is the model's rotation,
+    ``rows[slot]`` tokens of a sequence are held; lower it to take the last ones back
+    (drafts that were refused), whose pages the sequence keeps.  ``rotary`` is the model's rotation,
     without one that of the config's rope_theta and rope_scaling with the
     reference's frequencies.  Calls run on one stream: a page that a closed
     sequence leaves is written again without a wait."""
@@ -719,7 +720,10 @@ class PagedCache:
             raise ValueError("a sequence is extended by a 1-D tensor of tokens, one at least")
         held = [self._held(slot) for slot in slots]
         past = [self.rows[slot] for slot in slots]
-        need = [-(-(p + c) // self.page_rows) - len(h) for p, c, h in zip(past, counts, held)]
+        for slot, p, h in zip(slots, past, held):
+            if not 0 <= p <= len(h) * self.page_rows:
+                raise ValueError(f"the pages of the sequence in slot {slot} do not hold {p} rows")
+        need = [max(0, -(-(p + c) // self.page_rows) - len(h)) for p, c, h in zip(past, counts, held)]
         if sum(need) > len(self._free):
             raise ValueError(f"{sum(need)} pages are needed, {len(self._free)} are free")
         taken = self._free[len(self._free) - sum(need):][::-1]

@@ -240,3 +240,30 @@ def test_scales_are_powers_of_two():
         for bad in (3.1 / 448, 3.0, 1.0 + 2.0 ** -23, 2.0 ** 121, 2.0 ** -127, 1e-45, -1.0, float("inf"), -0.25):
             with pytest.raises(ValueError, match=rf"{name}\[2, 1\].*power of two"):
                 pool(name, bad)
+
+
+def test_rows_that_are_taken_back(cache):
+    """A sequence with fewer rows than its pages hold takes none from the others, keeps its
+    pages and writes into them again; rows that it never had are refused."""
+    c, w, calls = cache
+    a, b = c.open(), c.open()
+    c.extend([a, b], [ids(40), ids(3)], w)
+    pa, pb = list(c._pages[a]), list(c._pages[b])
+    c.rows[a] = 10  # two pages more than it needs
+    c.extend([a, b], [ids(1), ids(30)], w)
+    _, table, past, counts = calls[-1]
+    assert past == [10, 3] and counts == [1, 30]
+    assert table[0] == pa and table[1][0] == pb[0]
+    assert all(0 <= x < 6 for x in table[1]) and len(set(table[0] + table[1])) == 6
+    assert c.rows[:2] == [11, 33] and c.free_pages == 0
+    c.extend([a], [ids(37)], w)
+    assert calls[-1][1] == [pa] and c.rows[a] == 48
+    for rows in (-1, 49):
+        c.rows[a] = rows
+        before = len(calls)
+        with pytest.raises(ValueError, match="do not hold"):
+            c.extend([b, a], [ids(1), ids(1)], w)
+        assert len(calls) == before
+    c.close(a)
+    c.close(b)
+    assert sorted(c._free) == list(range(6))
