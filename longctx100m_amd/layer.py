@@ -718,6 +718,8 @@ class PagedCache:
             raise ValueError("extend takes sequences, each once, and tokens for each")
         if min(counts) == 0 or any(t.dim() != 1 for t in ids):
             raise ValueError("a sequence is extended by a 1-D tensor of tokens, one at least")
+        if len(weights["layers"]) != len(self.pools):
+            raise ValueError(f"a cache of {len(self.pools)} layers for weights of {len(weights['layers'])}")
         held = [self._held(slot) for slot in slots]
         past = [self.rows[slot] for slot in slots]
         for slot, p, h in zip(slots, past, held):

@@ -267,3 +267,12 @@ def test_rows_that_are_taken_back(cache):
     c.close(a)
     c.close(b)
     assert sorted(c._free) == list(range(6))
+
+
+def test_weights_of_as_many_layers(cache):
+    c, w, calls = cache
+    a = c.open()
+    for layers in ([{}], [{}, {}, {}]):
+        with pytest.raises(ValueError, match="2 layers"):
+            c.extend([a], [ids(1)], dict(w, layers=layers))
+    assert not calls and c.rows[a] == 0 and c.free_pages == 6
