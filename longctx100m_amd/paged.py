@@ -101,9 +101,10 @@ class Pages:
         return self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr()
 
     def device(self) -> int:
-        if not self.k.is_cuda:
+        device = self.k.get_device()
+        if device < 0:
             raise ValueError("tensors must live on the GPU (device pointers are passed to HIP)")
-        return self.k.get_device()
+        return device
 
 
 def _describe(pages: Pages, table: torch.Tensor, b: int, n: int, heads_q: int, dtype: int) -> _lib.Paged:

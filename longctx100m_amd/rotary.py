@@ -120,6 +120,18 @@ class Rotary:
         self.__dict__.update(head_dim=head_dim, rotary_dim=rotary_dim, interleaved=bool(interleaved),
                              inv_freq=inv_freq, factor=own if factor is None else float(factor),
                              turns=host.to(device))
+        self._describe()
+
+    def _describe(self) -> None:
+        self.__dict__["_c"] = _lib.Rotary(self.head_dim, self.rotary_dim, self.interleaved, self.factor)
+
+    # A copy has a description of its own (which could not be copied: it holds a pointer).
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k != "_c"}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._describe()
 
     def __setattr__(self, name, value):  # turns follow from the rest
         raise AttributeError(f"{name} of a rotation cannot be set: make another Rotary")
@@ -143,7 +155,8 @@ class Rotary:
         """The rotation as the C ABI takes it, for tensors of that GPU."""
         if self.turns.get_device() != device:
             raise ValueError(f"the rotary frequencies live on {self.turns.device}, not on cuda:{device}")
-        return _lib.Rotary(self.head_dim, self.rotary_dim, self.interleaved, self.factor, self.turns.data_ptr())
+        self._c.turns = self.turns.data_ptr()
+        return self._c
 
 
 def heads_of(t: torch.Tensor, shape: Sequence[int], name: str) -> _lib.Rows:
@@ -214,9 +227,7 @@ class _Rotate(torch.autograd.Function):
         return _Rotate.apply(grad, positions, rotary, 1 - inverse), None, None, None
 
 
-def _differentiable(x, positions, rotary, out, inverse: int) -> torch.Tensor:
-    if not (isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled()):
-        return _turn(x, positions, rotary, out, inverse)
+def _with_graph(x, positions, rotary, out, inverse: int) -> torch.Tensor:
     if out is not None:
         raise ValueError("rows that need a gradient are not rotated into out: leave it away, or use torch.no_grad()")
     return _Rotate.apply(x, positions, rotary, inverse)
@@ -228,11 +239,15 @@ def rotate(x: torch.Tensor, positions: Union[torch.Tensor, int], rotary: Rotary,
     with contiguous head_dim) to ``positions``: int64 [(batch,) tokens] on the GPU,
     or the number of each sequence's first one.  ``out`` may be x.  Differentiable in x
     where no ``out`` is given."""
-    return _differentiable(x, positions, rotary, out, 0)
+    if getattr(x, "requires_grad", False) and torch.is_grad_enabled():
+        return _with_graph(x, positions, rotary, out, 0)
+    return _turn(x, positions, rotary, out, 0)
 
 
 def rotate_backward(grad: torch.Tensor, positions: Union[torch.Tensor, int], rotary: Rotary, *,
                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The gradient of :func:`rotate`'s x from that of its result (which autograd calls by
     itself)."""
-    return _differentiable(grad, positions, rotary, out, 1)
+    if getattr(grad, "requires_grad", False) and torch.is_grad_enabled():
+        return _with_graph(grad, positions, rotary, out, 1)
+    return _turn(grad, positions, rotary, out, 1)
