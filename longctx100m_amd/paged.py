@@ -37,14 +37,16 @@ from .rotary import Rotary, heads_of
 PAGE_ROWS = (16, 32, 64, 128)
 
 
-def _check_scales(scale: torch.Tensor, name: str) -> None:
+def _check_scales(k_scale: torch.Tensor, v_scale: torch.Tensor) -> None:
+    scale = torch.stack((k_scale, v_scale))
     bits = scale.view(torch.int32)
-    bad = ((bits & 0x7fffff) != 0) | (bits < 0) | (bits > 247 << 23)  # (2^120: of the largest finite values)
-    bad = (bad & (scale == scale)).nonzero()
-    if bad.numel():
-        page, head = bad[0].tolist()
-        raise ValueError(f"{name}[{page}, {head}] = {float(scale[page, head])} is no power of two from 2^-126 to 2^120 "
-                         "(nor 0 or NaN, of a page that is not in use)")
+    # A sign, a mantissa, or an exponent above 2^120's, which the largest finite values take.
+    bad = ((bits & -0x7f800001) != 0) | (bits > 247 << 23)
+    bad &= scale == scale
+    if bool(bad.any()):
+        which, page, head = bad.nonzero()[0].tolist()
+        raise ValueError(f"{'kv'[which]}_scale[{page}, {head}] = {float(scale[which, page, head])} is no power of two "
+                         "from 2^-126 to 2^120 (nor 0 or NaN, of a page that is not in use)")
 
 
 class Pages:
@@ -69,8 +71,7 @@ class Pages:
         p = cls.__new__(cls)
         p._set(k, v, k_scale, v_scale)
         if not (k.is_cuda and torch.cuda.is_current_stream_capturing()):
-            _check_scales(k_scale, "k_scale")
-            _check_scales(v_scale, "v_scale")
+            _check_scales(k_scale, v_scale)
         return p
 
     def _set(self, k, v, k_scale, v_scale):
