@@ -337,7 +337,8 @@ int lc_cache_commit(const lc_cache_t* cache, int32_t layers, void* const* ks, vo
  * heads: K as e4m3 codes (OCP: 448 the largest, no infinities) [pages, heads_kv,
  * page_rows, head_dim], V as [pages, heads_kv, head_dim, page_rows], and for each
  * page and head one scale for K and one for V [pages, heads_kv] fp32.  What a code
- * stands for is code * scale; scales are powers of two from 2^-126 on.
+ * stands for is code * scale; scales are powers of two from 2^-126 to 2^120 (others
+ * give wrong values without an error).
  * Row r of sequence b lies in row r % page_rows of page table[b][r / page_rows]
  * (int32 [batch, table_width], device).  An entry outside 0 .. pages - 1, and any
  * row from table_width * page_rows on, is no page: nothing is written there and

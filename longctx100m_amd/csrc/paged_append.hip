@@ -8,10 +8,11 @@
 // it has to, and writes the codes; only if the scale went up does it touch the
 // codes of earlier rows.  Rows behind the new ones stay as they are.  So a row
 // is read once, and a decoded token costs a row's bytes.  8,192 tokens of 32/8 heads
-// of 128 in bf16, queries included, move 185 MB in 45 us (4.1 TB/s): the pages' workgroups
-// load, reduce over their barrier and store, one phase after the other, and the
-// angles are 6 us of instructions.  (Several heads a workgroup, which share the
-// angles, need 40 registers more: 58 us.)
+// of 128 in bf16, queries included, move 185 MB in 43 to 45 us, kernel and call alike (4.1 to
+// 4.3 TB/s; 34.5 where one set of inputs again and again stays in the 256 MB cache): the
+// pages' workgroups load, reduce over their barrier and store, one phase after the
+// other, and the angles are 6 us of instructions.  (Several heads a workgroup, which
+// share the angles, need 40 registers more: 58 us.)
 //
 // Keys are [row][dim] in a page, values [dim][row]: the attention's second
 // product wants 16 consecutive keys of one dim in a lane, and gets them with
@@ -227,8 +228,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
   __shared__ float2 cs[kTurnTokens * kTurnPairs];
   __shared__ float buf[4];
   // The queries first: their workgroups stream, those of the pages mostly wait and
-  // compute, and fill in behind (8,192 tokens of 32/8 heads of 128: 48 us, the pages
-  // first 52.5, both in turn 57.5).
+  // compute, and fill in behind (8,192 tokens of 32/8 heads of 128, compared when the
+  // kernel took 48 us: the pages first 52.5, both in turn 57.5).
   const int q_blocks = gridDim.x - a.kv_blocks;
   if ((int)blockIdx.x >= q_blocks) {
     int x = blockIdx.x - q_blocks;

@@ -10,7 +10,9 @@
 // without any rounding, by one conversion (two values, with the scale) that
 // costs less than the products.  fp32 queries and probabilities go in as three
 // bf16 parts, x = x0 + x1 + x2, which hold all their 24 bits: an fp32 attention
-// at a third of the bf16 rate instead of a sixteenth.
+// at a third of the bf16 rate instead of a sixteenth.  bf16 queries round their
+// probabilities to bf16, by 2^-8 at most each, the sum l not: outputs, which end in
+// bf16, are off by 1.7 to 2.0e-3 instead of the 1.65e-3 of their own rounding.
 //
 //   S^T = K Q^T     A = K, B = Q^T
 //   O^T += V^T P^T  A = V^T, B = P^T, straight from the S^T accumulators
@@ -956,8 +958,10 @@ constexpr int64_t kShort = 16;  // tiles of a sequence that are not split over w
 
 // Many rows go by tiles that a workgroup shares once all blocks of 16 rows together
 // would read more than this, at the tables' width; up to there, and up to kFewRows
-// rows a KV head, each block reads the cache by itself, later ones from L2 (32/8 heads;
-// blocks of 16 against tiles, us).  Of 128: 24 tokens over 2,000 keys (25 MB) 18.4
+// rows a KV head, each block reads the cache by itself.  Later ones read it from L2 where
+// KV heads are a multiple of eight: a head's blocks lie that many workgroups apart, which
+// go to the XCDs in turn.  Measured with 32/8 heads only (blocks of 16 against tiles,
+// us).  Of 128: 24 tokens over 2,000 keys (25 MB) 18.4
 // and 21.4, 64 over 500 (18 MB) 12.7 and 20.6, 64 over 4,000 (133 MB) 27.3 and 31.9, 32
 // over 16,000 (263 MB) 38.5 and 31.8, 256 over 8,000 (1.1 GB) 98 and 63; eight
 // sequences' 64 over 500 (148 MB) 27 and 36, 32 over 2,000 (266 MB) 41 and 33.  Of 64: 64
@@ -969,6 +973,10 @@ constexpr int64_t kFewRows = 48;
 // Query rows from which a wave each is enough for the merge.
 constexpr int64_t kManyRows = 1024;
 
+// Of the tiled form one workgroup runs on a CU, so those beyond 256 wait for a second
+// round, and slots are whole: the time goes in steps.  32/8 heads of 128 behind 16,001:
+// 1,024 tokens (two slots) 331 us, 1,088 488, 1,536 502, 2,048 (256 workgroups) 565, 2,112 956,
+// 3,000 1,003, 4,096 1,127.
 struct Plan {
   bool tiled;
   int rows;  // of a workgroup
@@ -1039,7 +1047,8 @@ hipError_t launch_paged_attn(const PagedProblem& p, const void* q, void* out, fl
   auto launch = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)(x.slots * x.units)), dim3(64 * x.waves), 0, st, a);
   };
-  const bool once = x.units == p.pool.Hkv;  // the cache is read once
+  // The cache is read once: past L2, also what sequences of a common prefix share.
+  const bool once = x.units == p.pool.Hkv;
   auto by_dim = [&](auto parts, auto nt) {
     constexpr int P = decltype(parts)::value;
     constexpr bool NT = decltype(nt)::value;

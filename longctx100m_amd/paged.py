@@ -134,9 +134,10 @@ def append(pages: Pages, table: torch.Tensor, past: torch.Tensor, k: torch.Tenso
            q: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
     """Appends the new tokens' k and v [B, N, Hkv, D] (bf16 or fp32, any strides with
     contiguous D, e.g. columns of a fused projection) to the pages, k rotated to
-    positions past + i by ``rotary``.  With ``q`` [B, N, Hq, D] the tokens' queries are
-    rotated too and returned (``q_out``, contiguous, may be q; padded tokens' rows
-    in it are left alone, and are not written in one made here).
+    positions past + i by ``rotary`` (whose rotary_dim is a multiple of 16 here).  With
+    ``q`` [B, N, Hq, D] the tokens' queries are rotated too and returned (``q_out``,
+    contiguous, may be q; padded tokens' rows in it are left alone, and are not written
+    in one made here).  No gradients: they are lost here.
 
     The pages that new rows lie in must be their sequence's alone.  Their scales
     rise as needed, which rounds codes of earlier rows in them again: to the
