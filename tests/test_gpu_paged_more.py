@@ -100,3 +100,32 @@ def test_a_captured_training_step_of_a_rotation(gpu):
         gpu.cuda.synchronize()
         assert gpu.equal(y, rotary.rotate(x.detach(), at, r))
         assert gpu.equal(dx, rotary.rotate_backward(g, at, r))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_drafts_that_are_taken_back(gpu, dtype):
+    """A past that is lowered: the rows behind it are not seen, the next append writes over
+    them and the rows before stay, also where the drafts raised their page's scale."""
+    import numpy as np
+
+    from longctx100m_amd import paged
+    from oracle import paged as op
+    from tests.test_gpu_paged import _from_pages, _pool, _rows, _to_pages
+    from tests.test_paged_bounds import _attend, _expected, _faults
+
+    rng = np.random.default_rng(21)
+    hkv, d, rows = 2, 64, 16
+    table = np.array([[4, 1, 3], [0, 2, 5]])
+    pool = _pool(rng, 6, rows, hkv, d)
+    p = _to_pages(gpu, pool)
+    for past, n, scale in (([0, 0], 20, 1.0), ([20, 20], 9, 60.0), ([22, 15], 4, 1.0), ([3, 16], 13, 0.1)):
+        k, tk = _rows(gpu, rng, 2, n, hkv, d, dtype, scale)
+        v, tv = _rows(gpu, rng, 2, n, hkv, d, dtype, scale)
+        paged.append(p, _i32(gpu, table), _i32(gpu, past), tk, tv)
+        op.append(pool, table, past, [n] * 2, k, v)
+        got = _from_pages(p)
+        for name in ("k", "v", "k_scale", "v_scale"):
+            assert np.array_equal(got[name], pool[name]), name
+        q, _ = _rows(gpu, rng, 2, n, 4, d, dtype, 1.5)
+        want = _expected(q, pool, table, past, [n] * 2, dtype)
+        assert _faults(_attend(gpu, q, p, table, past, None, dtype), want) == []
